@@ -2301,3 +2301,91 @@ def expert_combine(y, plan: ExpertPlan, weights, x, base=None, base_gate=None) -
                                        gate_ld, gate_col, x.shape[0], top, x.shape[1], _code(x), _stream()))
     return out
 
+
+
+# ----------------------------------------------------------------------------------- #
+# eviction from the paged cache by accumulated attention weight
+
+def _here(what: str, **tensors) -> None:
+    """All of the tensors lie, contiguous, on the current device (whose stream the kernels are launched on)."""
+    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for name, t in tensors.items():
+        if not t.is_cuda:
+            raise KernelError(f"{what}: {name} is not on a CUDA device")
+        if t.get_device() != device:
+            raise KernelError(f"{what}: {name} is on device {t.get_device()}, the current device is {device}")
+        if not t.is_contiguous():
+            raise KernelError(f"{what}: {name} is not contiguous")
+
+
+def _int32(what: str, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32:
+            raise KernelError(f"{what}: {name} is {t.dtype}, {torch.int32} is needed")
+
+
+def _need_tables(what: str, block_table, kv_len) -> int:
+    """The number of requests of a block table [requests, pages] and their lengths."""
+    _int32(what, block_table=block_table, kv_len=kv_len)
+    if block_table.dim() != 2 or block_table.shape[1] < 1 or kv_len.dim() != 1 or kv_len.shape[0] != block_table.shape[0]:
+        raise KernelError(f"{what}: block tables {tuple(block_table.shape)} for lengths {tuple(kv_len.shape)}")
+    return kv_len.shape[0]
+
+
+def choose_kept(mass, block_table, kv_len, budget: int, keep_first: int, keep_last: int, max_kv_len: int) -> torch.Tensor:
+    """Which of a request's keys stay when it has more than `budget`: per kv head the first `keep_first`, the last
+    `keep_last` and of the others those with the largest accumulated attention weight (of equal ones those that stand
+    first; a weight that is no number counts as the largest). `mass` float32 [pages, kv_heads, page_size] lies in the pages
+    of `block_table` [requests, pages], as `paged_attention_mass` leaves it; `kv_len` are the requests' keys, at most `max_kv_len`.
+    Returns int32 [requests, kv_heads, budget]: the kept keys' indices in ascending order. A request with `budget` keys or
+    fewer keeps all; places that are left over hold -1."""
+    seqs = _need_tables("choose_kept", block_table, kv_len)
+    if mass.dtype != torch.float32 or mass.dim() != 3:
+        raise KernelError(f"choose_kept: mass is {mass.dtype} {tuple(mass.shape)}, float32 [pages, kv_heads, page_size] is needed")
+    if budget < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
+        raise KernelError(f"choose_kept: {keep_first} first and {keep_last} last keys of a budget of {budget}")
+    if not 0 <= max_kv_len <= block_table.shape[1] * mass.shape[2]:
+        raise KernelError(f"choose_kept: {max_kv_len} keys for tables of {block_table.shape[1]} pages of {mass.shape[2]}")
+    _here("choose_kept", mass=mass, block_table=block_table, kv_len=kv_len)
+    kept = torch.empty((seqs, mass.shape[1], budget), dtype=torch.int32, device=mass.device)
+    lib = _lib("evict")
+    _set_bounds("evict", mass)
+    _check(lib, lib.pae_choose_kept(kept.data_ptr(), mass.data_ptr(), block_table.data_ptr(), block_table.shape[1], kv_len.data_ptr(), seqs, mass.shape[1],
+                                    mass.shape[2], budget, keep_first, keep_last, max_kv_len, _stream()))
+    return kept
+
+
+def compact_kept(keys, values, mass, block_table, kv_len, kept) -> None:
+    """Moves the rows of the kept keys (`choose_kept`) to the front of their requests' pages, in their order: place i of a
+    request and kv head gets the row of key kept[.., i], of `keys` and `values` [pages, kv_heads, page_size, head size] and of
+    `mass` [pages, kv_heads, page_size] alike. values and mass may be None; values may have another head size, and may be the keys
+    themselves (a latent's pages). A request then has min(kv_len, budget) keys; what lies behind them is left as it was. Rows that
+    stay where they are, such as a shared prefix of at most `keep_first` keys, are not written. The indices ascend in every
+    row, as `choose_kept` leaves them; one that is negative, not below kv_len, or below its place moves nothing."""
+    seqs = _need_tables("compact_kept", block_table, kv_len)
+    _int32("compact_kept", kept=kept)
+    if keys.dim() != 4:
+        raise KernelError(f"compact_kept: keys {tuple(keys.shape)}, [pages, kv_heads, page_size, head size] is needed")
+    pages, kv_heads, page_size, key_dim = keys.shape
+    if kept.dim() != 3 or kept.shape[0] != seqs or kept.shape[1] != kv_heads:
+        raise KernelError(f"compact_kept: kept {tuple(kept.shape)} for {seqs} requests of {kv_heads} kv heads")
+    given = dict(keys=keys, block_table=block_table, kv_len=kv_len, kept=kept)
+    if values is not None and values.data_ptr() == keys.data_ptr() and values.shape == keys.shape:
+        values = None
+    if values is not None:
+        if values.dtype != keys.dtype or values.dim() != 4 or values.shape[:3] != keys.shape[:3]:
+            raise KernelError(f"compact_kept: values {values.dtype} {tuple(values.shape)} beside keys {keys.dtype} {tuple(keys.shape)}")
+        given["values"] = values
+    if mass is not None:
+        if mass.dtype != torch.float32 or mass.shape != keys.shape[:3]:
+            raise KernelError(f"compact_kept: mass {mass.dtype} {tuple(mass.shape)} beside keys {tuple(keys.shape)}")
+        given["mass"] = mass
+    _here("compact_kept", **given)
+    size = keys.element_size()
+    key_bytes, value_bytes = key_dim * size, 0 if values is None else values.shape[3] * size
+    together = key_bytes | value_bytes | keys.data_ptr() | (0 if values is None else values.data_ptr())
+    unit = 16 if together % 16 == 0 else 4 if together % 4 == 0 else 2
+    lib = _lib("evict")
+    _set_bounds("evict", keys)
+    _check(lib, lib.pae_compact_kept(keys.data_ptr(), _ptr(values), _ptr(mass), block_table.data_ptr(), block_table.shape[1], kv_len.data_ptr(),
+                                     kept.data_ptr(), seqs, kv_heads, page_size, kept.shape[2], key_bytes, value_bytes, unit, _stream()))
