@@ -56,6 +56,10 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)_
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// 16 bytes, or zeros where `there` is false.
+__device__ __forceinline__ void cp_async16_or_zeros(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -272,7 +276,8 @@ __device__ __forceinline__ void decode_slice(const DecodeParams& p, uint8_t* min
       const int row = i / (D / 8), c = i % (D / 8);
       const int off = TileLayout<D>::offset_bytes(row, c);
       cp_async16(k_dst + off, p.keys + (row0 + row) * D + c * 8);
-      cp_async16(k_dst + TILE_BYTES + off, p.values + (row0 + row) * D + c * 8);
+      // Zeros behind the last key: the probability 0 times what a page holds there is 0 only for a number.
+      cp_async16_or_zeros(k_dst + TILE_BYTES + off, p.values + (row0 + row) * D + c * 8, key0 + row < end);
     }
   };
 

@@ -115,6 +115,18 @@ __device__ __forceinline__ uint32_t value_step(int k, int rows_a_box) {
   const int row = k * 16;
   return (uint32_t)(row + (D / 64 - 1) * (row & -rows_a_box)) * 128;
 }
+// Rows `from` .. `rows` - 1 of a tile of values become zeros, by a converged warp, before the tensor core reads them: they lie behind the
+// last visible key, and a probability of 0 times what a page holds there is 0 only for a number.
+template <int D>
+__device__ __forceinline__ void clear_values(uint8_t* tile, int from, int rows, int rows_a_box, int lane) {
+  constexpr int CHUNKS = D / 8;
+  for (int i = lane; i < (rows - from) * CHUNKS; i += 32) {
+    const int row = from + i / CHUNKS, chunk = i % CHUNKS;
+    *(uint4*)(tile + ((row / rows_a_box) * (D / 64) + chunk / 8) * rows_a_box * 128 + (row % rows_a_box) * 128 + (chunk % 8) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
 // 32 consecutive float32 columns of this thread's lane of tensor memory.
 __device__ __forceinline__ void tmem_load32(uint32_t address, float* v) {
   uint32_t r[32];
@@ -397,6 +409,8 @@ __global__ void __launch_bounds__(THREADS) prefill_tcgen05_kernel(const __grid_c
         if (t + 1 < n_tiles) issue_scores(t + 1);
         const int st = t & 1;
         ok = ok && mbar_wait_warp(bar(V_FULL, st), (t >> 1) & 1, abort_flag, p.error, 5);
+        if (ok && kv_begin + (t + 1) * BKEYS > kv_end)
+          clear_values<D>(generic_base + L::V_OFFSET + st * L::KV_BYTES, kv_end - kv_begin - t * BKEYS, BKEYS, p.page_size, lane);
         ok = ok && mbar_wait_warp(bar(P_READY, st), (t >> 1) & 1, abort_flag, p.error, 6);
         if (t >= 2) ok = ok && mbar_wait_warp(bar(O_EMPTY, st), ((t >> 1) - 1) & 1, abort_flag, p.error, 7);
         if (!ok) break;
@@ -921,6 +935,8 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_tcgen05_paired_kernel(cons
         if (t + 1 < n_tiles) issue_scores(t + 1);
         const int stage = t % KV_STAGES;
         ok = ok && mbar_wait_warp(bar(V_FULL, stage), (t / KV_STAGES) & 1, abort_flag, p.error, 5);
+        if (ok && kv_begin + (t + 1) * BKEYS > kv_end)
+          clear_values<D>(generic_base + L::V_OFFSET + stage * L::KV_BYTES, kv_end - kv_begin - t * BKEYS, BKEYS, box_rows, lane);
         ok = ok && mbar_wait_warp(bar(P_READY, t & 1), (t >> 1) & 1, abort_flag, p.error, 6);
         if (!ok) break;
         tcgen05_fence_after();
