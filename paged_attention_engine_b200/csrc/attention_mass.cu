@@ -1,0 +1,457 @@
+// The attention weight that a step's queries give to the cached keys, added up per key: what an eviction
+// goes by (evict.cu). Of request b, kv head g and key j
+//
+//   w[b, g, j] = sum over the step's tokens t of b at or behind j, and the query heads h of g, of
+//                exp(s_thj - max_k s_thk) / sum_k exp(s_thk - max_k s_thk),   s = scale q . k
+//   mass[page(b, j), g, place(b, j)] = (j is a key of this step ? 0 : mass) + w,    j >= keep_first
+//
+// in float32 throughout: scores, maxima, sums, weights. Requests that only pad a step (slot -1) add nothing.
+// No atomics: a key's sum is one thread's, in the order of the rows.
+//
+//   slices, merge   steps of single tokens in bfloat16 (head sizes 32, 64, 128): the sliced decode attention of attention_mma.cuh,
+//                   which leaves the scaled scores beside its partial outputs (4 bytes for each query head and key, where the keys and values
+//                   are 4 * head size bytes for each kv head and key), and one kernel that merges the slices and, in further blocks,
+//                   turns the scores into weights once a row's maximum and sum are known.
+//   stats, columns  every other step: the rows' maxima and sums over runs of keys, then per tile of keys the
+//                   weights of all rows that see it, from scores that are computed again. CUDA cores, any type and head size.
+#include "attention_mma.cuh"
+
+using namespace pae;
+using namespace pae_attention;
+
+namespace {
+
+struct MassParams {
+  float* mass;                  // [pages, kv_heads, page_size]
+  const int* block_table;
+  const int* q_start;
+  const int* kv_len;
+  const int* slots;             // [tokens] or null: a request whose first slot is negative pads the step
+  int table_width, heads, kv_heads, page_size, keep_first;
+};
+
+__device__ __forceinline__ bool pads(const MassParams& m, int token) { return m.slots != nullptr && m.slots[token] < 0; }
+
+__device__ __forceinline__ float* mass_of(const MassParams& m, int b, int g, int j) {
+  const int page = checked_page(m.block_table[(size_t)b * m.table_width + checked_table_index(j / m.page_size, m.table_width)]);
+  return m.mass + ((size_t)page * m.kv_heads + g) * m.page_size + j % m.page_size;
+}
+
+// ---------------------------------------------------------------------------------------
+// single tokens, bfloat16
+// ---------------------------------------------------------------------------------------
+// As decode_slices_kernel, which see; the scaled scores (units of log2) go to `scores` [request, head, span].
+template <int D>
+__global__ void __launch_bounds__(SLICE_WARPS * 32) mass_slices_kernel(const DecodeParams p, float* __restrict__ scores, int span) {
+  dependent_launch_trigger();
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slice = blockIdx.x * SLICE_WARPS + warp;
+  const int g = blockIdx.y, b = blockIdx.z;
+  const int token = p.q_start[b], kv_len = p.kv_len[b];
+  const int begin = slice * p.slice_keys, end = min(kv_len, begin + p.slice_keys);
+  const int groups = p.heads / p.kv_heads;
+  if (p.q_start[b + 1] - token != 1 || slice >= p.max_slices || begin >= kv_len) {
+    dependent_launch_wait();
+    return;
+  }
+  const int row_elems = (p.heads + 2 * p.kv_heads) * D;
+  constexpr int TILE_BYTES = TILE_KEYS * D * 2;
+  const uint32_t mine = smem_u32(smem + warp * SLICE_STAGES * 2 * TILE_BYTES);
+  const int* table = p.block_table + (size_t)b * p.table_width;
+  auto fetch = [&](int stage, int key0) {
+    const int page = checked_page(table[checked_table_index(key0 / p.page_size, p.table_width)]);
+    const size_t row0 = ((size_t)page * p.kv_heads + g) * p.page_size + key0 % p.page_size;
+    const uint32_t k_dst = mine + stage * 2 * TILE_BYTES;
+#pragma unroll
+    for (int i = lane; i < TILE_KEYS * D / 8; i += 32) {
+      const int row = i / (D / 8), c = i % (D / 8);
+      const int off = TileLayout<D>::offset_bytes(row, c);
+      cp_async16(k_dst + off, p.keys + (row0 + row) * D + c * 8);
+      cp_async16_or_zeros(k_dst + TILE_BYTES + off, p.values + (row0 + row) * D + c * 8, key0 + row < end);
+    }
+  };
+  const int tiles = (end - begin + TILE_KEYS - 1) / TILE_KEYS;
+  int early = 0;                         // tiles of earlier tokens only are asked for before the wait
+  while (early < SLICE_STAGES - 1 && early < tiles && begin + (early + 1) * TILE_KEYS <= kv_len - 1) {
+    fetch(early, begin + early * TILE_KEYS);
+    cp_async_commit();
+    ++early;
+  }
+  dependent_launch_wait();
+  uint32_t q[D / 16][4];
+  load_query_fragments<D>(q, [&](int r) -> const __nv_bfloat16* {
+    return r < groups ? p.qkv + (size_t)token * row_elems + (size_t)(g * groups + r) * D : nullptr;
+  });
+  for (int i = early; i < SLICE_STAGES - 1; ++i) {
+    if (i < tiles) fetch(i, begin + i * TILE_KEYS);
+    cp_async_commit();
+  }
+  float o[D / 8][4];
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  float row_max[2] = {-FLT_MAX, -FLT_MAX}, row_sum[2] = {0.f, 0.f};
+  float* row_scores = scores + ((size_t)b * p.heads + g * groups + (lane >> 2)) * span + (lane & 3) * 2;
+  for (int t = 0; t < tiles; ++t) {
+    const int ahead = t + SLICE_STAGES - 1;
+    if (ahead < tiles) fetch(ahead % SLICE_STAGES, begin + ahead * TILE_KEYS);
+    cp_async_commit();
+    cp_async_wait<SLICE_STAGES - 1>();
+    __syncwarp();
+    const uint32_t k_tile = mine + (t % SLICE_STAGES) * 2 * TILE_BYTES;
+    const int key0 = begin + t * TILE_KEYS;
+    float s[2][4];
+    scores_16_keys<D>(s, q, k_tile, 0);
+    // The span is a whole number of tiles, so keys behind the last are written too; nobody reads them.
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      if ((lane >> 2) + half * 8 < groups) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *(float2*)(row_scores + (size_t)half * 8 * span + key0 + i * 8) =
+              make_float2(s[i][half * 2] * p.scale_log2, s[i][half * 2 + 1] * p.scale_log2);
+      }
+    uint32_t pa[4];
+    softmax_step<D>(s, row_max, row_sum, o, pa, p.scale_log2, key0 + TILE_KEYS <= end, [&](int, int key) { return key0 + key < end; });
+    accumulate_16_keys<D>(o, pa, k_tile + TILE_BYTES, 0);
+    __syncwarp();
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = (lane >> 2) + half * 8;
+    if (r >= groups) continue;
+    const size_t at = ((size_t)b * p.heads + g * groups + r) * p.max_slices + slice;
+    float* out = p.part_out + at * D;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) *(float2*)(out + n * 8 + (lane & 3) * 2) = make_float2(o[n][half * 2], o[n][half * 2 + 1]);
+    if ((lane & 3) == 0) {
+      p.part_max[at] = row_max[half];
+      p.part_sum[at] = row_sum[half];
+    }
+  }
+}
+
+// Blocks 0 .. heads - 1 of a request merge the slices of a head; the others add the weights of a chunk of one kv head's keys.
+constexpr int MASS_CHUNK = 512;          // keys per block, four a thread
+
+template <int D, int DEPTH>
+__global__ void __launch_bounds__(MERGE_WARPS * 32) mass_merge_kernel(__nv_bfloat16* __restrict__ out, const DecodeParams p, const MassParams m,
+                                                                      const float* __restrict__ scores, int span, int chunks) {
+  dependent_launch_trigger();
+  extern __shared__ float weights[];     // [max_slices], then [MERGE_WARPS][D]
+  __shared__ float top_of[16], inverse_of[16];
+  const int b = blockIdx.y;
+  const int token = p.q_start[b], n_kv = p.kv_len[b];
+  const bool single = p.q_start[b + 1] - token == 1;
+  dependent_launch_wait();
+  if (!single) return;
+  const int slices = min(p.max_slices, (n_kv + p.slice_keys - 1) / p.slice_keys);
+  if ((int)blockIdx.x < p.heads) {
+    const int h = blockIdx.x;
+    const size_t at = ((size_t)b * p.heads + h) * p.max_slices;
+    merge_parts<D, DEPTH>(out + ((size_t)token * p.heads + h) * D, p.part_out + at * D, p.part_max + at, p.part_sum + at, slices, p.max_slices, weights);
+    return;
+  }
+  const int g = ((int)blockIdx.x - p.heads) / chunks, key0 = (((int)blockIdx.x - p.heads) % chunks) * MASS_CHUNK;
+  const int last = min(n_kv, slices * p.slice_keys);
+  if (key0 >= last || key0 + MASS_CHUNK <= m.keep_first || pads(m, token)) return;
+  const int groups = p.heads / p.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < groups; r += MERGE_WARPS) {
+    const size_t at = ((size_t)b * p.heads + g * groups + r) * p.max_slices;
+    float top = -FLT_MAX, total = 0.f;
+    for (int s = lane; s < slices; s += 32) top = fmaxf(top, p.part_max[at + s]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int s = lane; s < slices; s += 32) total += p.part_sum[at + s] * exp2f(p.part_max[at + s] - top);
+    total = warp_sum(total);
+    if (lane == 0) {
+      top_of[r] = top;
+      inverse_of[r] = total > 0.f ? 1.f / total : 0.f;
+    }
+  }
+  __syncthreads();
+  const int j0 = key0 + threadIdx.x * 4;
+  if (j0 >= last) return;
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  const float* from = scores + ((size_t)b * p.heads + g * groups) * span + j0;
+  for (int r = 0; r < groups; ++r) {
+    const float4 s = *(const float4*)(from + (size_t)r * span);
+    const float top = top_of[r], inverse = inverse_of[r];
+    w[0] += exp2f(s.x - top) * inverse;
+    w[1] += exp2f(s.y - top) * inverse;
+    w[2] += exp2f(s.z - top) * inverse;
+    w[3] += exp2f(s.w - top) * inverse;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = j0 + i;
+    if (j < m.keep_first || j >= last) continue;
+    float* to = mass_of(m, b, g, j);
+    *to = (j == n_kv - 1 ? 0.f : *to) + w[i];
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// every other step
+// ---------------------------------------------------------------------------------------
+constexpr int ROWS = 16;                 // (token, head) pairs a tile, four a warp
+constexpr int KEYS = 32;                 // keys a tile, one a lane
+constexpr int THREADS = 128;
+constexpr int MOST_RUNS = 16;            // of keys, that a request's maxima and sums are taken over
+
+template <typename T>
+struct RowParams {
+  MassParams m;
+  const T* qkv;                 // [tokens, (heads + 2 kv_heads) * d]
+  const T* keys;                // [pages, kv_heads, page_size, d]
+  const int* q_pos0;
+  float* part_max;              // [runs, tokens * heads], in units of log2
+  float* part_sum;
+  int d, runs, run_keys, row_tiles;
+  long long rows;               // tokens * heads
+  float scale_log2;
+};
+
+// A tile of rows, row r from row_ptr(r) (null: zeros), as float32 with `stride` floats a row.
+template <typename T, typename RowPtr>
+__device__ __forceinline__ void load_tile(float* tile, int rows, int d, int stride, RowPtr row_ptr) {
+  for (int r = threadIdx.x >> 5; r < rows; r += THREADS / 32) {
+    const T* from = row_ptr(r);
+    for (int i = threadIdx.x & 31; i < d; i += 32) tile[r * stride + i] = from != nullptr ? to_float<T>(from[i]) : 0.f;
+  }
+}
+
+// The scores of this thread's key (its lane) with the four rows of its warp, scaled, in units of log2.
+__device__ __forceinline__ void four_scores(float (&s)[4], const float* q_tile, const float* k_tile, int d, int stride, float scale_log2) {
+  const float* k = k_tile + (threadIdx.x & 31) * stride;
+  const float* q = q_tile + (threadIdx.x >> 5) * 4 * stride;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] = 0.f;
+  for (int c = 0; c < d; ++c) {
+    const float v = k[c];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = fmaf(q[i * stride + c], v, s[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] *= scale_log2;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* key_row(const RowParams<T>& p, int b, int g, int j) {
+  const int page = checked_page(p.m.block_table[(size_t)b * p.m.table_width + checked_table_index(j / p.m.page_size, p.m.table_width)]);
+  return p.keys + (((size_t)page * p.m.kv_heads + g) * p.m.page_size + j % p.m.page_size) * p.d;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) row_stats_kernel(const RowParams<T> p) {
+  extern __shared__ float shared[];
+  dependent_launch_prologue();
+  const int tile = blockIdx.x % p.row_tiles, run = blockIdx.x / p.row_tiles, g = blockIdx.y, b = blockIdx.z;
+  const int groups = p.m.heads / p.m.kv_heads, token0 = p.m.q_start[b];
+  const int count = (p.m.q_start[b + 1] - token0) * groups;
+  const int row0 = tile * ROWS;
+  if (row0 >= count || pads(p.m, token0)) return;
+  const int pos0 = p.q_pos0[b], n = p.m.kv_len[b];
+  const int visible = min(n, pos0 + (min(row0 + ROWS, count) - 1) / groups + 1);        // keys that some row of the tile sees
+  const int begin = run * p.run_keys, end = min(visible, begin + p.run_keys);
+  const int stride = p.d + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* q_tile = shared;
+  float* k_tile = shared + ROWS * stride;
+  load_tile<T>(q_tile, ROWS, p.d, stride, [&](int r) -> const T* {
+    const int i = row0 + r;
+    return i < count ? p.qkv + (size_t)(token0 + i / groups) * (p.m.heads + 2 * p.m.kv_heads) * p.d + (size_t)(g * groups + i % groups) * p.d : nullptr;
+  });
+  float top[4], sum[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    top[i] = -FLT_MAX;
+    sum[i] = 0.f;
+  }
+  for (int key0 = begin; key0 < end; key0 += KEYS) {
+    __syncthreads();
+    load_tile<T>(k_tile, KEYS, p.d, stride, [&](int r) -> const T* { return key0 + r < end ? key_row(p, b, g, key0 + r) : nullptr; });
+    __syncthreads();
+    float s[4];
+    four_scores(s, q_tile, k_tile, p.d, stride, p.scale_log2);
+    const int j = key0 + lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (j >= end || j > pos0 + (row0 + warp * 4 + i) / groups) continue;
+      const float higher = fmaxf(top[i], s[i]);
+      sum[i] = (top[i] == -FLT_MAX ? 0.f : sum[i] * exp2f(top[i] - higher)) + exp2f(s[i] - higher);
+      top[i] = higher;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float both = top[i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) both = fmaxf(both, __shfl_xor_sync(0xffffffffu, both, o));
+    const float total = warp_sum(top[i] == -FLT_MAX ? 0.f : sum[i] * exp2f(top[i] - both));
+    const int r = row0 + warp * 4 + i;
+    if (lane == 0 && r < count) {
+      const size_t at = (size_t)run * p.rows + (size_t)(token0 + r / groups) * p.m.heads + g * groups + r % groups;
+      p.part_max[at] = both;
+      p.part_sum[at] = total;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) column_mass_kernel(const RowParams<T> p) {
+  extern __shared__ float shared[];
+  __shared__ float top_of[ROWS], inverse_of[ROWS], sums[THREADS / 32][KEYS];
+  dependent_launch_prologue();
+  const int g = blockIdx.y, b = blockIdx.z, key0 = blockIdx.x * KEYS;
+  const int groups = p.m.heads / p.m.kv_heads, token0 = p.m.q_start[b];
+  const int tokens = p.m.q_start[b + 1] - token0, count = tokens * groups;
+  const int pos0 = p.q_pos0[b], n = min(p.m.kv_len[b], pos0 + tokens);
+  if (key0 >= n || key0 + KEYS <= p.m.keep_first || tokens < 1 || pads(p.m, token0)) return;
+  const int stride = p.d + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = key0 + lane;
+  float* q_tile = shared;
+  float* k_tile = shared + ROWS * stride;
+  load_tile<T>(k_tile, KEYS, p.d, stride, [&](int r) -> const T* { return key0 + r < n ? key_row(p, b, g, key0 + r) : nullptr; });
+  float sum = 0.f;
+  const int first_row = max(0, key0 - pos0) * groups;            // rows before it see none of the tile
+  for (int row0 = first_row / ROWS * ROWS; row0 < count; row0 += ROWS) {
+    __syncthreads();
+    load_tile<T>(q_tile, ROWS, p.d, stride, [&](int r) -> const T* {
+      const int i = row0 + r;
+      return i < count ? p.qkv + (size_t)(token0 + i / groups) * (p.m.heads + 2 * p.m.kv_heads) * p.d + (size_t)(g * groups + i % groups) * p.d : nullptr;
+    });
+    if (threadIdx.x < ROWS && row0 + (int)threadIdx.x < count) {
+      const int r = row0 + threadIdx.x;
+      const size_t at = (size_t)(token0 + r / groups) * p.m.heads + g * groups + r % groups;
+      // Only the runs that a row's tile reached left something.
+      const int visible = min(p.m.kv_len[b], pos0 + (min(row0 + ROWS, count) - 1) / groups + 1);
+      const int runs = min(p.runs, (visible + p.run_keys - 1) / p.run_keys);
+      float top = -FLT_MAX, total = 0.f;
+      for (int k = 0; k < runs; ++k) top = fmaxf(top, p.part_max[(size_t)k * p.rows + at]);
+      for (int k = 0; k < runs; ++k) total += p.part_sum[(size_t)k * p.rows + at] * exp2f(p.part_max[(size_t)k * p.rows + at] - top);
+      top_of[threadIdx.x] = top;
+      inverse_of[threadIdx.x] = total > 0.f ? 1.f / total : 0.f;
+    }
+    __syncthreads();
+    float s[4];
+    four_scores(s, q_tile, k_tile, p.d, stride, p.scale_log2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = row0 + warp * 4 + i;
+      if (r < count && j <= pos0 + r / groups) sum += exp2f(s[i] - top_of[warp * 4 + i]) * inverse_of[warp * 4 + i];
+    }
+  }
+  sums[warp][lane] = sum;
+  __syncthreads();
+  if (warp == 0 && j >= p.m.keep_first && j < n) {
+    float w = 0.f;
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) w += sums[i][lane];
+    float* to = mass_of(p.m, b, g, j);
+    *to = (j >= pos0 ? 0.f : *to) + w;
+  }
+}
+
+template <int D>
+int launch_decode_mass(const DecodeParams& p, const MassParams& m, __nv_bfloat16* out, float* scores, int span, int seqs, cudaStream_t s) {
+  const size_t bytes = slices_smem_bytes(D);
+  if (int err = allow_smem(mass_slices_kernel<D>, bytes, "paged_attention_mass")) return err;
+  launch_kernel(mass_slices_kernel<D>, dim3((p.max_slices + SLICE_WARPS - 1) / SLICE_WARPS, p.kv_heads, seqs), dim3(SLICE_WARPS * 32), bytes, s, p, scores, span);
+  if (int err = check_launch("paged_attention_mass")) return err;
+  const int chunks = (span + MASS_CHUNK - 1) / MASS_CHUNK;
+  const auto merge = merge_in_few_registers(p.heads, seqs, p.max_slices) ? mass_merge_kernel<D, 8> : mass_merge_kernel<D, MERGE_DEPTH>;
+  launch_kernel(merge, dim3(p.heads + p.kv_heads * chunks, seqs), dim3(MERGE_WARPS * 32), (p.max_slices + MERGE_WARPS * D) * sizeof(float), s, out, p, m, scores,
+                span, chunks);
+  return check_launch("paged_attention_mass");
+}
+
+template <typename T>
+int launch_rows(RowParams<T> p, const void* qkv, const void* keys, int seqs, int max_q_len, int max_kv_len, cudaStream_t s) {
+  p.qkv = (const T*)qkv;
+  p.keys = (const T*)keys;
+  const size_t stats_bytes = (size_t)(ROWS + KEYS) * (p.d + 1) * sizeof(float);
+  static DevicesSet stats_devices, column_devices;
+  if (int err = raise_shared_memory(stats_devices, row_stats_kernel<T>, 200 * 1024, "attention_mass")) return err;
+  if (int err = raise_shared_memory(column_devices, column_mass_kernel<T>, 200 * 1024, "attention_mass")) return err;
+  launch_kernel(row_stats_kernel<T>, dim3(p.row_tiles * p.runs, p.m.kv_heads, seqs), dim3(THREADS), stats_bytes, s, p);
+  if (int err = check_launch("attention_mass")) return err;
+  launch_kernel(column_mass_kernel<T>, dim3((max_kv_len + KEYS - 1) / KEYS, p.m.kv_heads, seqs), dim3(THREADS), stats_bytes, s, p);
+  return check_launch("attention_mass");
+}
+
+int runs_of(int tokens_rows_tiles, int kv_heads, int seqs, int max_kv_len) {
+  const long long blocks = (long long)tokens_rows_tiles * kv_heads * seqs;
+  int runs = 1;
+  while (runs < MOST_RUNS && blocks * runs < 4 * 148 && max_kv_len > runs * 4 * KEYS) runs *= 2;
+  return runs;
+}
+
+}  // namespace
+
+PAE_DEFINE_LAST_ERROR()
+
+// Floats of scratch for a step of single tokens in bfloat16, cut into slices (as pae_paged_attention_decode).
+PAE_EXPORT long long pae_decode_mass_floats(int seqs, int heads, int d, int slice_keys, int max_slices) {
+  return decode_scratch_floats(seqs, heads, d, max_slices) + (long long)seqs * heads * slice_keys * max_slices;
+}
+
+// Requests that bring exactly one token: out as pae_paged_attention_decode without a window, and the weights of their keys. Others are skipped.
+PAE_EXPORT int pae_paged_attention_decode_mass(void* out, const void* qkv, const void* keys, const void* values, float* mass, const int* block_table,
+                                               int table_width, const int* q_start, const int* kv_len, const int* slots, int seqs, int heads, int kv_heads,
+                                               int d, int page_size, float scale, int keep_first, int slice_keys, int max_slices, float* scratch,
+                                               void* stream) {
+  if (seqs == 0) return 0;
+  if (int err = check_sizes("paged_attention_mass", heads, kv_heads, d, page_size, seqs)) return err;
+  if (heads / kv_heads > 16) return fail(2, "paged_attention_mass: %d query heads per kv head are more than 16", heads / kv_heads);
+  if (slice_keys < 16 || slice_keys % 16 || max_slices < 1) return fail(2, "paged_attention_mass: slices of %d keys x %d", slice_keys, max_slices);
+  if ((size_t)(max_slices + MERGE_WARPS * d) * sizeof(float) > 40 * 1024) return fail(2, "paged_attention_mass: %d slices are more than the merge takes", max_slices);
+  if ((uintptr_t)scratch & 15) return fail(2, "paged_attention_mass: the scratch does not start on a 16-byte boundary");
+  DecodeParams p{};
+  p.qkv = (const __nv_bfloat16*)qkv;
+  p.keys = (const __nv_bfloat16*)keys;
+  p.values = (const __nv_bfloat16*)values;
+  p.block_table = block_table;
+  p.q_start = q_start;
+  p.kv_len = kv_len;
+  const size_t rows = (size_t)seqs * heads * max_slices;
+  const int span = slice_keys * max_slices;
+  float* scores = scratch;                                       // rows of a multiple of 16 floats: aligned
+  p.part_out = scratch + (size_t)seqs * heads * span;
+  p.part_max = p.part_out + rows * d;
+  p.part_sum = p.part_max + rows;
+  p.table_width = table_width;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.page_size = page_size;
+  p.slice_keys = slice_keys;
+  p.max_slices = max_slices;
+  p.scale_log2 = scale * LOG2E;
+  const MassParams m = {mass, block_table, q_start, kv_len, slots, table_width, heads, kv_heads, page_size, keep_first};
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (d == 32) return launch_decode_mass<32>(p, m, (__nv_bfloat16*)out, scores, span, seqs, s);
+  if (d == 64) return launch_decode_mass<64>(p, m, (__nv_bfloat16*)out, scores, span, seqs, s);
+  return launch_decode_mass<128>(p, m, (__nv_bfloat16*)out, scores, span, seqs, s);
+}
+
+// Floats of scratch for pae_attention_mass_rows.
+PAE_EXPORT long long pae_attention_mass_floats(int tokens, int heads) { return 2ll * MOST_RUNS * tokens * heads; }
+
+// The weights of any step's keys, whatever its rows, type (0 float32, 1 bfloat16) and head size; the attention's output is not computed.
+PAE_EXPORT int pae_attention_mass_rows(float* mass, const void* qkv, const void* keys, const int* block_table, int table_width, const int* q_start,
+                                       const int* q_pos0, const int* kv_len, const int* slots, int tokens, int seqs, int max_q_len, int max_kv_len, int heads,
+                                       int kv_heads, int d, int page_size, float scale, int keep_first, int dtype, float* scratch, void* stream) {
+  if (seqs == 0 || max_kv_len < 1) return 0;
+  if (kv_heads > 65535 || seqs > 65535) return fail(1, "paged_attention_mass: %d requests of %d kv heads, at most 65535 of each", seqs, kv_heads);
+  if (d < 1 || d > 1024) return fail(2, "paged_attention_mass: head_dim %d is not 1 to 1024", d);
+  const MassParams m = {mass, block_table, q_start, kv_len, slots, table_width, heads, kv_heads, page_size, keep_first};
+  const int groups = heads / kv_heads, row_tiles = (int)(((long long)max_q_len * groups + ROWS - 1) / ROWS);
+  const int runs = runs_of(row_tiles, kv_heads, seqs, max_kv_len);
+  const int run_keys = ((max_kv_len + runs - 1) / runs + KEYS - 1) / KEYS * KEYS;
+  const long long rows = (long long)tokens * heads;
+  float* part_max = scratch;
+  float* part_sum = scratch + (long long)MOST_RUNS * rows;
+  const float scale_log2 = scale * LOG2E;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (dtype == kF32) return launch_rows<float>({m, nullptr, nullptr, q_pos0, part_max, part_sum, d, runs, run_keys, row_tiles, rows, scale_log2}, qkv, keys, seqs, max_q_len, max_kv_len, s);
+  return launch_rows<__nv_bfloat16>({m, nullptr, nullptr, q_pos0, part_max, part_sum, d, runs, run_keys, row_tiles, rows, scale_log2}, qkv, keys, seqs, max_q_len, max_kv_len, s);
+}

@@ -222,12 +222,18 @@ __device__ __forceinline__ void compact_strip(const CompactParams& p, int pool, 
 
 template <typename Unit>
 __global__ void __launch_bounds__(COMPACT_THREADS) compact_kernel(const CompactParams p) {
-  dependent_launch_prologue();
+  // The next kernel is not let go early: an attention that follows directly fetches keys of earlier tokens before it waits for
+  // the kernel before it (common.cuh), and those are what is written here.
+  dependent_launch_wait();
   int strip = blockIdx.x;
-  if (strip < p.strips[0]) return compact_strip<Unit>(p, 0, strip);
-  strip -= p.strips[0];
-  if (strip < p.strips[1]) return compact_strip<Unit>(p, 1, strip);
-  compact_strip<uint32_t>(p, 2, 0);
+  if (strip < p.strips[0]) {
+    compact_strip<Unit>(p, 0, strip);
+  } else if ((strip -= p.strips[0]) < p.strips[1]) {
+    compact_strip<Unit>(p, 1, strip);
+  } else {
+    compact_strip<uint32_t>(p, 2, 0);
+  }
+  __threadfence();
 }
 
 }  // namespace

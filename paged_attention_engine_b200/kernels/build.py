@@ -62,6 +62,7 @@ FAMILIES: dict[str, list[str]] = {
     "gated_delta": ["gated_delta.cu", "attention_mma.cuh", "common.cuh"],
     "post_norm": ["post_norm.cu", "common.cuh"],
     "state_space": ["state_space.cu", "common.cuh"],
+    "attention_mass": ["attention_mass.cu", "attention_mma.cuh", "common.cuh"],
     "evict": ["evict.cu", "common.cuh"],
     "attention_decode_noalloc": [
         "attention_decode_noalloc.cu", "attention_decode_noalloc.h", "attention_mma.cuh", "common.cuh",

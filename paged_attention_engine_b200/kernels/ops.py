@@ -2304,7 +2304,7 @@ def expert_combine(y, plan: ExpertPlan, weights, x, base=None, base_gate=None) -
 
 
 # ----------------------------------------------------------------------------------- #
-# eviction from the paged cache by accumulated attention weight
+# attention over the paged cache that adds up its weights per key, and eviction by them
 
 def _here(what: str, **tensors) -> None:
     """All of the tensors lie, contiguous, on the current device (whose stream the kernels are launched on)."""
@@ -2330,6 +2330,74 @@ def _need_tables(what: str, block_table, kv_len) -> int:
     if block_table.dim() != 2 or block_table.shape[1] < 1 or kv_len.dim() != 1 or kv_len.shape[0] != block_table.shape[0]:
         raise KernelError(f"{what}: block tables {tuple(block_table.shape)} for lengths {tuple(kv_len.shape)}")
     return kv_len.shape[0]
+
+
+def _need_attention(what: str, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads: int, num_kv_heads: int, head_dim: int,
+                    page_size: int) -> int:
+    """What an attention of a step over the paged cache is given: the number of its requests."""
+    _code(qkv)
+    seqs = _need_tables(what, block_table, kv_len)
+    _int32(what, q_start=q_start, q_pos0=q_pos0)
+    if num_kv_heads < 1 or num_heads < num_kv_heads or num_heads % num_kv_heads:
+        raise KernelError(f"{what}: {num_heads} heads over {num_kv_heads} kv heads")
+    if qkv.dim() != 2 or qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim:
+        raise KernelError(f"{what}: qkv {tuple(qkv.shape)} for {num_heads}+2x{num_kv_heads} heads of {head_dim}")
+    shape = (keys.shape[0], num_kv_heads, page_size, head_dim)
+    for name, t in (("keys", keys), ("values", values)):
+        if t.dtype != qkv.dtype or t.shape != shape:
+            raise KernelError(f"{what}: {name} {t.dtype} {tuple(t.shape)}, {qkv.dtype} [pages, {num_kv_heads}, {page_size}, {head_dim}] is needed")
+    if q_start.shape != (seqs + 1,) or q_pos0.shape != (seqs,):
+        raise KernelError(f"{what}: q_start {tuple(q_start.shape)} and q_pos0 {tuple(q_pos0.shape)} for {seqs} requests")
+    return seqs
+
+
+def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, num_heads: int, num_kv_heads: int, head_dim: int,
+                         page_size: int, max_q_len: int, max_kv_len: int, scale: float, keep_first: int = 0, slots=None, num_single=None,
+                         multi_index=None) -> torch.Tensor:
+    """`paged_attention` without a window, which also adds up what weight the step's queries gave each key: mass[page, g, place]
+    += the sum over the step's tokens that see the key, and over the query heads of kv head g, of the key's softmax weight.
+    `mass` is float32 [pages, kv_heads, page_size], in the pages of the keys. A key of this step starts from nothing, whatever its place held
+    before. Keys before `keep_first` are left alone (they are not to be evicted): requests may share
+    the pages that hold such keys only; every other page belongs to one request of the step. `slots` (int32 [tokens], as
+    `qkv_projection` takes them): a request whose first slot is negative only pads the step and adds nothing."""
+    qkv = materialized(qkv)
+    seqs = _need_attention("paged_attention_mass", qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size)
+    tokens = qkv.shape[0]
+    if mass.dtype != torch.float32 or mass.shape != keys.shape[:3]:
+        raise KernelError(f"paged_attention_mass: mass {mass.dtype} {tuple(mass.shape)} beside keys {tuple(keys.shape)}")
+    if keep_first < 0:
+        raise KernelError(f"paged_attention_mass: {keep_first} first keys")
+    if not 0 <= max_kv_len <= block_table.shape[1] * page_size:
+        raise KernelError(f"paged_attention_mass: {max_kv_len} keys for tables of {block_table.shape[1]} pages of {page_size}")
+    given = dict(qkv=qkv, keys=keys, values=values, mass=mass, block_table=block_table, q_start=q_start, q_pos0=q_pos0, kv_len=kv_len)
+    if slots is not None:
+        _int32("paged_attention_mass", slots=slots)
+        if slots.shape != (tokens,):
+            raise KernelError(f"paged_attention_mass: slots {tuple(slots.shape)} for {tokens} tokens")
+        given["slots"] = slots
+    _here("paged_attention_mass", **given)
+    if max_q_len == 1 and max_kv_len > 0 and plain_attention_takes(num_heads, num_kv_heads, head_dim, page_size, qkv.dtype):
+        plain, lib = _lib("attention_mma"), _lib("attention_mass")
+        slice_keys, max_slices = decode_slicing(seqs, num_kv_heads, max_kv_len, wave_blocks=plain.pae_decode_blocks_per_wave(head_dim),
+                                                slices_per_block=plain.pae_decode_slices_per_block())
+        out = torch.empty((tokens, num_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+        scratch = torch.empty(lib.pae_decode_mass_floats(seqs, num_heads, head_dim, slice_keys, max_slices), dtype=torch.float32, device=qkv.device)
+        _set_bounds("attention_mass", keys)
+        _check(lib, lib.pae_paged_attention_decode_mass(
+            out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), mass.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
+            kv_len.data_ptr(), _ptr(slots), seqs, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices, scratch.data_ptr(),
+            _stream()), 2)
+        return out
+    out = paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_kv_len, scale,
+                          0, num_single=num_single, multi_index=multi_index)
+    lib = _lib("attention_mass")
+    scratch = torch.empty(lib.pae_attention_mass_floats(tokens, num_heads), dtype=torch.float32, device=qkv.device)
+    _set_bounds("attention_mass", keys)
+    _check(lib, lib.pae_attention_mass_rows(
+        mass.data_ptr(), qkv.data_ptr(), keys.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(),
+        _ptr(slots), tokens, seqs, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, _code(qkv), scratch.data_ptr(),
+        _stream()), 2)
+    return out
 
 
 def choose_kept(mass, block_table, kv_len, budget: int, keep_first: int, keep_last: int, max_kv_len: int) -> torch.Tensor:
