@@ -1,0 +1,659 @@
+// Attention of a step whose requests share the first keys of their contexts: groups of consecutive requests, each group with one run of
+// shared keys that lies once in the pages, and behind it every request's own keys.
+//
+//   out[t, h] = (sum over shared keys j of e_j v_j + sum over own keys j <= position(t) of e_j v_j) / (sum of all e_j),
+//   e_j = exp(scale q . k_j - m), m the largest of the row's scaled scores
+//
+// A softmax over two sets of keys is the two sets' (maximum, sum, unnormalised output) brought to one maximum and added, so the
+// shared keys are taken for all rows (token, query head of the kv head) of a group at once: they are read once a
+// group and not once a request, and there are enough rows to fill the tensor cores. One launch of blocks of two kinds, and a merge:
+//
+//   shared   128 rows x a slice of the shared keys, 64 keys a tile, as the paired prefill attention works (attention_tcgen05.cu), which see for
+//            the roles and the references that may lie behind the maxima: keys and values by TMA, both products as tcgen05.mma, scores,
+//            probabilities and output in tensor memory. There is no mask but for the slice's last tile: every query stands behind the shared keys.
+//   own      six warps, each 16 rows of one request x a slice of its own keys, 16 keys a tile by mma.sync, as the sliced decode attention works
+//            (attention_mma.cuh). These blocks wait for memory while the others compute.
+//   merge    a row's slices, shared and own, in their order.
+//
+// Scores are scaled in float32, maxima, sums and outputs are float32; probabilities are rounded to bfloat16 for the second
+// product, as the value operand is, and the result once. Every wait on an mbarrier is bounded and reports through `error`.
+#include <cfloat>
+
+#include "attention_mma.cuh"
+#include "attention_pages.cuh"
+
+using namespace pae;
+using namespace pae_tcgen05;
+using pae_attention::TILE_KEYS;
+using pae_attention::TileLayout;
+
+namespace {
+
+constexpr int ROWS = 128;                // of a shared block
+constexpr int BKEYS = 64;                // keys per tile of a shared block
+constexpr int THREADS = 192;             // TMA warp, MMA warp, four softmax warps; or six warps with a slice each
+constexpr int SOFTMAX_WARPS = 4;
+constexpr int KV_STAGES = 2;
+constexpr int OWN_WARPS = THREADS / 32;
+constexpr int OWN_STAGES = 2;
+constexpr int OWN_ROWS = 16;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float REFERENCE_SLACK = 8.f;   // as the paired prefill attention
+constexpr float REFERENCE_LIMIT = 256.f;
+
+struct Params {
+  const __nv_bfloat16* qkv;     // [tokens, heads + 2 kv_heads, D]
+  const __nv_bfloat16* keys;    // [pages, kv_heads, page_size, D]
+  const __nv_bfloat16* values;
+  const int* block_table;
+  const int* q_start;
+  const int* q_pos0;
+  const int* kv_len;
+  const int* prefix_len;        // [requests], alike in a group
+  const int* group_start;       // [groups + 1]
+  float* part_out;              // [tokens, heads, slots, D]
+  float* part_max;              // [tokens, heads, slots], units of log2
+  float* part_sum;
+  int table_width, heads, kv_heads, page_size, max_prefix;
+  int shared_blocks, row_tiles, shared_slices, shared_keys;      // keys per slice of the shared ones, a multiple of BKEYS
+  int own_units, own_row_tiles, own_slices, own_keys;            // likewise of the own ones, a multiple of TILE_KEYS
+  int slots;                    // slices of a row at most: shared ones, then own ones
+  float scale_log2, slack;
+  int* error;
+};
+
+template <int D>
+struct Layout {
+  static constexpr int HALVES = D / 64;
+  static constexpr int Q_HALF_BYTES = ROWS * 128;
+  static constexpr int KV_HALF_BYTES = BKEYS * 128;
+  static constexpr int Q_BYTES = HALVES * Q_HALF_BYTES;
+  static constexpr int KV_BYTES = HALVES * KV_HALF_BYTES;
+  static constexpr int Q_OFFSET = 0;
+  static constexpr int K_OFFSET = Q_BYTES;
+  static constexpr int V_OFFSET = K_OFFSET + KV_STAGES * KV_BYTES;
+  static constexpr int BAR_OFFSET = V_OFFSET + KV_STAGES * KV_BYTES;
+  static constexpr size_t SMEM_BYTES = (size_t)BAR_OFFSET + 256 + 768;     // 768 for the 1024-byte alignment of the tiles: two blocks fit an SM
+  static constexpr int S_COLUMNS = BKEYS;
+  static constexpr int O_COLUMN = 2 * S_COLUMNS;
+  static constexpr int TMEM_COLUMNS = 256;
+  static constexpr int OWN_BYTES = OWN_STAGES * 2 * TILE_KEYS * D * 2;     // of a warp
+  static_assert(OWN_WARPS * OWN_BYTES <= BAR_OFFSET, "the six warps' stages lie where the tiles of the other kind do");
+};
+
+enum Bar : int {
+  Q_FULL = 0, O_FULL = 1, S_FULL = 2, P_READY = 4, O_REST = 6,
+  K_FULL = 7, K_EMPTY = K_FULL + KV_STAGES, V_FULL = K_EMPTY + KV_STAGES, V_EMPTY = V_FULL + KV_STAGES, NUM_BARS = V_EMPTY + KV_STAGES
+};
+
+// ---------------------------------------------------------------------------------------
+// the shared keys
+// ---------------------------------------------------------------------------------------
+template <int D>
+__device__ __forceinline__ void shared_slice(const PageMaps& maps, const Params& p, uint8_t* raw_smem) {
+  using L = Layout<D>;
+  const uint32_t raw = smem_u32(raw_smem);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* generic_base = raw_smem + (base - raw);
+  const uint32_t bars = base + L::BAR_OFFSET;
+  volatile uint32_t* tmem_holder = (volatile uint32_t*)(generic_base + L::BAR_OFFSET + 8 * NUM_BARS);
+  volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
+  auto bar = [&](int which, int i = 0) { return bars + 8u * (which + i); };
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+
+  // What this block works on: the row tiles of a kv head and a slice are neighbours, they read the same keys.
+  int index = blockIdx.x;
+  const int row_tile = index % p.row_tiles;
+  index /= p.row_tiles;
+  const int g = index % p.kv_heads;
+  index /= p.kv_heads;
+  const int slice = index % p.shared_slices, group = index / p.shared_slices;
+  const int b = p.group_start[group], b_end = p.group_start[group + 1];
+  const int groups = p.heads / p.kv_heads;
+  int first_token = 0, rows = 0, kv_end = 0;
+  const int kv_begin = slice * p.shared_keys;
+  if (b < b_end) {
+    first_token = p.q_start[b];
+    rows = min(ROWS, (p.q_start[b_end] - first_token) * groups - row_tile * ROWS);
+    kv_end = min(min(p.prefix_len[b], p.max_prefix), kv_begin + p.shared_keys);
+  }
+  if (rows <= 0 || kv_begin >= kv_end) {               // the same in every thread
+    dependent_launch_trigger();
+    dependent_launch_wait();
+    return;
+  }
+  const int n_tiles = (kv_end - kv_begin + BKEYS - 1) / BKEYS;
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar(Q_FULL), SOFTMAX_WARPS * 32);
+    for (int i = 0; i < KV_STAGES; ++i) {
+      mbar_init(bar(K_FULL, i), 1);
+      mbar_init(bar(K_EMPTY, i), 1);
+      mbar_init(bar(V_FULL, i), 1);
+      mbar_init(bar(V_EMPTY, i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(S_FULL, i), 1);
+      mbar_init(bar(P_READY, i), SOFTMAX_WARPS);
+    }
+    mbar_init(bar(O_REST), 1);
+    mbar_init(bar(O_FULL), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32((const void*)tmem_holder), L::TMEM_COLUMNS);
+    tmem_relinquish();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  dependent_launch_trigger();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  const int box_rows = min(p.page_size, BKEYS);
+  dependent_launch_wait();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer: lane i brings box i of a tile
+    const int* table = p.block_table + (size_t)b * p.table_width;
+    const bool mine = lane < BKEYS / box_rows;
+    const int last_page = (kv_end - 1) / p.page_size, page_shift = 31 - __clz(p.page_size);
+    // Rows of a tile behind the last shared key are masked: any page will do, the last is taken.
+    auto page_of = [&](int t) {
+      const int key = kv_begin + t * BKEYS + lane * box_rows;
+      return mine && t < n_tiles ? checked_page(table[checked_table_index(min(key >> page_shift, last_page), p.table_width)]) : 0;
+    };
+    auto load = [&](bool values, int t, int page) {
+      const int stage = t % KV_STAGES;
+      const uint32_t full = bar(values ? V_FULL : K_FULL, stage);
+      if (t >= KV_STAGES && !mbar_wait_warp(bar(values ? V_EMPTY : K_EMPTY, stage), (t / KV_STAGES - 1) & 1, abort_flag, p.error, values ? 10 : 1))
+        return false;
+      if (lane == 0) mbar_expect_tx(full, L::KV_BYTES);
+      __syncwarp();
+      load_pages<D>(maps, values, base + (values ? L::V_OFFSET : L::K_OFFSET) + stage * L::KV_BYTES, full, BKEYS, box_rows, lane, g, page,
+                    (kv_begin + t * BKEYS + lane * box_rows) & (p.page_size - 1));
+      return true;
+    };
+    int page0 = page_of(0), page1 = page_of(1), page2 = page_of(2);               // of tiles t, t + 1, t + 2
+    bool ok = load(false, 0, page0);
+    int keys_issued = 1, values_issued = 0;
+    if (n_tiles > 1) {
+      ok = ok && load(false, 1, page1);
+      keys_issued = 2;
+    }
+    for (int t = 0; t < n_tiles && ok; ++t) {
+      const int page3 = page_of(t + 3);
+      if (!(ok = load(true, t, page0))) break;
+      values_issued = t + 1;
+      if (t + 2 < n_tiles) {
+        if (!(ok = load(false, t + 2, page2))) break;
+        keys_issued = t + 3;
+      }
+      page0 = page1;
+      page1 = page2;
+      page2 = page3;
+    }
+    if (lane == 0 && *abort_flag) {      // copies that were issued still write into this block's shared memory
+      for (int t = max(0, keys_issued - KV_STAGES); t < keys_issued; ++t)
+        for (uint32_t w = 0; w < WAIT_LIMIT && !mbar_try_wait(bar(K_FULL, t % KV_STAGES), (t / KV_STAGES) & 1); ++w) __nanosleep(64);
+      for (int t = max(0, values_issued - KV_STAGES); t < values_issued; ++t)
+        for (uint32_t w = 0; w < WAIT_LIMIT && !mbar_try_wait(bar(V_FULL, t % KV_STAGES), (t / KV_STAGES) & 1); ++w) __nanosleep(64);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    const bool leader = elect_one();
+    constexpr uint32_t idesc_s = instruction_descriptor(ROWS, BKEYS, false);
+    constexpr uint32_t idesc_o = instruction_descriptor(ROWS, D, true);
+    const uint64_t q_first = smem_descriptor(base + L::Q_OFFSET), k_first = smem_descriptor(base + L::K_OFFSET);
+    const uint64_t v_first = mn_major_descriptor(base + L::V_OFFSET, box_rows * 128);
+    bool ok = mbar_wait_warp(bar(Q_FULL), 0, abort_flag, p.error, 2);
+    auto issue_scores = [&](int t) {
+      const int st = t & 1, stage = t % KV_STAGES;
+      ok = ok && mbar_wait_warp(bar(K_FULL, stage), (t / KV_STAGES) & 1, abort_flag, p.error, 3);
+      // These scores go where the probabilities of tile t - 2 lay.
+      if (t >= 2) ok = ok && mbar_wait_warp(bar(O_REST), (t - 2) & 1, abort_flag, p.error, 4);
+      if (!ok) return;
+      tcgen05_fence_after();
+      const uint64_t keys = further(k_first, stage * L::KV_BYTES);
+      if (leader) {
+#pragma unroll
+        for (int half = 0; half < L::HALVES; ++half)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16(tmem_base + st * L::S_COLUMNS, further(q_first, half * L::Q_HALF_BYTES + k * 32),
+                      further(keys, half * L::KV_HALF_BYTES + k * 32), idesc_s, (half > 0 || k > 0) ? 1u : 0u);
+        tcgen05_commit(bar(S_FULL, st));
+        tcgen05_commit(bar(K_EMPTY, stage));
+      }
+      __syncwarp();
+    };
+    issue_scores(0);
+    for (int t = 0; t < n_tiles && ok; ++t) {
+      if (t + 1 < n_tiles) issue_scores(t + 1);
+      const int stage = t % KV_STAGES;
+      ok = ok && mbar_wait_warp(bar(V_FULL, stage), (t / KV_STAGES) & 1, abort_flag, p.error, 5);
+      if (ok && kv_begin + (t + 1) * BKEYS > kv_end)
+        clear_values<D>(generic_base + L::V_OFFSET + stage * L::KV_BYTES, kv_end - kv_begin - t * BKEYS, BKEYS, box_rows, lane);
+      ok = ok && mbar_wait_warp(bar(P_READY, t & 1), (t >> 1) & 1, abort_flag, p.error, 6);
+      if (!ok) break;
+      tcgen05_fence_after();
+      const uint64_t values = further(v_first, stage * L::KV_BYTES);
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < BKEYS / 16; ++k)
+          umma_bf16_tmem_a(tmem_base + L::O_COLUMN, tmem_base + (t & 1) * L::S_COLUMNS + k * 8, further(values, value_step<D>(k, box_rows)), idesc_o,
+                           (t > 0 || k > 0) ? 1u : 0u);
+        tcgen05_commit(bar(O_REST));
+        tcgen05_commit(bar(V_EMPTY, stage));
+        if (t + 1 == n_tiles) tcgen05_commit(bar(O_FULL));
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax, one thread per row
+    const int quadrant = warp & 3;
+    const int r = quadrant * 32 + lane;                       // row of the tile, lane of tensor memory
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quadrant * 32) << 16);
+    const int row = row_tile * ROWS + r;                      // of the group
+    const size_t token = (size_t)(first_token + row / groups);
+    const int head = g * groups + row % groups;
+    {
+      // The thread brings its row's query into the operand's swizzled layout; rows behind the last are zeros.
+      const uint4* from = (const uint4*)(p.qkv + (token * (p.heads + 2 * p.kv_heads) + head) * D);
+      uint8_t* to = generic_base + L::Q_OFFSET + r * 128;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c)
+        *(uint4*)(to + (c >> 3) * L::Q_HALF_BYTES + (((c & 7) ^ (r & 7)) << 4)) = r < rows ? from[c] : make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(bar(Q_FULL));
+    }
+    float reference = -FLT_MAX, row_sum = 0.f;                // the reference in units of log2, scaled
+    bool ok = true;
+    for (int t = 0; t < n_tiles; ++t) {
+      const int st = t & 1;
+      ok = ok && mbar_wait(bar(S_FULL, st), (t >> 1) & 1, abort_flag, p.error, 8);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tcgen05_fence_after();
+      const int visible = kv_end - kv_begin - t * BKEYS;      // of the tile; below BKEYS in a slice's last tile only
+      uint32_t packed[BKEYS / 2];
+      uint64_t sum01, sum23, factor2, offset2;
+      auto begin = [&] {
+        const float offset = reference != -FLT_MAX ? -reference : 0.f;     // without one all scores are -infinity or no number: 0 or no number
+        factor2 = pack2(p.scale_log2, p.scale_log2);
+        offset2 = pack2(offset, offset);
+        sum01 = sum23 = 0;
+      };
+      auto take = [&](const float* s, int i, auto counts) {   // s: the scores of keys i .. i + 3
+        float e[4];
+        unpack2(fma2(pack2(s[0], s[1]), factor2, offset2), e[0], e[1]);
+        unpack2(fma2(pack2(s[2], s[3]), factor2, offset2), e[2], e[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = counts(i + j) ? fast_exp2(e[j]) : 0.f;
+        sum01 = add2(sum01, pack2(e[0], e[1]));
+        sum23 = add2(sum23, pack2(e[2], e[3]));
+        const __nv_bfloat162 h01 = __floats2bfloat162_rn(e[0], e[1]), h23 = __floats2bfloat162_rn(e[2], e[3]);
+        packed[i / 2] = *(const uint32_t*)&h01;
+        packed[i / 2 + 1] = *(const uint32_t*)&h23;
+      };
+      auto take32 = [&](const float* s, int first) {
+        if (visible >= BKEYS) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) take(s + i, first + i, [](int) { return true; });
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) take(s + i, first + i, [&](int key) { return key < visible; });
+        }
+      };
+      auto tile_sum = [&] {
+        float sums[4];
+        unpack2(sum01, sums[0], sums[1]);
+        unpack2(sum23, sums[2], sums[3]);
+        return (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      };
+      const uint32_t scores = lane_base + st * L::S_COLUMNS;
+      bool taken = false;
+      float slack = p.slack;
+      if (p.slack > 0.f && !__any_sync(0xffffffffu, reference == -FLT_MAX)) {
+        // Against the references as they are; should a sum come out above REFERENCE_LIMIT (or not a number), the tile is taken again below.
+        float s[32], behind[32];
+        tmem_ask32(scores, s);
+        tmem_arrived(s);
+        tmem_ask32(scores + 32, behind);
+        begin();
+        take32(s, 0);
+        tmem_arrived(behind);
+        take32(behind, 32);
+        const float sum = tile_sum();
+        taken = __all_sync(0xffffffffu, sum <= REFERENCE_LIMIT);
+        if (taken) row_sum += sum;
+        else slack = 0.f;
+      }
+      if (!taken) {
+        float s[BKEYS];
+        tmem_load64(scores, s);
+        float m4[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX};
+#pragma unroll
+        for (int i = 0; i < BKEYS; ++i) m4[i & 3] = fmaxf(m4[i & 3], i < visible ? s[i] : -FLT_MAX);
+        float tile_max = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        if (tile_max != -FLT_MAX) tile_max *= p.scale_log2;        // the scale is positive: max(s) scales with it
+        const bool moves = tile_max > reference + slack || (reference == -FLT_MAX && tile_max != -FLT_MAX);
+        if (__any_sync(0xffffffffu, moves)) {
+          const float shrink = !moves ? 1.f : (reference == -FLT_MAX ? 0.f : fast_exp2(reference - tile_max));
+          if (moves) {
+            reference = tile_max;
+            row_sum *= shrink;
+          }
+          if (t >= 1) {
+            ok = mbar_wait(bar(O_REST), (t - 1) & 1, abort_flag, p.error, 7);      // the product of the tile before has completed
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tcgen05_fence_after();
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              float o[32];
+              uint32_t back[32];
+              tmem_load32(lane_base + L::O_COLUMN + c, o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) back[i] = __float_as_uint(o[i] * shrink);
+              tmem_store32(lane_base + L::O_COLUMN + c, back);
+            }
+          }
+        }
+        begin();
+        take32(s, 0);
+        take32(s + 32, 32);
+        row_sum += tile_sum();
+      }
+      tmem_store32(scores, packed);      // over the scores, which are in registers
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(P_READY, st));
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      ok = mbar_wait(bar(O_FULL), 0, abort_flag, p.error, 9);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        tcgen05_fence_after();
+        const size_t at = (token * p.heads + head) * p.slots + slice;
+        float* out = p.part_out + at * D;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tmem_load32(lane_base + L::O_COLUMN + c, o);        // every lane takes part
+          if (r < rows) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) *(float4*)(out + c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+        }
+        if (r < rows) {
+          p.part_max[at] = reference;
+          p.part_sum[at] = row_sum;
+        }
+      }
+    }
+  }
+
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem_base, L::TMEM_COLUMNS);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// the own keys
+// ---------------------------------------------------------------------------------------
+// Where the own keys of a tile of OWN_ROWS rows begin and end: its slices start at `base`.
+struct OwnSpan {
+  int first, base, end;
+};
+__device__ __forceinline__ OwnSpan own_span(int shared, int kv_len, int pos0, int tokens, int groups, int row_tile) {
+  OwnSpan s;
+  s.first = shared;
+  s.base = shared / TILE_KEYS * TILE_KEYS;
+  s.end = min(kv_len, pos0 + min((row_tile * OWN_ROWS + OWN_ROWS - 1) / groups, tokens - 1) + 1);
+  return s;
+}
+
+template <int D>
+__device__ __forceinline__ void own_slice(const Params& p, uint8_t* smem) {
+  using namespace pae_attention;
+  dependent_launch_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int unit = ((int)blockIdx.x - p.shared_blocks) * OWN_WARPS + warp;
+  const int slice = unit % p.own_slices;
+  int rest = unit / p.own_slices;
+  const int row_tile = rest % p.own_row_tiles;
+  rest /= p.own_row_tiles;
+  const int g = rest % p.kv_heads, b = rest / p.kv_heads;
+  const int groups = p.heads / p.kv_heads;
+  int token0 = 0, tokens = 0, pos0 = 0, shared = 0;
+  OwnSpan span = {0, 0, 0};
+  if (unit < p.own_units) {
+    token0 = p.q_start[b];
+    tokens = p.q_start[b + 1] - token0;
+    pos0 = p.q_pos0[b];
+    shared = min(p.prefix_len[b], p.max_prefix);
+    span = own_span(shared, p.kv_len[b], pos0, tokens, groups, row_tile);
+  }
+  const int begin = span.base + slice * p.own_keys, end = min(span.end, begin + p.own_keys);
+  if (unit >= p.own_units || row_tile * OWN_ROWS >= tokens * groups || span.end <= span.first || begin >= end) {
+    dependent_launch_wait();
+    return;
+  }
+  constexpr int TILE_BYTES = TILE_KEYS * D * 2;
+  const uint32_t mine = pae_attention::smem_u32(smem + warp * Layout<D>::OWN_BYTES);
+  const int* table = p.block_table + (size_t)b * p.table_width;
+  auto fetch = [&](int stage, int key0) {
+    const int page = checked_page(table[checked_table_index(key0 / p.page_size, p.table_width)]);
+    const size_t row0 = ((size_t)page * p.kv_heads + g) * p.page_size + key0 % p.page_size;
+    const uint32_t k_dst = mine + stage * 2 * TILE_BYTES;
+#pragma unroll
+    for (int i = lane; i < TILE_KEYS * D / 8; i += 32) {
+      const int row = i / (D / 8), c = i % (D / 8);
+      const int off = TileLayout<D>::offset_bytes(row, c);
+      cp_async16(k_dst + off, p.keys + (row0 + row) * D + c * 8);
+      cp_async16_or_zeros(k_dst + TILE_BYTES + off, p.values + (row0 + row) * D + c * 8, key0 + row >= span.first && key0 + row < end);
+    }
+  };
+  const int tiles = (end - begin + TILE_KEYS - 1) / TILE_KEYS;
+  // Tiles of earlier tokens only are asked for before the wait for the kernel before.
+  int early = 0;
+  while (early < OWN_STAGES - 1 && early < tiles && begin + (early + 1) * TILE_KEYS <= pos0) {
+    fetch(early, begin + early * TILE_KEYS);
+    cp_async_commit();
+    ++early;
+  }
+  dependent_launch_wait();
+  const int row0 = row_tile * OWN_ROWS, rows = min(OWN_ROWS, tokens * groups - row0);
+  auto token_of = [&](int r) { return (row0 + r) / groups; };
+  auto head_of = [&](int r) { return g * groups + (row0 + r) % groups; };
+  uint32_t q[D / 16][4];
+  load_query_fragments<D>(q, [&](int r) -> const __nv_bfloat16* {
+    return r < rows ? p.qkv + ((size_t)(token0 + token_of(r)) * (p.heads + 2 * p.kv_heads) + head_of(r)) * D : nullptr;
+  });
+  for (int i = early; i < OWN_STAGES - 1; ++i) {
+    if (i < tiles) fetch(i, begin + i * TILE_KEYS);
+    cp_async_commit();
+  }
+  float o[D / 8][4];
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  float row_max[2] = {-FLT_MAX, -FLT_MAX}, row_sum[2] = {0.f, 0.f};
+  int row_end[2];                            // the keys before it are visible to the row
+#pragma unroll
+  for (int half = 0; half < 2; ++half) row_end[half] = min(end, pos0 + token_of((lane >> 2) + half * 8) + 1);
+  const int all_see = min(end, pos0 + token_of(0) + 1);
+  for (int t = 0; t < tiles; ++t) {
+    const int ahead = t + OWN_STAGES - 1;
+    if (ahead < tiles) fetch(ahead % OWN_STAGES, begin + ahead * TILE_KEYS);
+    cp_async_commit();
+    cp_async_wait<OWN_STAGES - 1>();
+    __syncwarp();
+    const uint32_t k_tile = mine + (t % OWN_STAGES) * 2 * TILE_BYTES;
+    const int key0 = begin + t * TILE_KEYS;
+    float s[2][4];
+    scores_16_keys<D>(s, q, k_tile, 0);
+    uint32_t pa[4];
+    softmax_step<D>(s, row_max, row_sum, o, pa, p.scale_log2, key0 >= span.first && key0 + TILE_KEYS <= all_see,
+                    [&](int half, int key) { return key0 + key >= span.first && key0 + key < row_end[half]; });
+    accumulate_16_keys<D>(o, pa, k_tile + TILE_BYTES, 0);
+    __syncwarp();
+  }
+  cp_async_wait<0>();
+  const int slot = (shared + p.shared_keys - 1) / p.shared_keys + slice;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = (lane >> 2) + half * 8;
+    if (r >= rows) continue;
+    const size_t at = ((size_t)(token0 + token_of(r)) * p.heads + head_of(r)) * p.slots + slot;
+    float* out = p.part_out + at * D;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) *(float2*)(out + n * 8 + (lane & 3) * 2) = make_float2(o[n][half * 2], o[n][half * 2 + 1]);
+    if ((lane & 3) == 0) {
+      p.part_max[at] = row_max[half];
+      p.part_sum[at] = row_sum[half];
+    }
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constant__ PageMaps maps, const Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  if ((int)blockIdx.x < p.shared_blocks) shared_slice<D>(maps, p, smem);
+  else own_slice<D>(p, smem);
+}
+
+template <int D, int DEPTH>
+__global__ void __launch_bounds__(pae_attention::MERGE_WARPS * 32) prefix_merge_kernel(__nv_bfloat16* __restrict__ out, const Params p) {
+  dependent_launch_trigger();
+  extern __shared__ float weights[];          // [slots], then [MERGE_WARPS][D]
+  const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0;
+  const int shared = min(p.prefix_len[b], p.max_prefix), kv_len = p.kv_len[b], pos0 = p.q_pos0[b];
+  dependent_launch_wait();
+  if (i >= tokens) return;
+  const OwnSpan span = own_span(shared, kv_len, pos0, tokens, groups, (i * groups + h % groups) / OWN_ROWS);
+  int slices = (shared + p.shared_keys - 1) / p.shared_keys;
+  if (span.end > span.first) slices += (span.end - span.base + p.own_keys - 1) / p.own_keys;
+  slices = min(slices, p.slots);
+  const size_t row = (size_t)(token0 + i) * p.heads + h, at = row * p.slots;
+  pae_attention::merge_parts<D, DEPTH>(out + row * D, p.part_out + at * D, p.part_max + at, p.part_sum + at, slices, p.slots, weights);
+}
+
+// ---------------------------------------------------------------------------------------
+// how the keys are cut
+// ---------------------------------------------------------------------------------------
+struct Cut {
+  int row_tiles, shared_slices, shared_keys, own_row_tiles, own_slices, own_keys, slots;
+  long long shared_blocks, own_units;
+};
+// Two blocks of either kind share an SM. The own slices are as many as the warps of that many blocks, of 32 keys at least; the shared slices as many as
+// fill what the own blocks leave of one wave (three quarters of it at least), of two tiles at least.
+Cut cut_keys(int seqs, int groups, int heads, int kv_heads, int max_q_len, int max_prefix, int max_own, int max_group_tokens) {
+  const int share = heads / kv_heads, wave = 2 * pae_attention::multiprocessors();
+  Cut c;
+  c.row_tiles = (int)(((long long)max_group_tokens * share + ROWS - 1) / ROWS);
+  c.own_row_tiles = (int)(((long long)max_q_len * share + OWN_ROWS - 1) / OWN_ROWS);
+  const long long pairs = (long long)seqs * kv_heads * c.own_row_tiles;
+  const int own = max_own + TILE_KEYS - 1;               // a span may begin inside a tile
+  long long most = (long long)wave * OWN_WARPS / pairs;
+  if (most > (own + 31) / 32) most = (own + 31) / 32;
+  if (most < 1) most = 1;
+  c.own_keys = (int)(((own + most - 1) / most + TILE_KEYS - 1) / TILE_KEYS * TILE_KEYS);
+  c.own_slices = (own + c.own_keys - 1) / c.own_keys;
+  c.own_units = pairs * c.own_slices;
+  const long long per_slice = (long long)groups * kv_heads * c.row_tiles, own_blocks = (c.own_units + OWN_WARPS - 1) / OWN_WARPS;
+  const int tiles = (max_prefix + BKEYS - 1) / BKEYS;
+  long long slices = (wave - (own_blocks < wave / 4 ? own_blocks : wave / 4)) / per_slice;
+  if (slices > (tiles + 1) / 2) slices = (tiles + 1) / 2;
+  if (slices < 1) slices = 1;
+  const int slice_tiles = tiles > 0 ? (int)((tiles + slices - 1) / slices) : 1;
+  c.shared_keys = slice_tiles * BKEYS;
+  c.shared_slices = tiles > 0 ? (tiles + slice_tiles - 1) / slice_tiles : 0;
+  c.shared_blocks = per_slice * c.shared_slices;
+  c.slots = c.shared_slices + c.own_slices;
+  return c;
+}
+
+template <int D>
+int launch(const Params& p, void* out, long long pages, int seqs, int max_q_len, cudaStream_t s) {
+  PageMaps maps;
+  if (int err = encode_page_maps(&maps, p.keys, p.values, pages, p.kv_heads, p.page_size, D, BKEYS)) return err;
+  static DevicesSet devices;
+  if (int err = raise_shared_memory(devices, prefix_kernel<D>, Layout<D>::SMEM_BYTES, "paged_attention_prefix")) return err;
+  const int own_blocks = (p.own_units + OWN_WARPS - 1) / OWN_WARPS;
+  launch_kernel(prefix_kernel<D>, dim3(p.shared_blocks + own_blocks), dim3(THREADS), Layout<D>::SMEM_BYTES, s, maps, p);
+  if (int err = check_launch("paged_attention_prefix")) return err;
+  const auto merge = pae_attention::merge_in_few_registers(p.heads * max_q_len, seqs, p.slots) ? prefix_merge_kernel<D, 8> : prefix_merge_kernel<D, 24>;
+  launch_kernel(merge, dim3(p.heads, max_q_len, seqs), dim3(pae_attention::MERGE_WARPS * 32),
+                (p.slots + pae_attention::MERGE_WARPS * D) * sizeof(float), s, (__nv_bfloat16*)out, p);
+  return check_launch("paged_attention_prefix");
+}
+
+}  // namespace
+
+PAE_DEFINE_LAST_ERROR()
+
+PAE_EXPORT int pae_attention_prefix_supports(int heads, int kv_heads, int d, int page_size) {
+  return (d == 64 || d == 128) && (page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128) && kv_heads >= 1 && heads % kv_heads == 0;
+}
+
+// Floats of scratch that pae_paged_attention_prefix needs for the same sizes.
+PAE_EXPORT long long pae_attention_prefix_floats(int tokens, int seqs, int groups, int heads, int kv_heads, int d, int max_q_len, int max_prefix, int max_own,
+                                                 int max_group_tokens) {
+  const Cut c = cut_keys(seqs, groups, heads, kv_heads, max_q_len, max_prefix, max_own, max_group_tokens);
+  return (long long)tokens * heads * c.slots * (d + 2);
+}
+
+PAE_EXPORT int pae_paged_attention_prefix(void* out, const void* qkv, const void* keys, const void* values, long long pages, const int* block_table,
+                                          int table_width, const int* q_start, const int* q_pos0, const int* kv_len, const int* prefix_len,
+                                          const int* group_start, int tokens, int seqs, int groups, int heads, int kv_heads, int d, int page_size,
+                                          int max_q_len, int max_prefix, int max_own, int max_group_tokens, float scale, float* scratch, int* error,
+                                          void* stream) {
+  if (tokens == 0 || seqs == 0) return 0;
+  if (!pae_attention_prefix_supports(heads, kv_heads, d, page_size))
+    return fail(2, "paged_attention_prefix: head_dim %d with pages of %d is not taken (64 or 128; 16, 32, 64 or 128)", d, page_size);
+  if (seqs > 65535 || max_q_len > 65535) return fail(3, "paged_attention_prefix: %d requests of up to %d tokens exceed one launch", seqs, max_q_len);
+  if ((((uintptr_t)qkv | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)out | (uintptr_t)scratch) & 15) != 0)
+    return fail(2, "paged_attention_prefix: an operand does not start on a 16-byte boundary");
+  const Cut c = cut_keys(seqs, groups, heads, kv_heads, max_q_len, max_prefix, max_own, max_group_tokens);
+  if ((size_t)(c.slots + pae_attention::MERGE_WARPS * d) * sizeof(float) > 40 * 1024 || c.shared_blocks + c.own_units > 0x7fffffffll)
+    return fail(3, "paged_attention_prefix: %d slices a row, %lld blocks and %lld warps exceed one launch", c.slots, c.shared_blocks, c.own_units);
+  Params p = {};
+  p.qkv = (const __nv_bfloat16*)qkv;
+  p.keys = (const __nv_bfloat16*)keys;
+  p.values = (const __nv_bfloat16*)values;
+  p.block_table = block_table;
+  p.q_start = q_start;
+  p.q_pos0 = q_pos0;
+  p.kv_len = kv_len;
+  p.prefix_len = prefix_len;
+  p.group_start = group_start;
+  const size_t rows = (size_t)tokens * heads * c.slots;
+  p.part_out = scratch;
+  p.part_max = scratch + rows * d;
+  p.part_sum = p.part_max + rows;
+  p.table_width = table_width;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.page_size = page_size;
+  p.max_prefix = max_prefix;
+  p.shared_blocks = (int)c.shared_blocks;
+  p.row_tiles = c.row_tiles;
+  p.shared_slices = c.shared_slices;
+  p.shared_keys = c.shared_keys;
+  p.own_units = (int)c.own_units;
+  p.own_row_tiles = c.own_row_tiles;
+  p.own_slices = c.own_slices;
+  p.own_keys = c.own_keys;
+  p.slots = c.slots;
+  p.scale_log2 = scale * LOG2E;
+  p.slack = c.shared_blocks >= 2LL * pae_attention::multiprocessors() ? REFERENCE_SLACK : 0.f;
+  p.error = error;
+  if (d == 64) return launch<64>(p, out, pages, seqs, max_q_len, (cudaStream_t)stream);
+  return launch<128>(p, out, pages, seqs, max_q_len, (cudaStream_t)stream);
+}

@@ -2304,7 +2304,7 @@ def expert_combine(y, plan: ExpertPlan, weights, x, base=None, base_gate=None) -
 
 
 # ----------------------------------------------------------------------------------- #
-# attention over the paged cache that adds up its weights per key, and eviction by them
+# attention over the paged cache of requests that share a prefix; attention that adds up its weights per key, and eviction by them
 
 def _here(what: str, **tensors) -> None:
     """All of the tensors lie, contiguous, on the current device (whose stream the kernels are launched on)."""
@@ -2349,6 +2349,53 @@ def _need_attention(what: str, qkv, keys, values, block_table, q_start, q_pos0, 
     if q_start.shape != (seqs + 1,) or q_pos0.shape != (seqs,):
         raise KernelError(f"{what}: q_start {tuple(q_start.shape)} and q_pos0 {tuple(q_pos0.shape)} for {seqs} requests")
     return seqs
+
+
+# From how many tokens a request on a step is an ordinary one: a query tile of one request fills the tensor cores then, and its keys are
+# read once for all of its tokens anyway.
+PREFIX_ATTENTION_MAX_TOKENS = 63
+
+
+def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_len, prefix_len, group_start, num_heads: int, num_kv_heads: int,
+                           head_dim: int, page_size: int, max_q_len: int, max_prefix_len: int, max_own_len: int, max_group_tokens: int, scale: float,
+                           num_single=None, info: dict | None = None) -> torch.Tensor:
+    """`paged_attention` without a window for requests that share the first keys of their contexts, which are read once for all.
+    Requests group_start[i] .. group_start[i + 1] - 1 (int32 [groups + 1], from 0 to the number of requests) are a group: their first
+    prefix_len[b] keys (int32 [requests], the same for all of a group; 0: nothing is shared) are the same, and every token of the step stands behind
+    them. They are read through the block table of the group's first request. The result is that of `paged_attention` but for the order of the sums.
+    The longest request brings `max_q_len` tokens, the largest group `max_group_tokens`; `max_prefix_len` and `max_own_len` bound the shared keys and the
+    keys behind them. `info`, when given, receives which kernel ran ("kernel": "shared", or what `paged_attention` says where each request reads its
+    keys by itself: other types, head sizes and page sizes than the tensor-core kernel's, long portions, groups of one request)."""
+    qkv = materialized(qkv)
+    what = "paged_attention_prefix"
+    seqs = _need_attention(what, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size)
+    _int32(what, prefix_len=prefix_len, group_start=group_start)
+    if prefix_len.shape != (seqs,) or group_start.dim() != 1 or not 2 <= group_start.shape[0] <= seqs + 1:
+        raise KernelError(f"{what}: prefix_len {tuple(prefix_len.shape)} and group_start {tuple(group_start.shape)} for {seqs} requests")
+    tokens, groups = qkv.shape[0], group_start.shape[0] - 1
+    if max_prefix_len < 0 or max_own_len < 0 or max_prefix_len > block_table.shape[1] * page_size:
+        raise KernelError(f"{what}: {max_prefix_len} shared and {max_own_len} own keys for tables of {block_table.shape[1]} pages of {page_size}")
+    if not 0 <= max_q_len <= max_group_tokens <= tokens:
+        raise KernelError(f"{what}: requests of up to {max_q_len} tokens in groups of up to {max_group_tokens}, of {tokens}")
+    _here(what, qkv=qkv, keys=keys, values=values, block_table=block_table, q_start=q_start, q_pos0=q_pos0, kv_len=kv_len, prefix_len=prefix_len,
+          group_start=group_start)
+    lib = _lib("attention_prefix")
+    if not (qkv.dtype == torch.bfloat16 and use_tensor_cores and 0 < max_q_len <= PREFIX_ATTENTION_MAX_TOKENS and max_prefix_len > 0
+            and max_group_tokens > max_q_len and lib.pae_attention_prefix_supports(num_heads, num_kv_heads, head_dim, page_size)
+            and not (qkv.data_ptr() | keys.data_ptr() | values.data_ptr()) & 15):
+        return paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len,
+                               min(max_prefix_len + max_own_len, block_table.shape[1] * page_size), scale, 0, num_single=num_single, info=info)
+    if info is not None:
+        info.update(kernel="shared")
+    out = torch.empty((tokens, num_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+    scratch = torch.empty(lib.pae_attention_prefix_floats(tokens, seqs, groups, num_heads, num_kv_heads, head_dim, max_q_len, max_prefix_len, max_own_len,
+                                                          max_group_tokens), dtype=torch.float32, device=qkv.device)
+    _set_bounds("attention_prefix", keys)
+    _check(lib, lib.pae_paged_attention_prefix(
+        out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), keys.shape[0], block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
+        q_pos0.data_ptr(), kv_len.data_ptr(), prefix_len.data_ptr(), group_start.data_ptr(), tokens, seqs, groups, num_heads, num_kv_heads, head_dim,
+        page_size, max_q_len, max_prefix_len, max_own_len, max_group_tokens, scale, scratch.data_ptr(), _error_flag(qkv.device).data_ptr(), _stream()), 2)
+    return out
 
 
 def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, num_heads: int, num_kv_heads: int, head_dim: int,

@@ -39,3 +39,46 @@ def _compact(keys=None, values=None, mass=None, block_table=None, kv_len=None, k
 def test_compaction_refuses(arguments, message):
     with pytest.raises(ops.KernelError, match=message):
         _compact(**arguments)
+
+
+HEADS, KV_HEADS, DIM, PAGE = 4, 2, 8, 16
+
+
+def _attention(**other):
+    """The tensors of a step of 3 requests of 5 tokens in all, on the CPU, with some of them replaced."""
+    given = dict(qkv=torch.zeros(5, (HEADS + 2 * KV_HEADS) * DIM), keys=torch.zeros(9, KV_HEADS, PAGE, DIM), values=torch.zeros(9, KV_HEADS, PAGE, DIM), block_table=_i32(3, 4),
+                 q_start=_i32(4), q_pos0=_i32(3), kv_len=_i32(3))
+    given.update({k: v for k, v in other.items() if k in given})
+    return given
+
+
+STEP_REFUSALS = [
+    (dict(qkv=torch.zeros(5, 60)), "qkv \\(5, 60\\) for 4\\+2x2 heads of 8"), (dict(qkv=torch.zeros(5, 64, dtype=torch.float16)), "torch.float16 is not supported"),
+    (dict(keys=torch.zeros(9, KV_HEADS, PAGE, DIM, dtype=torch.bfloat16)), "keys torch.bfloat16"), (dict(values=torch.zeros(9, KV_HEADS, 8, DIM)), "values torch.float32 \\(9, 2, 8, 8\\)"),
+    (dict(values=torch.zeros(8, KV_HEADS, PAGE, DIM)), "values"), (dict(q_start=_i32(3)), "q_start \\(3,\\)"), (dict(q_pos0=_i32(4)), "q_pos0 \\(4,\\)"),
+    (dict(kv_len=_i32(3).long()), "kv_len is torch.int64"), (dict(q_start=torch.zeros(4)), "q_start is torch.float32"), (dict(block_table=_i32(2, 4)), "block tables"),
+    (dict(num_heads=3), "3 heads over 2 kv heads"), (dict(num_kv_heads=0), "4 heads over 0 kv heads"), (dict(), "is not on a CUDA device")]
+
+
+@pytest.mark.parametrize("arguments,message", STEP_REFUSALS + [
+    (dict(mass=torch.zeros(9, KV_HEADS, PAGE, dtype=torch.bfloat16)), "mass torch.bfloat16"), (dict(mass=torch.zeros(9, KV_HEADS, 8)), "mass torch.float32 \\(9, 2, 8\\)"),
+    (dict(keep_first=-1), "-1 first keys"), (dict(max_kv_len=65), "65 keys"), (dict(slots=_i32(4)), "slots \\(4,\\) for 5 tokens"), (dict(slots=_i32(5).long()), "slots is torch.int64")])
+def test_mass_refuses(arguments, message):
+    a = dict(mass=torch.zeros(9, KV_HEADS, PAGE), num_heads=HEADS, num_kv_heads=KV_HEADS, head_dim=DIM, page_size=PAGE, max_q_len=3, max_kv_len=64, scale=1.0)
+    a.update(_attention(**arguments))
+    a.update({k: v for k, v in arguments.items()})
+    with pytest.raises(ops.KernelError, match=message):
+        ops.paged_attention_mass(**a)
+
+
+@pytest.mark.parametrize("arguments,message", STEP_REFUSALS + [
+    (dict(prefix_len=_i32(2)), "prefix_len \\(2,\\)"), (dict(prefix_len=_i32(3).long()), "prefix_len is torch.int64"), (dict(group_start=_i32(1)), "group_start \\(1,\\)"),
+    (dict(group_start=_i32(5)), "group_start \\(5,\\)"), (dict(group_start=torch.zeros(3)), "group_start is torch.float32"), (dict(max_prefix_len=-1), "-1 shared"),
+    (dict(max_own_len=-1), "-1 own keys"), (dict(max_prefix_len=65), "65 shared"), (dict(max_group_tokens=6), "groups of up to 6, of 5"), (dict(max_q_len=4), "up to 4 tokens in groups of up to 3")])
+def test_prefix_refuses(arguments, message):
+    a = dict(prefix_len=_i32(3), group_start=_i32(3), num_heads=HEADS, num_kv_heads=KV_HEADS, head_dim=DIM, page_size=PAGE, max_q_len=2, max_prefix_len=20, max_own_len=30,
+             max_group_tokens=3, scale=1.0)
+    a.update(_attention(**arguments))
+    a.update({k: v for k, v in arguments.items()})
+    with pytest.raises(ops.KernelError, match=message):
+        ops.paged_attention_prefix(**a)
