@@ -50,6 +50,9 @@ constexpr int THREADS = 320;         // TMA warp, MMA warp, eight softmax warps 
 constexpr int SOFTMAX_THREADS = 256;
 constexpr float LOG2E = 1.4426950408889634f;
 
+// Of a row without a key, +infinity: its weights are 0.
+__device__ __forceinline__ float logarithm(float reference, float sum) { return sum == 0.f ? INFINITY : reference + log2f(sum); }
+
 struct Params {
   __nv_bfloat16* out;               // [tokens, heads, D]
   const int* block_table;
@@ -59,6 +62,7 @@ struct Params {
   int table_width, heads, kv_heads, page_size, window, skip_single;
   const int* work_index;  // the requests that this launch works on, one per grid z (null: request z)
   float scale_log2;
+  float* lse;             // [tokens, heads] or null: receives the logarithm of a row's denominator, in units of log2 (attention_mass_prompt.cu)
   float slack;            // paired form: a row's reference may lie below its maximum by 2^slack (0: it follows every maximum)
   int* error;
 };
@@ -492,6 +496,7 @@ __global__ void __launch_bounds__(THREADS) prefill_tcgen05_kernel(const __grid_c
 
   if (warp >= 2 && rank == 0 && ok && r < rows) {
     const float inv = row_sum > 0.f ? 1.f / row_sum : 0.f;
+    if (p.lse != nullptr && side == 0) p.lse[(size_t)(first_token + tile * BQ + r) * p.heads + h] = logarithm(row_max, row_sum);
     __nv_bfloat16* out = p.out + ((size_t)(first_token + tile * BQ + r) * p.heads + h) * D + side * HALF_D;
 #pragma unroll
     for (int c = 0; c < HALF_D; c += 8) {
@@ -914,6 +919,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_tcgen05_paired_kernel(cons
       if (ok) {
         tcgen05_fence_after();
         const float inv = row_sum > 0.f ? 1.f / row_sum : 0.f;
+        if (p.lse != nullptr && r < rows) p.lse[(size_t)(first_token + tile * BQ + r) * p.heads + h] = logarithm(reference, row_sum);
         __nv_bfloat16* out = p.out + ((size_t)(first_token + tile * BQ + r) * p.heads + h) * D;
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
@@ -1028,13 +1034,13 @@ PAE_EXPORT int pae_attention_tcgen05_supports(int heads, int kv_heads, int d, in
 }
 
 // Attention of every request that brings more than one token (or every request, unless
-// skip_single; `singles` is how many bring one, -1 when the caller does not know). form 0 picks the kernel by the size of the launch, 1 and 2 name it (tests); `chosen` (a host pointer, or null) receives the blocks per query tile of this launch: 1 without clusters, 0 for the paired kernel. `work_index` (device, or null) lists the `work_count` requests that the launch is to cover, in place of all `seqs`. qkv [tokens, heads + 2 kv_heads, d]; keys, values [pages, kv_heads, page_size, d].
+// skip_single; `singles` is how many bring one, -1 when the caller does not know). form 0 picks the kernel by the size of the launch, 1 and 2 name it (tests); `chosen` (a host pointer, or null) receives the blocks per query tile of this launch: 1 without clusters, 0 for the paired kernel. `work_index` (device, or null) lists the `work_count` requests that the launch is to cover, in place of all `seqs`. `lse` (or null) [tokens, heads] receives the logarithms of the rows' denominators. qkv [tokens, heads + 2 kv_heads, d]; keys, values [pages, kv_heads, page_size, d].
 PAE_EXPORT int pae_paged_attention_prefill_tcgen05(void* out, const void* qkv, const void* keys, const void* values,
                                                    long long pages, const int* block_table, int table_width,
                                                    const int* q_start, const int* q_pos0, const int* kv_len, int tokens,
                                                    int seqs, int max_q_len, int max_kv_len, int heads, int kv_heads, int d,
                                                    int page_size, float scale, int window, int skip_single, int singles, int form, int* chosen,
-                                                   const int* work_index, int work_count, int* error, void* stream) {
+                                                   const int* work_index, int work_count, float* lse, int* error, void* stream) {
   if (seqs == 0 || max_q_len == 0 || tokens == 0) return 0;
   if (work_index != nullptr && (work_count < 1 || work_count > seqs))
     return fail(2, "paged_attention_tcgen05: a list of %d requests to work on, of %d", work_count, seqs);
@@ -1057,6 +1063,7 @@ PAE_EXPORT int pae_paged_attention_prefill_tcgen05(void* out, const void* qkv, c
   p.skip_single = skip_single;
   p.scale_log2 = scale * LOG2E;
   p.error = error;
+  p.lse = lse;
   cudaStream_t s = (cudaStream_t)stream;
   p.work_index = work_index;
   const int working_seqs = work_index != nullptr ? work_count : (skip_single && singles > 0 && singles < seqs ? seqs - singles : seqs);

@@ -64,6 +64,7 @@ FAMILIES: dict[str, list[str]] = {
     "state_space": ["state_space.cu", "common.cuh"],
     "attention_prefix": ["attention_prefix.cu", "attention_mma.cuh", "attention_pages.cuh", "tcgen05.cuh", "common.cuh"],
     "attention_mass": ["attention_mass.cu", "attention_mma.cuh", "common.cuh"],
+    "attention_mass_prompt": ["attention_mass_prompt.cu", "attention_pages.cuh", "tcgen05.cuh", "common.cuh"],
     "evict": ["evict.cu", "common.cuh"],
     "attention_decode_noalloc": [
         "attention_decode_noalloc.cu", "attention_decode_noalloc.h", "attention_mma.cuh", "common.cuh",

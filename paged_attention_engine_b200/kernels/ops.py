@@ -1079,7 +1079,7 @@ def paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num
                     block_table.shape[1], _ptr(q_start), _ptr(q_pos0), _ptr(kv_len), tokens, seqs,
                     max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size,
                     scale, window, (1 if decode_after else 0), singles, form,
-                    ctypes.byref(chosen), _ptr(listed), (listed.numel() if listed is not None else 0),
+                    ctypes.byref(chosen), _ptr(listed), (listed.numel() if listed is not None else 0), None,
                     _ptr(_error_flag(qkv.device)), _stream()))
                 if info is not None:
                     info.update(kernel="tcgen05", cluster=chosen.value)
@@ -2398,6 +2398,47 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     return out
 
 
+def _decode_mass(out, qkv, keys, values, mass, block_table, q_start, kv_len, slots, sizes, max_kv_len: int, scale: float, keep_first: int, singles: int) -> None:
+    """The requests of a step that bring one token: their rows of `out`, and their keys' weights."""
+    num_heads, num_kv_heads, head_dim, page_size = sizes
+    seqs = kv_len.shape[0]
+    plain, lib = _lib("attention_mma"), _lib("attention_mass")
+    slice_keys, max_slices = decode_slicing(singles, num_kv_heads, max_kv_len, wave_blocks=plain.pae_decode_blocks_per_wave(head_dim),
+                                            slices_per_block=plain.pae_decode_slices_per_block())
+    scratch = torch.empty(lib.pae_decode_mass_floats(seqs, num_heads, head_dim, slice_keys, max_slices), dtype=torch.float32, device=qkv.device)
+    _set_bounds("attention_mass", keys)
+    _check(lib, lib.pae_paged_attention_decode_mass(
+        out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), mass.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
+        kv_len.data_ptr(), _ptr(slots), seqs, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices, scratch.data_ptr(),
+        _stream()), 2)
+
+
+def _prompt_mass(lib, out, qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, slots, sizes, max_q_len: int, max_kv_len: int, scale: float,
+                 keep_first: int, singles: int, multi_index) -> None:
+    """The requests of a step that bring several tokens: the attention, which leaves the logarithms of the rows' denominators, and the weights."""
+    num_heads, num_kv_heads, head_dim, page_size = sizes
+    tokens, seqs = qkv.shape[0], kv_len.shape[0]
+    listed = multi_index if multi_index is not None and singles > 0 else None
+    if listed is not None:
+        _need(listed, "paged_attention_mass: multi_index", torch.int32)
+        if listed.numel() != seqs - singles:
+            raise KernelError(f"paged_attention_mass: {listed.numel()} requests listed, {seqs - singles} bring more than one token")
+    attention = _lib("attention_tcgen05")
+    logarithms = torch.empty((tokens, num_heads), dtype=torch.float32, device=qkv.device)
+    scratch = torch.empty(lib.pae_attention_mass_prompt_floats(seqs, num_heads, num_kv_heads, max_q_len, max_kv_len), dtype=torch.float32, device=qkv.device)
+    error = _error_flag(qkv.device).data_ptr()
+    _set_bounds("attention_tcgen05", keys)
+    _set_bounds("attention_mass_prompt", keys)
+    _check(attention, attention.pae_paged_attention_prefill_tcgen05(
+        out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), keys.shape[0], block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
+        q_pos0.data_ptr(), kv_len.data_ptr(), tokens, seqs, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, 0, 1, singles, 0, None,
+        _ptr(listed), (listed.numel() if listed is not None else 0), logarithms.data_ptr(), error, _stream()))
+    _check(lib, lib.pae_attention_mass_prompt(
+        mass.data_ptr(), qkv.data_ptr(), keys.data_ptr(), keys.shape[0], logarithms.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
+        q_pos0.data_ptr(), kv_len.data_ptr(), _ptr(slots), tokens, seqs, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first,
+        scratch.data_ptr(), error, _stream()), 2)
+
+
 def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, num_heads: int, num_kv_heads: int, head_dim: int,
                          page_size: int, max_q_len: int, max_kv_len: int, scale: float, keep_first: int = 0, slots=None, num_single=None,
                          multi_index=None) -> torch.Tensor:
@@ -2423,18 +2464,19 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
             raise KernelError(f"paged_attention_mass: slots {tuple(slots.shape)} for {tokens} tokens")
         given["slots"] = slots
     _here("paged_attention_mass", **given)
-    if max_q_len == 1 and max_kv_len > 0 and plain_attention_takes(num_heads, num_kv_heads, head_dim, page_size, qkv.dtype):
-        plain, lib = _lib("attention_mma"), _lib("attention_mass")
-        slice_keys, max_slices = decode_slicing(seqs, num_kv_heads, max_kv_len, wave_blocks=plain.pae_decode_blocks_per_wave(head_dim),
-                                                slices_per_block=plain.pae_decode_slices_per_block())
-        out = torch.empty((tokens, num_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
-        scratch = torch.empty(lib.pae_decode_mass_floats(seqs, num_heads, head_dim, slice_keys, max_slices), dtype=torch.float32, device=qkv.device)
-        _set_bounds("attention_mass", keys)
-        _check(lib, lib.pae_paged_attention_decode_mass(
-            out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), mass.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
-            kv_len.data_ptr(), _ptr(slots), seqs, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices, scratch.data_ptr(),
-            _stream()), 2)
-        return out
+    singles = num_single if num_single is not None else (seqs if max_q_len == 1 else -1)
+    sizes = (num_heads, num_kv_heads, head_dim, page_size)
+    if max_kv_len > 0 and max_q_len > 0 and plain_attention_takes(*sizes, qkv.dtype):
+        prompt = _lib("attention_mass_prompt") if max_q_len > 1 else None
+        if prompt is None or (use_tcgen05_attention and prompt.pae_attention_mass_prompt_supports(*sizes)
+                              and not (qkv.data_ptr() | keys.data_ptr() | values.data_ptr()) & 15):
+            out = torch.empty((tokens, num_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+            if prompt is not None:
+                _prompt_mass(prompt, out, qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, slots, sizes, max_q_len, max_kv_len, scale, keep_first,
+                             singles, multi_index)
+            if singles != 0:
+                _decode_mass(out, qkv, keys, values, mass, block_table, q_start, kv_len, slots, sizes, max_kv_len, scale, keep_first, seqs if singles < 0 else singles)
+            return out
     out = paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_kv_len, scale,
                           0, num_single=num_single, multi_index=multi_index)
     lib = _lib("attention_mass")

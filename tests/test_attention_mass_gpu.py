@@ -116,3 +116,21 @@ def test_equal_bits_in_every_run_and_batch(ops):
     step = Step([260, 90], [100, 90], 12, 2, 64, 16, F32, 13)
     runs = [_run(ops, step) for _ in range(3)]
     assert all(torch.equal(o, runs[0][0]) and torch.equal(m, runs[0][1]) for o, m in runs)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(28, 4, 128, 16), (12, 2, 64, 64), (40, 8, 128, 128), (5, 1, 128, 32), (128, 1, 64, 16), (8, 8, 128, 16)])
+@pytest.mark.parametrize("lengths,tokens", [([1500], [1500]), ([2000, 900, 333], [700, 900, 1]), ([129, 128, 127, 1, 700], [129, 2, 127, 1, 1]), ([1800], [257])])
+def test_long_portions(ops, heads, kv_heads, dim, page, lengths, tokens):
+    """Keys as the rows of a tensor-core product, rows in chunks, beside requests of one token."""
+    step = Step(lengths, tokens, heads, kv_heads, dim, page, BF16, heads + sum(tokens))
+    for keep_first in (0, 130):
+        _check(step, *_run(ops, step, keep_first), keep_first)
+    ops.check_device_errors()
+
+
+def test_a_mixed_step_as_the_engine_describes_it(ops):
+    """`num_single` and the list of the requests that bring more than one token."""
+    step = Step([300, 500, 77, 200], [1, 130, 1, 200], 12, 2, 128, 16, BF16, 9)
+    _check(step, *_run(ops, step, num_single=2, multi_index=i32([1, 3], "cuda")))
+    step = Step([300, 500], [64, 130], 12, 2, 128, 16, BF16, 9)
+    _check(step, *_run(ops, step, num_single=0))
