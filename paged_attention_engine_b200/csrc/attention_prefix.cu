@@ -6,13 +6,13 @@
 //
 // A softmax over two sets of keys is the two sets' (maximum, sum, unnormalised output) brought to one maximum and added, so the
 // shared keys are taken for all rows (token, query head of the kv head) of a group at once: they are read once a
-// group and not once a request, and there are enough rows to fill the tensor cores. One launch of blocks of two kinds, and a merge:
+// group and not once a request, and there are enough rows to fill the tensor cores. The own keys go the same way, with the rows of one
+// request. One launch and a merge:
 //
-//   shared   128 rows x a slice of the shared keys, 64 keys a tile, as the paired prefill attention works (attention_tcgen05.cu), which see for
-//            the roles and the references that may lie behind the maxima: keys and values by TMA, both products as tcgen05.mma, scores,
-//            probabilities and output in tensor memory. There is no mask but for the slice's last tile: every query stands behind the shared keys.
-//   own      six warps, each 16 rows of one request x a slice of its own keys, 16 keys a tile by mma.sync, as the sliced decode attention works
-//            (attention_mma.cuh). These blocks wait for memory while the others compute.
+//   slices   a block takes up to 128 rows x a slice of shared keys, or of a request's own, 64 keys a tile, as the paired prefill attention works
+//            (attention_tcgen05.cu), which see for the roles and the references that may lie behind the maxima: keys and values by TMA,
+//            both products as tcgen05.mma, scores, probabilities and output in tensor memory. Softmax warps without a row take no part, so that over
+//            own keys, which few rows read, a tile costs little more than its bytes.
 //   merge    a row's slices, shared and own, in their order.
 //
 // Scores are scaled in float32, maxima, sums and outputs are float32; probabilities are rounded to bfloat16 for the second
@@ -24,19 +24,14 @@
 
 using namespace pae;
 using namespace pae_tcgen05;
-using pae_attention::TILE_KEYS;
-using pae_attention::TileLayout;
 
 namespace {
 
-constexpr int ROWS = 128;                // of a shared block
-constexpr int BKEYS = 64;                // keys per tile of a shared block
-constexpr int THREADS = 192;             // TMA warp, MMA warp, four softmax warps; or six warps with a slice each
+constexpr int ROWS = 128;                // of a block
+constexpr int BKEYS = 64;                // keys per tile
+constexpr int THREADS = 192;             // TMA warp, MMA warp, four softmax warps (one thread per row)
 constexpr int SOFTMAX_WARPS = 4;
 constexpr int KV_STAGES = 2;
-constexpr int OWN_WARPS = THREADS / 32;
-constexpr int OWN_STAGES = 2;
-constexpr int OWN_ROWS = 16;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float REFERENCE_SLACK = 8.f;   // as the paired prefill attention
 constexpr float REFERENCE_LIMIT = 256.f;
@@ -56,7 +51,7 @@ struct Params {
   float* part_sum;
   int table_width, heads, kv_heads, page_size, max_prefix;
   int shared_blocks, row_tiles, shared_slices, shared_keys;      // keys per slice of the shared ones, a multiple of BKEYS
-  int own_units, own_row_tiles, own_slices, own_keys;            // likewise of the own ones, a multiple of TILE_KEYS
+  int own_row_tiles, own_slices, own_keys;                       // likewise of the own ones
   int slots;                    // slices of a row at most: shared ones, then own ones
   float scale_log2, slack;
   int* error;
@@ -77,8 +72,6 @@ struct Layout {
   static constexpr int S_COLUMNS = BKEYS;
   static constexpr int O_COLUMN = 2 * S_COLUMNS;
   static constexpr int TMEM_COLUMNS = 256;
-  static constexpr int OWN_BYTES = OWN_STAGES * 2 * TILE_KEYS * D * 2;     // of a warp
-  static_assert(OWN_WARPS * OWN_BYTES <= BAR_OFFSET, "the six warps' stages lie where the tiles of the other kind do");
 };
 
 enum Bar : int {
@@ -86,12 +79,98 @@ enum Bar : int {
   K_FULL = 7, K_EMPTY = K_FULL + KV_STAGES, V_FULL = K_EMPTY + KV_STAGES, V_EMPTY = V_FULL + KV_STAGES, NUM_BARS = V_EMPTY + KV_STAGES
 };
 
-// ---------------------------------------------------------------------------------------
-// the shared keys
-// ---------------------------------------------------------------------------------------
+// The pages of a run of keys from `begin` (where a box of rows starts) to `end`, for a converged warp: the table is read 32 boxes at a time, one
+// load ahead of need.
+struct PageRun {
+  const int* table;
+  int begin, box_rows, shift, last, width, lane;
+  int held, ahead, window;                 // entries of boxes window * 32 + lane, and of the next 32
+  __device__ __forceinline__ int entry(int box) const {
+    return checked_page(table[checked_table_index(min((begin + box * box_rows) >> shift, last), width)]);     // behind the end any page will do
+  }
+  __device__ __forceinline__ void start(const int* t, int b, int e, int rows, int page_size, int w, int l) {
+    table = t, begin = b, box_rows = rows, width = w, lane = l, window = 0;
+    shift = 31 - __clz(page_size);         // page sizes are powers of two
+    last = (e - 1) >> shift;
+    held = entry(lane);
+    ahead = entry(32 + lane);
+  }
+  // Box `lane` of tile t (all lanes call; tiles in ascending order, at most 32 boxes behind the furthest).
+  __device__ __forceinline__ int page(int t, int boxes) {
+    const int box = t * boxes + lane;
+    const int first = __shfl_sync(0xffffffffu, box, 0);
+    if (first >= (window + 1) * 32) {
+      held = ahead;
+      ++window;
+      ahead = entry((window + 1) * 32 + lane);
+    }
+    return __shfl_sync(0xffffffffu, held, box & 31);
+  }
+};
+// Where the own keys of a tile of ROWS rows begin and end; their slices start at `base`, where a box of rows does.
+struct OwnSpan {
+  int first, base, end;
+};
+__device__ __forceinline__ OwnSpan own_span(const Params& p, int shared, int kv_len, int pos0, int tokens, int groups, int row_tile) {
+  OwnSpan s;
+  s.first = shared;
+  s.base = shared & -min(p.page_size, BKEYS);
+  s.end = min(kv_len, pos0 + min((row_tile * ROWS + ROWS - 1) / groups, tokens - 1) + 1);
+  return s;
+}
+
+// What a block works on: rows row0 .. row0 + rows - 1 (token, head of kv head g) behind `first_token`, keys begin .. end - 1 by the table of
+// request b. Row r sees those from `first` on that stand at or before pos0 + its token's index.
+struct Work {
+  int b, g, first_token, row0, rows, begin, end, first, pos0, slot;
+};
+constexpr int EVERY_KEY = 1 << 30;       // pos0 of rows behind all keys
+__device__ __forceinline__ Work find_work(const Params& p, int index) {
+  const int groups = p.heads / p.kv_heads;
+  Work w = {0, 0, 0, 0, 0, 0, 0, 0, EVERY_KEY, 0};
+  if (index < p.shared_blocks) {
+    // The row tiles of a kv head and a slice are neighbours: they read the same keys.
+    const int row_tile = index % p.row_tiles;
+    index /= p.row_tiles;
+    w.g = index % p.kv_heads;
+    index /= p.kv_heads;
+    w.slot = index % p.shared_slices;
+    const int group = index / p.shared_slices;
+    w.b = p.group_start[group];
+    const int b_end = p.group_start[group + 1];
+    if (w.b >= b_end) return w;
+    w.first_token = p.q_start[w.b];
+    w.row0 = row_tile * ROWS;
+    w.rows = min(ROWS, (p.q_start[b_end] - w.first_token) * groups - w.row0);
+    w.begin = w.slot * p.shared_keys;
+    w.end = min(min(p.prefix_len[w.b], p.max_prefix), w.begin + p.shared_keys);
+    return w;
+  }
+  index -= p.shared_blocks;
+  const int slice = index % p.own_slices;
+  index /= p.own_slices;
+  const int row_tile = index % p.own_row_tiles;
+  index /= p.own_row_tiles;
+  w.g = index % p.kv_heads;
+  w.b = index / p.kv_heads;
+  w.first_token = p.q_start[w.b];
+  const int tokens = p.q_start[w.b + 1] - w.first_token, shared = min(p.prefix_len[w.b], p.max_prefix);
+  w.pos0 = p.q_pos0[w.b];
+  const OwnSpan span = own_span(p, shared, p.kv_len[w.b], w.pos0, tokens, groups, row_tile);
+  if (span.end <= span.first) return w;
+  w.row0 = row_tile * ROWS;
+  w.rows = min(ROWS, tokens * groups - w.row0);
+  w.first = shared;
+  w.begin = span.base + slice * p.own_keys;
+  w.end = min(span.end, w.begin + p.own_keys);
+  w.slot = (shared + p.shared_keys - 1) / p.shared_keys + slice;
+  return w;
+}
+
 template <int D>
-__device__ __forceinline__ void shared_slice(const PageMaps& maps, const Params& p, uint8_t* raw_smem) {
+__global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constant__ PageMaps maps, const Params p) {
   using L = Layout<D>;
+  extern __shared__ uint8_t raw_smem[];
   const uint32_t raw = smem_u32(raw_smem);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* generic_base = raw_smem + (base - raw);
@@ -100,30 +179,19 @@ __device__ __forceinline__ void shared_slice(const PageMaps& maps, const Params&
   volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
   auto bar = [&](int which, int i = 0) { return bars + 8u * (which + i); };
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-
-  // What this block works on: the row tiles of a kv head and a slice are neighbours, they read the same keys.
-  int index = blockIdx.x;
-  const int row_tile = index % p.row_tiles;
-  index /= p.row_tiles;
-  const int g = index % p.kv_heads;
-  index /= p.kv_heads;
-  const int slice = index % p.shared_slices, group = index / p.shared_slices;
-  const int b = p.group_start[group], b_end = p.group_start[group + 1];
-  const int groups = p.heads / p.kv_heads;
-  int first_token = 0, rows = 0, kv_end = 0;
-  const int kv_begin = slice * p.shared_keys;
-  if (b < b_end) {
-    first_token = p.q_start[b];
-    rows = min(ROWS, (p.q_start[b_end] - first_token) * groups - row_tile * ROWS);
-    kv_end = min(min(p.prefix_len[b], p.max_prefix), kv_begin + p.shared_keys);
-  }
-  if (rows <= 0 || kv_begin >= kv_end) {               // the same in every thread
+  const Work work = find_work(p, blockIdx.x);
+  if (work.rows <= 0 || work.begin >= work.end) {      // the same in every thread
     dependent_launch_trigger();
     dependent_launch_wait();
     return;
   }
+  const int rows = work.rows, kv_begin = work.begin, kv_end = work.end, g = work.g, groups = p.heads / p.kv_heads;
   const int n_tiles = (kv_end - kv_begin + BKEYS - 1) / BKEYS;
+  const int row_warps = (rows + 31) / 32;              // the softmax warps that have rows
 
+  const int box_rows = min(p.page_size, BKEYS);
+  PageRun pages;                                       // of the producer; the table was on the device before the step's first kernel began
+  if (warp == 0) pages.start(p.block_table + (size_t)work.b * p.table_width, kv_begin, kv_end, box_rows, p.page_size, p.table_width, lane);
   if (threadIdx.x == 0) {
     mbar_init(bar(Q_FULL), SOFTMAX_WARPS * 32);
     for (int i = 0; i < KV_STAGES; ++i) {
@@ -134,7 +202,7 @@ __device__ __forceinline__ void shared_slice(const PageMaps& maps, const Params&
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(S_FULL, i), 1);
-      mbar_init(bar(P_READY, i), SOFTMAX_WARPS);
+      mbar_init(bar(P_READY, i), row_warps);
     }
     mbar_init(bar(O_REST), 1);
     mbar_init(bar(O_FULL), 1);
@@ -150,19 +218,12 @@ __device__ __forceinline__ void shared_slice(const PageMaps& maps, const Params&
   dependent_launch_trigger();
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_holder;
-  const int box_rows = min(p.page_size, BKEYS);
   dependent_launch_wait();
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer: lane i brings box i of a tile
-    const int* table = p.block_table + (size_t)b * p.table_width;
-    const bool mine = lane < BKEYS / box_rows;
-    const int last_page = (kv_end - 1) / p.page_size, page_shift = 31 - __clz(p.page_size);
-    // Rows of a tile behind the last shared key are masked: any page will do, the last is taken.
-    auto page_of = [&](int t) {
-      const int key = kv_begin + t * BKEYS + lane * box_rows;
-      return mine && t < n_tiles ? checked_page(table[checked_table_index(min(key >> page_shift, last_page), p.table_width)]) : 0;
-    };
+    const int boxes = BKEYS / box_rows;
+    auto page_of = [&](int t) { return t < n_tiles ? pages.page(t, boxes) : 0; };
     auto load = [&](bool values, int t, int page) {
       const int stage = t % KV_STAGES;
       const uint32_t full = bar(values ? V_FULL : K_FULL, stage);
@@ -254,32 +315,43 @@ __device__ __forceinline__ void shared_slice(const PageMaps& maps, const Params&
     const int quadrant = warp & 3;
     const int r = quadrant * 32 + lane;                       // row of the tile, lane of tensor memory
     const uint32_t lane_base = tmem_base + ((uint32_t)(quadrant * 32) << 16);
-    const int row = row_tile * ROWS + r;                      // of the group
-    const size_t token = (size_t)(first_token + row / groups);
+    const int row = work.row0 + r;
+    const size_t token = (size_t)(work.first_token + row / groups);
     const int head = g * groups + row % groups;
+    const int row_end = min(kv_end, work.pos0 + row / groups + 1);               // the keys before it are visible to the row
+    const int all_see = min(kv_end, work.pos0 + work.row0 / groups + 1);         // those before it to every row
     {
-      // The thread brings its row's query into the operand's swizzled layout; rows behind the last are zeros.
-      const uint4* from = (const uint4*)(p.qkv + (token * (p.heads + 2 * p.kv_heads) + head) * D);
-      uint8_t* to = generic_base + L::Q_OFFSET + r * 128;
+      // The warp brings its rows' queries, neighbouring lanes a row's, into the operand's swizzled layout; rows behind the last are zeros.
+      constexpr int CHUNKS = D / 8, ROWS_A_PASS = 32 / CHUNKS;
+      const int query = (int)token * (p.heads + 2 * p.kv_heads) + head, chunk = lane % CHUNKS;
+      uint4 held[32 / ROWS_A_PASS];
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c)
-        *(uint4*)(to + (c >> 3) * L::Q_HALF_BYTES + (((c & 7) ^ (r & 7)) << 4)) = r < rows ? from[c] : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 32 / ROWS_A_PASS; ++i) {
+        const int mine = i * ROWS_A_PASS + lane / CHUNKS, from = __shfl_sync(0xffffffffu, query, mine);
+        held[i] = quadrant * 32 + mine < rows ? ((const uint4*)(p.qkv + (size_t)from * D))[chunk] : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 32 / ROWS_A_PASS; ++i) {
+        const int mine = quadrant * 32 + i * ROWS_A_PASS + lane / CHUNKS;
+        *(uint4*)(generic_base + L::Q_OFFSET + (chunk >> 3) * L::Q_HALF_BYTES + mine * 128 + (((chunk & 7) ^ (mine & 7)) << 4)) = held[i];
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(bar(Q_FULL));
     }
     float reference = -FLT_MAX, row_sum = 0.f;                // the reference in units of log2, scaled
     bool ok = true;
-    for (int t = 0; t < n_tiles; ++t) {
+    for (int t = 0; t < (quadrant < row_warps ? n_tiles : 0); ++t) {
       const int st = t & 1;
       ok = ok && mbar_wait(bar(S_FULL, st), (t >> 1) & 1, abort_flag, p.error, 8);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
-      const int visible = kv_end - kv_begin - t * BKEYS;      // of the tile; below BKEYS in a slice's last tile only
+      const int key0 = kv_begin + t * BKEYS, lo = work.first - key0, hi = r < rows ? row_end - key0 : 0;
+      const bool unmasked = lo <= 0 && key0 + BKEYS <= all_see;      // else the row sees the tile's keys lo .. hi - 1
       uint32_t packed[BKEYS / 2];
       uint64_t sum01, sum23, factor2, offset2;
       auto begin = [&] {
-        const float offset = reference != -FLT_MAX ? -reference : 0.f;     // without one all scores are -infinity or no number: 0 or no number
+        const float offset = reference != -FLT_MAX ? -reference : 0.f;     // without one the visible scores are -infinity or no number: 0 or no number
         factor2 = pack2(p.scale_log2, p.scale_log2);
         offset2 = pack2(offset, offset);
         sum01 = sum23 = 0;
@@ -297,12 +369,12 @@ __device__ __forceinline__ void shared_slice(const PageMaps& maps, const Params&
         packed[i / 2 + 1] = *(const uint32_t*)&h23;
       };
       auto take32 = [&](const float* s, int first) {
-        if (visible >= BKEYS) {
+        if (unmasked) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4) take(s + i, first + i, [](int) { return true; });
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) take(s + i, first + i, [&](int key) { return key < visible; });
+          for (int i = 0; i < 32; i += 4) take(s + i, first + i, [&](int key) { return key >= lo && key < hi; });
         }
       };
       auto tile_sum = [&] {
@@ -314,7 +386,7 @@ __device__ __forceinline__ void shared_slice(const PageMaps& maps, const Params&
       const uint32_t scores = lane_base + st * L::S_COLUMNS;
       bool taken = false;
       float slack = p.slack;
-      if (p.slack > 0.f && !__any_sync(0xffffffffu, reference == -FLT_MAX)) {
+      if (p.slack > 0.f && !__any_sync(0xffffffffu, r < rows && reference == -FLT_MAX)) {
         // Against the references as they are; should a sum come out above REFERENCE_LIMIT (or not a number), the tile is taken again below.
         float s[32], behind[32];
         tmem_ask32(scores, s);
@@ -333,8 +405,13 @@ __device__ __forceinline__ void shared_slice(const PageMaps& maps, const Params&
         float s[BKEYS];
         tmem_load64(scores, s);
         float m4[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX};
+        if (unmasked) {
 #pragma unroll
-        for (int i = 0; i < BKEYS; ++i) m4[i & 3] = fmaxf(m4[i & 3], i < visible ? s[i] : -FLT_MAX);
+          for (int i = 0; i < BKEYS; ++i) m4[i & 3] = fmaxf(m4[i & 3], s[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < BKEYS; ++i) m4[i & 3] = fmaxf(m4[i & 3], i >= lo && i < hi ? s[i] : -FLT_MAX);
+        }
         float tile_max = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         if (tile_max != -FLT_MAX) tile_max *= p.scale_log2;        // the scale is positive: max(s) scales with it
         const bool moves = tile_max > reference + slack || (reference == -FLT_MAX && tile_max != -FLT_MAX);
@@ -371,21 +448,29 @@ __device__ __forceinline__ void shared_slice(const PageMaps& maps, const Params&
       if (lane == 0) mbar_arrive(bar(P_READY, st));
     }
     ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
+    if (ok && quadrant < row_warps) {
       ok = mbar_wait(bar(O_FULL), 0, abort_flag, p.error, 9);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tcgen05_fence_after();
-        const size_t at = (token * p.heads + head) * p.slots + slice;
-        float* out = p.part_out + at * D;
+        // Through shared memory, where keys and values lay (every product has read them): a row leaves as one run of bytes.
+        const uint32_t at = (uint32_t)((token * p.heads + head) * p.slots + work.slot);
+        float* mine = (float*)(generic_base + L::K_OFFSET) + quadrant * 32 * D;      // [32][D], 16-byte chunk c of row r at c ^ (r & 7)
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           float o[32];
-          tmem_load32(lane_base + L::O_COLUMN + c, o);        // every lane takes part
-          if (r < rows) {
+          tmem_load32(lane_base + L::O_COLUMN + c, o);
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) *(float4*)(out + c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-          }
+          for (int j = 0; j < 32; j += 4) *(float4*)(mine + lane * D + ((((c + j) >> 2) ^ (lane & 7)) << 2)) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        }
+        __syncwarp();
+        constexpr int CHUNKS = D / 4, ROWS_A_PASS = 32 / CHUNKS;
+        const int chunk = lane % CHUNKS;
+#pragma unroll 8
+        for (int i = 0; i < 32; i += ROWS_A_PASS) {
+          const int from = i + lane / CHUNKS;
+          const uint32_t to = __shfl_sync(0xffffffffu, at, from);
+          if (quadrant * 32 + from < rows) *(float4*)(p.part_out + (size_t)to * D + chunk * 4) = *(const float4*)(mine + from * D + ((chunk ^ (from & 7)) << 2));
         }
         if (r < rows) {
           p.part_max[at] = reference;
@@ -403,128 +488,12 @@ __device__ __forceinline__ void shared_slice(const PageMaps& maps, const Params&
   }
 }
 
-// ---------------------------------------------------------------------------------------
-// the own keys
-// ---------------------------------------------------------------------------------------
-// Where the own keys of a tile of OWN_ROWS rows begin and end: its slices start at `base`.
-struct OwnSpan {
-  int first, base, end;
-};
-__device__ __forceinline__ OwnSpan own_span(int shared, int kv_len, int pos0, int tokens, int groups, int row_tile) {
-  OwnSpan s;
-  s.first = shared;
-  s.base = shared / TILE_KEYS * TILE_KEYS;
-  s.end = min(kv_len, pos0 + min((row_tile * OWN_ROWS + OWN_ROWS - 1) / groups, tokens - 1) + 1);
-  return s;
-}
-
-template <int D>
-__device__ __forceinline__ void own_slice(const Params& p, uint8_t* smem) {
-  using namespace pae_attention;
-  dependent_launch_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int unit = ((int)blockIdx.x - p.shared_blocks) * OWN_WARPS + warp;
-  const int slice = unit % p.own_slices;
-  int rest = unit / p.own_slices;
-  const int row_tile = rest % p.own_row_tiles;
-  rest /= p.own_row_tiles;
-  const int g = rest % p.kv_heads, b = rest / p.kv_heads;
+// The slices of token i of a request and head r of a kv head: shared ones, then own ones.
+__device__ __forceinline__ int slices_of(const Params& p, int shared, int kv_len, int pos0, int tokens, int i, int r) {
   const int groups = p.heads / p.kv_heads;
-  int token0 = 0, tokens = 0, pos0 = 0, shared = 0;
-  OwnSpan span = {0, 0, 0};
-  if (unit < p.own_units) {
-    token0 = p.q_start[b];
-    tokens = p.q_start[b + 1] - token0;
-    pos0 = p.q_pos0[b];
-    shared = min(p.prefix_len[b], p.max_prefix);
-    span = own_span(shared, p.kv_len[b], pos0, tokens, groups, row_tile);
-  }
-  const int begin = span.base + slice * p.own_keys, end = min(span.end, begin + p.own_keys);
-  if (unit >= p.own_units || row_tile * OWN_ROWS >= tokens * groups || span.end <= span.first || begin >= end) {
-    dependent_launch_wait();
-    return;
-  }
-  constexpr int TILE_BYTES = TILE_KEYS * D * 2;
-  const uint32_t mine = pae_attention::smem_u32(smem + warp * Layout<D>::OWN_BYTES);
-  const int* table = p.block_table + (size_t)b * p.table_width;
-  auto fetch = [&](int stage, int key0) {
-    const int page = checked_page(table[checked_table_index(key0 / p.page_size, p.table_width)]);
-    const size_t row0 = ((size_t)page * p.kv_heads + g) * p.page_size + key0 % p.page_size;
-    const uint32_t k_dst = mine + stage * 2 * TILE_BYTES;
-#pragma unroll
-    for (int i = lane; i < TILE_KEYS * D / 8; i += 32) {
-      const int row = i / (D / 8), c = i % (D / 8);
-      const int off = TileLayout<D>::offset_bytes(row, c);
-      cp_async16(k_dst + off, p.keys + (row0 + row) * D + c * 8);
-      cp_async16_or_zeros(k_dst + TILE_BYTES + off, p.values + (row0 + row) * D + c * 8, key0 + row >= span.first && key0 + row < end);
-    }
-  };
-  const int tiles = (end - begin + TILE_KEYS - 1) / TILE_KEYS;
-  // Tiles of earlier tokens only are asked for before the wait for the kernel before.
-  int early = 0;
-  while (early < OWN_STAGES - 1 && early < tiles && begin + (early + 1) * TILE_KEYS <= pos0) {
-    fetch(early, begin + early * TILE_KEYS);
-    cp_async_commit();
-    ++early;
-  }
-  dependent_launch_wait();
-  const int row0 = row_tile * OWN_ROWS, rows = min(OWN_ROWS, tokens * groups - row0);
-  auto token_of = [&](int r) { return (row0 + r) / groups; };
-  auto head_of = [&](int r) { return g * groups + (row0 + r) % groups; };
-  uint32_t q[D / 16][4];
-  load_query_fragments<D>(q, [&](int r) -> const __nv_bfloat16* {
-    return r < rows ? p.qkv + ((size_t)(token0 + token_of(r)) * (p.heads + 2 * p.kv_heads) + head_of(r)) * D : nullptr;
-  });
-  for (int i = early; i < OWN_STAGES - 1; ++i) {
-    if (i < tiles) fetch(i, begin + i * TILE_KEYS);
-    cp_async_commit();
-  }
-  float o[D / 8][4];
-#pragma unroll
-  for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  float row_max[2] = {-FLT_MAX, -FLT_MAX}, row_sum[2] = {0.f, 0.f};
-  int row_end[2];                            // the keys before it are visible to the row
-#pragma unroll
-  for (int half = 0; half < 2; ++half) row_end[half] = min(end, pos0 + token_of((lane >> 2) + half * 8) + 1);
-  const int all_see = min(end, pos0 + token_of(0) + 1);
-  for (int t = 0; t < tiles; ++t) {
-    const int ahead = t + OWN_STAGES - 1;
-    if (ahead < tiles) fetch(ahead % OWN_STAGES, begin + ahead * TILE_KEYS);
-    cp_async_commit();
-    cp_async_wait<OWN_STAGES - 1>();
-    __syncwarp();
-    const uint32_t k_tile = mine + (t % OWN_STAGES) * 2 * TILE_BYTES;
-    const int key0 = begin + t * TILE_KEYS;
-    float s[2][4];
-    scores_16_keys<D>(s, q, k_tile, 0);
-    uint32_t pa[4];
-    softmax_step<D>(s, row_max, row_sum, o, pa, p.scale_log2, key0 >= span.first && key0 + TILE_KEYS <= all_see,
-                    [&](int half, int key) { return key0 + key >= span.first && key0 + key < row_end[half]; });
-    accumulate_16_keys<D>(o, pa, k_tile + TILE_BYTES, 0);
-    __syncwarp();
-  }
-  cp_async_wait<0>();
-  const int slot = (shared + p.shared_keys - 1) / p.shared_keys + slice;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = (lane >> 2) + half * 8;
-    if (r >= rows) continue;
-    const size_t at = ((size_t)(token0 + token_of(r)) * p.heads + head_of(r)) * p.slots + slot;
-    float* out = p.part_out + at * D;
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) *(float2*)(out + n * 8 + (lane & 3) * 2) = make_float2(o[n][half * 2], o[n][half * 2 + 1]);
-    if ((lane & 3) == 0) {
-      p.part_max[at] = row_max[half];
-      p.part_sum[at] = row_sum[half];
-    }
-  }
-}
-
-template <int D>
-__global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constant__ PageMaps maps, const Params p) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  if ((int)blockIdx.x < p.shared_blocks) shared_slice<D>(maps, p, smem);
-  else own_slice<D>(p, smem);
+  const OwnSpan span = own_span(p, shared, kv_len, pos0, tokens, groups, (i * groups + r) / ROWS);
+  const int own = span.end > span.first ? (span.end - span.base + p.own_keys - 1) / p.own_keys : 0;
+  return min((shared + p.shared_keys - 1) / p.shared_keys + own, p.slots);
 }
 
 template <int D, int DEPTH>
@@ -536,12 +505,58 @@ __global__ void __launch_bounds__(pae_attention::MERGE_WARPS * 32) prefix_merge_
   const int shared = min(p.prefix_len[b], p.max_prefix), kv_len = p.kv_len[b], pos0 = p.q_pos0[b];
   dependent_launch_wait();
   if (i >= tokens) return;
-  const OwnSpan span = own_span(shared, kv_len, pos0, tokens, groups, (i * groups + h % groups) / OWN_ROWS);
-  int slices = (shared + p.shared_keys - 1) / p.shared_keys;
-  if (span.end > span.first) slices += (span.end - span.base + p.own_keys - 1) / p.own_keys;
-  slices = min(slices, p.slots);
+  const int slices = slices_of(p, shared, kv_len, pos0, tokens, i, h % groups);
   const size_t row = (size_t)(token0 + i) * p.heads + h, at = row * p.slots;
   pae_attention::merge_parts<D, DEPTH>(out + row * D, p.part_out + at * D, p.part_max + at, p.part_sum + at, slices, p.slots, weights);
+}
+
+// The same by one warp a row, for launches of so many rows that warps are there for all SMs: every row is in flight at once.
+template <int D>
+__global__ void __launch_bounds__(128) prefix_merge_rows_kernel(__nv_bfloat16* __restrict__ out, const Params p) {
+  dependent_launch_trigger();
+  constexpr int PER_LANE = D / 32, DEPTH = 8;
+  const int h = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, i = blockIdx.y, b = blockIdx.z;
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0;
+  const int shared = min(p.prefix_len[b], p.max_prefix), kv_len = p.kv_len[b], pos0 = p.q_pos0[b];
+  dependent_launch_wait();
+  if (i >= tokens || h >= p.heads) return;
+  const int slices = slices_of(p, shared, kv_len, pos0, tokens, i, h % groups);
+  const size_t row = (size_t)(token0 + i) * p.heads + h, at = row * p.slots;
+  const float* maxima = p.part_max + at;
+  float top = -FLT_MAX, total = 0.f;
+  for (int s = lane; s < slices; s += 32) top = fmaxf(top, maxima[s]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int s = lane; s < slices; s += 32) total += p.part_sum[at + s] * exp2f(maxima[s] - top);
+  total = warp_sum(total);
+  float acc[PER_LANE];
+#pragma unroll
+  for (int j = 0; j < PER_LANE; ++j) acc[j] = 0.f;
+  for (int s0 = 0; s0 < slices; s0 += 32) {
+    const float weight = s0 + lane < slices ? exp2f(maxima[s0 + lane] - top) : 0.f;
+    const int count = min(32, slices - s0);
+    for (int k = 0; k < count; k += DEPTH) {
+      float part[DEPTH][PER_LANE];
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) {
+        const float* from = p.part_out + (at + s0 + k + u) * D + lane * PER_LANE;
+#pragma unroll
+        for (int j = 0; j < PER_LANE; ++j) part[u][j] = k + u < count ? from[j] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) {
+        const float w = __shfl_sync(0xffffffffu, weight, (k + u) & 31);
+        if (k + u < count) {
+#pragma unroll
+          for (int j = 0; j < PER_LANE; ++j) acc[j] += part[u][j] * w;
+        }
+      }
+    }
+  }
+  const float inv = total > 0.f ? 1.f / total : 0.f;
+#pragma unroll
+  for (int j = 0; j < PER_LANE; j += 2)
+    *(__nv_bfloat162*)(out + row * D + lane * PER_LANE + j) = __floats2bfloat162_rn(acc[j] * inv, acc[j + 1] * inv);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -549,27 +564,36 @@ __global__ void __launch_bounds__(pae_attention::MERGE_WARPS * 32) prefix_merge_
 // ---------------------------------------------------------------------------------------
 struct Cut {
   int row_tiles, shared_slices, shared_keys, own_row_tiles, own_slices, own_keys, slots;
-  long long shared_blocks, own_units;
+  long long shared_blocks, own_blocks;
 };
-// Two blocks of either kind share an SM. The own slices are as many as the warps of that many blocks, of 32 keys at least; the shared slices as many as
-// fill what the own blocks leave of one wave (three quarters of it at least), of two tiles at least.
-Cut cut_keys(int seqs, int groups, int heads, int kv_heads, int max_q_len, int max_prefix, int max_own, int max_group_tokens) {
+// Two blocks share an SM. Own keys are cut into as many slices as fill a wave, of one tile at least and OWN_TILES at most. The shared keys' blocks fill
+// that share of one wave that their tiles are of all tiles (a request's own keys taken as half of the longest's), half of it at least: what is left
+// goes to the own blocks, which wait for memory while the others compute. 64 requests, 8,000 shared and 20 to 700 own keys, 28 heads over 4 of
+// 128, us with the merge: 37.6 with the wave full of shared blocks, 36.2 with three quarters, 33.5 with half; 24 requests of five
+// tokens, 30,011 shared and 100 to 900 own keys, 40 heads over 8: 94.8, 112 and 154.
+constexpr int SHARED_TILES = 2;   // of a slice at least
+constexpr int OWN_TILES = 12;
+Cut cut_keys(int seqs, int groups, int heads, int kv_heads, int page_size, int max_q_len, int max_prefix, int max_own, int max_group_tokens) {
   const int share = heads / kv_heads, wave = 2 * pae_attention::multiprocessors();
   Cut c;
   c.row_tiles = (int)(((long long)max_group_tokens * share + ROWS - 1) / ROWS);
-  c.own_row_tiles = (int)(((long long)max_q_len * share + OWN_ROWS - 1) / OWN_ROWS);
+  c.own_row_tiles = (int)(((long long)max_q_len * share + ROWS - 1) / ROWS);
   const long long pairs = (long long)seqs * kv_heads * c.own_row_tiles;
-  const int own = max_own + TILE_KEYS - 1;               // a span may begin inside a tile
-  long long most = (long long)wave * OWN_WARPS / pairs;
-  if (most > (own + 31) / 32) most = (own + 31) / 32;
+  const int own_tiles = (max_own + (page_size < BKEYS ? page_size : BKEYS) - 1 + BKEYS - 1) / BKEYS;     // a span may begin inside a box
+  long long most = wave / pairs;
+  if (most < (own_tiles + OWN_TILES - 1) / OWN_TILES) most = (own_tiles + OWN_TILES - 1) / OWN_TILES;
+  if (most > own_tiles) most = own_tiles;
   if (most < 1) most = 1;
-  c.own_keys = (int)(((own + most - 1) / most + TILE_KEYS - 1) / TILE_KEYS * TILE_KEYS);
-  c.own_slices = (own + c.own_keys - 1) / c.own_keys;
-  c.own_units = pairs * c.own_slices;
-  const long long per_slice = (long long)groups * kv_heads * c.row_tiles, own_blocks = (c.own_units + OWN_WARPS - 1) / OWN_WARPS;
+  c.own_keys = own_tiles > 0 ? (int)((own_tiles + most - 1) / most) * BKEYS : BKEYS;
+  c.own_slices = own_tiles > 0 ? (own_tiles * BKEYS + c.own_keys - 1) / c.own_keys : 1;
+  c.own_blocks = pairs * c.own_slices;
+  const long long per_slice = (long long)groups * kv_heads * c.row_tiles;
   const int tiles = (max_prefix + BKEYS - 1) / BKEYS;
-  long long slices = (wave - (own_blocks < wave / 4 ? own_blocks : wave / 4)) / per_slice;
-  if (slices > (tiles + 1) / 2) slices = (tiles + 1) / 2;
+  const double shared_work = (double)per_slice * tiles, own_work = 0.5 * pairs * own_tiles;
+  const double blocks = wave * fmax(0.5, shared_work / fmax(1.0, shared_work + own_work));
+  long long slices = (long long)(blocks / per_slice + 0.5);
+  while (slices > 1 && slices * per_slice > wave) --slices;
+  if (slices > (tiles + SHARED_TILES - 1) / SHARED_TILES) slices = (tiles + SHARED_TILES - 1) / SHARED_TILES;
   if (slices < 1) slices = 1;
   const int slice_tiles = tiles > 0 ? (int)((tiles + slices - 1) / slices) : 1;
   c.shared_keys = slice_tiles * BKEYS;
@@ -580,14 +604,17 @@ Cut cut_keys(int seqs, int groups, int heads, int kv_heads, int max_q_len, int m
 }
 
 template <int D>
-int launch(const Params& p, void* out, long long pages, int seqs, int max_q_len, cudaStream_t s) {
+int launch(const Params& p, void* out, long long pages, int blocks, int seqs, int max_q_len, cudaStream_t s) {
   PageMaps maps;
   if (int err = encode_page_maps(&maps, p.keys, p.values, pages, p.kv_heads, p.page_size, D, BKEYS)) return err;
   static DevicesSet devices;
   if (int err = raise_shared_memory(devices, prefix_kernel<D>, Layout<D>::SMEM_BYTES, "paged_attention_prefix")) return err;
-  const int own_blocks = (p.own_units + OWN_WARPS - 1) / OWN_WARPS;
-  launch_kernel(prefix_kernel<D>, dim3(p.shared_blocks + own_blocks), dim3(THREADS), Layout<D>::SMEM_BYTES, s, maps, p);
+  launch_kernel(prefix_kernel<D>, dim3(blocks), dim3(THREADS), Layout<D>::SMEM_BYTES, s, maps, p);
   if (int err = check_launch("paged_attention_prefix")) return err;
+  if ((long long)p.heads * max_q_len * seqs >= 8LL * pae_attention::multiprocessors()) {
+    launch_kernel(prefix_merge_rows_kernel<D>, dim3((p.heads + 3) / 4, max_q_len, seqs), dim3(128), 0, s, (__nv_bfloat16*)out, p);
+    return check_launch("paged_attention_prefix");
+  }
   const auto merge = pae_attention::merge_in_few_registers(p.heads * max_q_len, seqs, p.slots) ? prefix_merge_kernel<D, 8> : prefix_merge_kernel<D, 24>;
   launch_kernel(merge, dim3(p.heads, max_q_len, seqs), dim3(pae_attention::MERGE_WARPS * 32),
                 (p.slots + pae_attention::MERGE_WARPS * D) * sizeof(float), s, (__nv_bfloat16*)out, p);
@@ -603,9 +630,9 @@ PAE_EXPORT int pae_attention_prefix_supports(int heads, int kv_heads, int d, int
 }
 
 // Floats of scratch that pae_paged_attention_prefix needs for the same sizes.
-PAE_EXPORT long long pae_attention_prefix_floats(int tokens, int seqs, int groups, int heads, int kv_heads, int d, int max_q_len, int max_prefix, int max_own,
-                                                 int max_group_tokens) {
-  const Cut c = cut_keys(seqs, groups, heads, kv_heads, max_q_len, max_prefix, max_own, max_group_tokens);
+PAE_EXPORT long long pae_attention_prefix_floats(int tokens, int seqs, int groups, int heads, int kv_heads, int d, int page_size, int max_q_len, int max_prefix,
+                                                 int max_own, int max_group_tokens) {
+  const Cut c = cut_keys(seqs, groups, heads, kv_heads, page_size, max_q_len, max_prefix, max_own, max_group_tokens);
   return (long long)tokens * heads * c.slots * (d + 2);
 }
 
@@ -620,9 +647,9 @@ PAE_EXPORT int pae_paged_attention_prefix(void* out, const void* qkv, const void
   if (seqs > 65535 || max_q_len > 65535) return fail(3, "paged_attention_prefix: %d requests of up to %d tokens exceed one launch", seqs, max_q_len);
   if ((((uintptr_t)qkv | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)out | (uintptr_t)scratch) & 15) != 0)
     return fail(2, "paged_attention_prefix: an operand does not start on a 16-byte boundary");
-  const Cut c = cut_keys(seqs, groups, heads, kv_heads, max_q_len, max_prefix, max_own, max_group_tokens);
-  if ((size_t)(c.slots + pae_attention::MERGE_WARPS * d) * sizeof(float) > 40 * 1024 || c.shared_blocks + c.own_units > 0x7fffffffll)
-    return fail(3, "paged_attention_prefix: %d slices a row, %lld blocks and %lld warps exceed one launch", c.slots, c.shared_blocks, c.own_units);
+  const Cut c = cut_keys(seqs, groups, heads, kv_heads, page_size, max_q_len, max_prefix, max_own, max_group_tokens);
+  if ((size_t)(c.slots + pae_attention::MERGE_WARPS * d) * sizeof(float) > 40 * 1024 || c.shared_blocks + c.own_blocks > 0x7fffffffll)
+    return fail(3, "paged_attention_prefix: %d slices a row, %lld + %lld blocks exceed one launch", c.slots, c.shared_blocks, c.own_blocks);
   Params p = {};
   p.qkv = (const __nv_bfloat16*)qkv;
   p.keys = (const __nv_bfloat16*)keys;
@@ -646,14 +673,13 @@ PAE_EXPORT int pae_paged_attention_prefix(void* out, const void* qkv, const void
   p.row_tiles = c.row_tiles;
   p.shared_slices = c.shared_slices;
   p.shared_keys = c.shared_keys;
-  p.own_units = (int)c.own_units;
   p.own_row_tiles = c.own_row_tiles;
   p.own_slices = c.own_slices;
   p.own_keys = c.own_keys;
   p.slots = c.slots;
   p.scale_log2 = scale * LOG2E;
-  p.slack = c.shared_blocks >= 2LL * pae_attention::multiprocessors() ? REFERENCE_SLACK : 0.f;
+  p.slack = REFERENCE_SLACK;
   p.error = error;
-  if (d == 64) return launch<64>(p, out, pages, seqs, max_q_len, (cudaStream_t)stream);
-  return launch<128>(p, out, pages, seqs, max_q_len, (cudaStream_t)stream);
+  if (d == 64) return launch<64>(p, out, pages, (int)(c.shared_blocks + c.own_blocks), seqs, max_q_len, (cudaStream_t)stream);
+  return launch<128>(p, out, pages, (int)(c.shared_blocks + c.own_blocks), seqs, max_q_len, (cudaStream_t)stream);
 }

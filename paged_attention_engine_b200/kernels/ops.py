@@ -2388,8 +2388,8 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     if info is not None:
         info.update(kernel="shared")
     out = torch.empty((tokens, num_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
-    scratch = torch.empty(lib.pae_attention_prefix_floats(tokens, seqs, groups, num_heads, num_kv_heads, head_dim, max_q_len, max_prefix_len, max_own_len,
-                                                          max_group_tokens), dtype=torch.float32, device=qkv.device)
+    scratch = torch.empty(lib.pae_attention_prefix_floats(tokens, seqs, groups, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_prefix_len,
+                                                          max_own_len, max_group_tokens), dtype=torch.float32, device=qkv.device)
     _set_bounds("attention_prefix", keys)
     _check(lib, lib.pae_paged_attention_prefix(
         out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), keys.shape[0], block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
