@@ -8,8 +8,9 @@
 //            values and weights alike. Rows from min(n, budget) on are left as they are.
 //
 // choose is a selection by digits: a weight becomes a 32-bit number of the same order (NaN above all
-// numbers, -0 as 0, the protected keys above both, so one rule decides), and four passes over the row in shared memory find the budget-th
-// largest, eight bits a pass, from counts per digit. Long rows are shared out over a cluster of blocks, whose
+// numbers, -0 as 0, the protected keys above both, so one rule decides), and three passes over the row in shared memory find the budget-th
+// largest, eleven, eleven and ten bits a pass, from counts per digit (with eight bits first the weights of a row, whose exponents differ little, fall into a handful
+// of digits, and the counts are waited for: 24 us for 48 requests of 2,900 keys and 4 kv heads, now 13). Long rows are shared out over a cluster of blocks, whose
 // counts are summed through distributed shared memory in the order of the ranks. Then each warp takes a run of neighbouring keys, counts
 // what stays of it, and writes its indices behind those of the runs before. Nothing depends on timing.
 //
@@ -25,9 +26,12 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int CHOOSE_THREADS = 512;
+constexpr int CHOOSE_THREADS = 1024;
 constexpr int CHOOSE_WARPS = CHOOSE_THREADS / 32;
-constexpr int COPIES = 4;                  // of the counts per digit, each fed by every fourth warp
+static_assert(CHOOSE_WARPS == 32, "a warp scans the warps' sums; a thread stands for two digits");
+constexpr int DIGITS = 2048;
+constexpr int MOST_STAGED = 47 * 1024;      // of a row's keys in a block's shared memory
+constexpr int COPIES = 2;                  // of the counts per digit, each fed by every other warp
 
 // A number of the same order as the weight: negative numbers' bits are complemented, the others' get the sign bit. 0 stands behind all of them.
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -43,14 +47,15 @@ struct ChooseParams {
   int* kept;                // [requests, kv_heads, budget]
   int table_width, kv_heads, page_size, budget, keep_first, keep_last, max_kv_len;
   int staged;               // keys per block that shared memory holds
+  int fours;                // whether four neighbouring weights can be read at once
 };
 
-__global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const ChooseParams p) {
+__global__ void __launch_bounds__(CHOOSE_THREADS, 2) choose_kernel(const ChooseParams p) {
   cg::cluster_group cluster = cg::this_cluster();
-  extern __shared__ uint32_t order[];                     // [staged]
-  __shared__ uint32_t counts[COPIES][256];
-  __shared__ uint32_t block_counts[256];                  // read by the other blocks of the cluster
-  __shared__ uint32_t scan[8];
+  extern __shared__ __align__(16) uint32_t order[];       // [staged, rounded up to fours]: zeros behind the last
+  __shared__ uint2 counts[COPIES][DIGITS / 2];
+  __shared__ uint2 block_counts[2][DIGITS / 2];           // read by the other blocks of the cluster, which may be one pass behind
+  __shared__ uint32_t scan[CHOOSE_WARPS];
   __shared__ uint32_t chosen[2];                          // the digit, and how many of the rest are still to be taken
   __shared__ uint32_t warp_above[CHOOSE_WARPS], warp_equal[CHOOSE_WARPS];
   __shared__ uint32_t block_above, block_equal;           // likewise
@@ -65,7 +70,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const ChoosePara
     for (int i = rank * CHOOSE_THREADS + tid; i < p.budget; i += ranks * CHOOSE_THREADS) kept[i] = i < n ? i : -1;
     return;
   }
-  const int share = (n + ranks - 1) / ranks;
+  const int share = ((n + ranks - 1) / ranks + 3) & ~3;
   const int begin = min(rank * share, n), mine = min(share, n - begin);
   const int* table = p.block_table + (size_t)b * p.table_width;
   auto look_up = [&](int i) -> uint32_t {
@@ -75,62 +80,127 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const ChoosePara
     return order_of(p.mass[((size_t)page * p.kv_heads + g) * p.page_size + j % p.page_size]);
   };
   const int staged = min(mine, p.staged);
-  for (int i = tid; i < staged; i += CHOOSE_THREADS) order[i] = look_up(i);
-  auto at = [&](int i) { return i < staged ? order[i] : look_up(i); };
+  if (p.fours) {
+    // Four neighbouring weights at a time, several times four under way.
+    constexpr int DEPTH = 2;
+    for (int i0 = tid * 4; i0 < staged; i0 += CHOOSE_THREADS * 4 * DEPTH) {
+      float4 w[DEPTH];
+      int pages[DEPTH];
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) {
+        const int i = i0 + u * CHOOSE_THREADS * 4;
+        pages[u] = i < staged ? checked_page(table[checked_table_index((begin + i) / p.page_size, p.table_width)]) : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) {
+        const int i = i0 + u * CHOOSE_THREADS * 4;
+        if (i < staged) w[u] = *(const float4*)(p.mass + ((size_t)pages[u] * p.kv_heads + g) * p.page_size + (begin + i) % p.page_size);
+      }
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) {
+        const int i = i0 + u * CHOOSE_THREADS * 4;
+        const float four[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = begin + i + k;
+          if (i + k < staged) order[i + k] = j < p.keep_first || j >= n - p.keep_last ? 0xFFFFFFFFu : order_of(four[k]);
+        }
+      }
+    }
+  } else {
+    for (int i = tid; i < staged; i += CHOOSE_THREADS) order[i] = look_up(i);
+  }
+  if (tid < (-staged & 3)) order[staged + tid] = 0u;
+  // Calls f(number) for the block's keys, four at a time from shared memory (with up to three zeros, which no weight is), the rest as they lie.
+  auto for_each = [&](auto f) {
+    for (int i = tid * 4; i < staged; i += CHOOSE_THREADS * 4) {
+      const uint4 v = *(const uint4*)(order + i);
+      f(v.x);
+      f(v.y);
+      f(v.z);
+      f(v.w);
+    }
+    for (int i = staged + tid; i < mine; i += CHOOSE_THREADS) f(look_up(i));
+  };
 
   // ---- the budget-th largest, digit by digit
   uint32_t prefix = 0, left = (uint32_t)p.budget;         // of the numbers that begin with `prefix`, the left-th largest
 #pragma unroll 1
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < COPIES * 256; i += CHOOSE_THREADS) (&counts[0][0])[i] = 0;
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), digits = pass == 2 ? 1024 : 2048;
+    for (int i = tid; i < COPIES * DIGITS / 2; i += CHOOSE_THREADS) (&counts[0][0])[i] = make_uint2(0, 0);
     __syncthreads();
-    for (int i = tid; i < mine; i += CHOOSE_THREADS) {
-      const uint32_t v = at(i);
-      if (shift == 24 || (v >> (shift + 8)) == prefix) atomicAdd(&counts[warp & (COPIES - 1)][(v >> shift) & 255u], 1u);
-    }
+    uint32_t* mine_counts = (uint32_t*)counts[warp & (COPIES - 1)];
+    const int above_shift = pass == 1 ? 21 : 10;
+    for_each([&](uint32_t v) {
+      if (pass == 0 || (v >> above_shift) == prefix) atomicAdd(&mine_counts[(v >> shift) & (digits - 1)], 1u);
+    });
     __syncthreads();
-    if (tid < 256) {
-      uint32_t sum = 0;
+    // Thread t stands for digits 2 (1023 - t) and the one above: how many numbers have a larger digit, by a scan.
+    const int pair = DIGITS / 2 - 1 - tid;
+    uint2 sum = counts[0][pair];
 #pragma unroll
-      for (int c = 0; c < COPIES; ++c) sum += counts[c][tid];
-      block_counts[tid] = sum;
+    for (int c = 1; c < COPIES; ++c) {
+      sum.x += counts[c][pair].x;
+      sum.y += counts[c][pair].y;
     }
-    if (ranks > 1) cluster.sync(); else __syncthreads();
-    // Thread t stands for digit 255 - t: how many numbers have a larger digit, by a scan.
-    uint32_t count = 0, before = 0;
-    if (tid < 256) {
-      for (int r = 0; r < ranks; ++r) count += cluster.map_shared_rank(block_counts, r)[255 - tid];
-      uint32_t inclusive = count;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t other = __shfl_up_sync(0xffffffffu, inclusive, o);
-        if (lane >= o) inclusive += other;
-      }
-      if (lane == 31) scan[warp] = inclusive;
-      before = inclusive - count;
-    }
-    __syncthreads();
-    if (tid < 256) {
-      for (int w = 0; w < warp; ++w) before += scan[w];
-      if (before < left && left <= before + count) {      // one thread
-        chosen[0] = 255u - tid;
-        chosen[1] = left - before;
+    if (ranks > 1) {
+      block_counts[pass & 1][pair] = sum;
+      cluster.sync();
+      for (int r = 1; r < ranks; ++r) {
+        const uint2 theirs = cluster.map_shared_rank(block_counts[pass & 1], (rank + r) % ranks)[pair];
+        sum.x += theirs.x;
+        sum.y += theirs.y;
       }
     }
-    if (ranks > 1) cluster.sync(); else __syncthreads();  // nobody writes its counts again before all have read them
-    prefix = (prefix << 8) | chosen[0];
+    uint32_t inclusive = sum.x + sum.y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t other = __shfl_up_sync(0xffffffffu, inclusive, o);
+      if (lane >= o) inclusive += other;
+    }
+    if (lane == 31) scan[warp] = inclusive;
+    __syncthreads();
+    uint32_t totals = scan[lane];                         // of the warps, scanned by every warp
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t other = __shfl_up_sync(0xffffffffu, totals, o);
+      if (lane >= o) totals += other;
+    }
+    const uint32_t earlier = __shfl_sync(0xffffffffu, totals, max(warp - 1, 0));
+    const uint32_t before = (warp > 0 ? earlier : 0u) + inclusive - sum.x - sum.y;
+    if (before < left && left <= before + sum.y) {        // one thread, one of its two digits
+      chosen[0] = 2u * pair + 1u;
+      chosen[1] = left - before;
+    } else if (before + sum.y < left && left <= before + sum.y + sum.x) {
+      chosen[0] = 2u * pair;
+      chosen[1] = left - before - sum.y;
+    }
+    __syncthreads();
+    prefix = pass == 0 ? chosen[0] : (prefix << (pass == 1 ? 11 : 10)) | chosen[0];
     left = chosen[1];
   }
   // All numbers above `prefix` stay, and of its equals the first `left`.
 
   // ---- the indices, in ascending order: a warp takes a run of keys
-  const int run = (((mine + CHOOSE_WARPS - 1) / CHOOSE_WARPS) + 31) & ~31;
+  const int run = (((mine + CHOOSE_WARPS - 1) / CHOOSE_WARPS) + 127) & ~127;
   const int first = min(warp * run, mine), last = min(first + run, mine);
+  auto four_at = [&](int i) {              // of a lane; zeros behind the run
+    if (i < staged && i < last) return *(const uint4*)(order + i);
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (i < last) {
+      v.x = look_up(i);
+      if (i + 1 < last) v.y = look_up(i + 1);
+      if (i + 2 < last) v.z = look_up(i + 2);
+      if (i + 3 < last) v.w = look_up(i + 3);
+    }
+    return v;
+  };
   uint32_t above = 0, equal = 0;
-  for (int i = first + lane; i < last; i += 32) {
-    const uint32_t v = at(i);
-    above += v > prefix;
-    equal += v == prefix;
+  for (int i = first + lane * 4; i < last; i += 128) {
+    const uint4 v = four_at(i);
+    above += (v.x > prefix) + (v.y > prefix) + (v.z > prefix) + (v.w > prefix);
+    equal += (v.x == prefix) + (v.y == prefix) + (v.z == prefix) + (v.w == prefix);
   }
   above = __reduce_add_sync(0xffffffffu, above);
   equal = __reduce_add_sync(0xffffffffu, equal);
@@ -139,35 +209,49 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const ChoosePara
     warp_equal[warp] = equal;
   }
   __syncthreads();
-  if (tid == 0) {
-    uint32_t a = 0, e = 0;
-    for (int w = 0; w < CHOOSE_WARPS; ++w) {
-      a += warp_above[w];
-      e += warp_equal[w];
+  const uint32_t all_above = warp_above[lane], all_equal = warp_equal[lane];
+  if (ranks > 1) {
+    if (warp == 0) {
+      const uint32_t a = __reduce_add_sync(0xffffffffu, all_above), e = __reduce_add_sync(0xffffffffu, all_equal);
+      if (lane == 0) {
+        block_above = a;
+        block_equal = e;
+      }
     }
-    block_above = a;
-    block_equal = e;
+    cluster.sync();
   }
-  if (ranks > 1) cluster.sync(); else __syncthreads();
-  uint32_t above_before = 0, equal_before = 0;
+  uint32_t above_before = __reduce_add_sync(0xffffffffu, lane < warp ? all_above : 0u);
+  uint32_t equal_before = __reduce_add_sync(0xffffffffu, lane < warp ? all_equal : 0u);
   for (int r = 0; r < rank; ++r) {
     above_before += *cluster.map_shared_rank(&block_above, r);
     equal_before += *cluster.map_shared_rank(&block_equal, r);
   }
-  for (int w = 0; w < warp; ++w) {
-    above_before += warp_above[w];
-    equal_before += warp_equal[w];
-  }
-  const uint32_t below_me = (1u << lane) - 1u;
-  for (int i0 = first; i0 < last; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t v = i < last ? at(i) : 0u;
-    const bool is_above = i < last && v > prefix, is_equal = i < last && v == prefix;
-    const uint32_t a = __ballot_sync(0xffffffffu, is_above), e = __ballot_sync(0xffffffffu, is_equal);
-    const uint32_t equals = equal_before + __popc(e & below_me);
-    if (is_above || (is_equal && equals < left)) kept[above_before + __popc(a & below_me) + min(equals, left)] = begin + i;
-    above_before += __popc(a);
-    equal_before += __popc(e);
+  for (int i0 = first; i0 < last; i0 += 128) {
+    const int i = i0 + lane * 4;
+    const uint4 v = four_at(i);
+    const uint32_t four[4] = {v.x, v.y, v.z, v.w};
+    uint32_t count = 0;                      // above in the low half, equal in the high one: at most 128 of each
+#pragma unroll
+    for (int k = 0; k < 4; ++k) count += (four[k] > prefix ? 1u : 0u) + (four[k] == prefix ? 0x10000u : 0u);
+    uint32_t inclusive = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t other = __shfl_up_sync(0xffffffffu, inclusive, o);
+      if (lane >= o) inclusive += other;
+    }
+    uint32_t a = above_before + ((inclusive - count) & 0xFFFFu), e = equal_before + ((inclusive - count) >> 16);
+    if (count != 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool is_equal = four[k] == prefix;
+        if (four[k] > prefix || (is_equal && e < left)) kept[a + min(e, left)] = begin + i + k;
+        a += four[k] > prefix;
+        e += is_equal;
+      }
+    }
+    const uint32_t all = __shfl_sync(0xffffffffu, inclusive, 31);
+    above_before += all & 0xFFFFu;
+    equal_before += all >> 16;
   }
   if (ranks > 1) cluster.sync();                          // no block leaves while its counts may be read
 }
@@ -175,8 +259,8 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const ChoosePara
 // ---------------------------------------------------------------------------------------
 // compact
 // ---------------------------------------------------------------------------------------
-constexpr int COMPACT_THREADS = 256;
 constexpr int IN_FLIGHT = 8;               // rows' pieces that a thread reads before it writes
+constexpr int MOST_ROWS = 2048;            // of a chunk
 
 struct CompactParams {
   uint8_t* pools[3];        // keys, values, weights: [pages, kv_heads, page_size] rows of row_units[i] units
@@ -188,50 +272,61 @@ struct CompactParams {
   int table_width, kv_heads, page_size, budget;
 };
 
-template <typename Unit>
-__device__ __forceinline__ void compact_strip(const CompactParams& p, int pool, int strip) {
+// Where a chunk's rows come from and go to, as row numbers of the pool (pages * kv_heads * page_size of them), found by one thread a row while the chunk before is
+// on its way; -1: the row does not move.
+template <int THREADS, typename Unit>
+__device__ __forceinline__ void compact_strip(const CompactParams& p, int pool, int strip, int2 (*moves)[MOST_ROWS]) {
   const int g = blockIdx.y, b = blockIdx.z;
   const int n = min(p.kv_len[b], p.table_width * p.page_size);
   const int places = min(n, p.budget);
   const int* kept = p.kept + ((size_t)b * p.kv_heads + g) * p.budget;
   const int* table = p.block_table + (size_t)b * p.table_width;
   const int units = p.row_units[pool], width = min(p.strip_units[pool], units - strip * p.strip_units[pool]);
-  const int rows_a_pass = COMPACT_THREADS / width;
+  const int rows_a_pass = min(THREADS / width, MOST_ROWS / IN_FLIGHT), chunk_rows = rows_a_pass * IN_FLIGHT;
   const int my_row = threadIdx.x / width, my_unit = strip * p.strip_units[pool] + threadIdx.x % width;
-  Unit* base = (Unit*)p.pools[pool];
-  auto unit_at = [&](int i) {
+  Unit* base = (Unit*)p.pools[pool] + my_unit;
+  auto row_of = [&](int i) {
     const int page = checked_page(table[checked_table_index(i / p.page_size, p.table_width)]);
-    return base + (((size_t)page * p.kv_heads + g) * p.page_size + i % p.page_size) * units + my_unit;
+    return (page * p.kv_heads + g) * p.page_size + i % p.page_size;
   };
-  for (int chunk = 0; chunk < places; chunk += rows_a_pass * IN_FLIGHT) {
+  auto find = [&](int chunk, int2* to) {
+    for (int r = threadIdx.x; r < chunk_rows; r += THREADS) {
+      const int i = chunk + r, from = i < places ? kept[i] : -1;
+      to[r] = from > i && from < n ? make_int2(row_of(from), row_of(i)) : make_int2(-1, 0);
+    }
+  };
+  find(0, moves[0]);
+  __syncthreads();
+  for (int chunk = 0, turn = 0; chunk < places; chunk += chunk_rows, turn ^= 1) {
     Unit held[IN_FLIGHT];
-    bool moves[IN_FLIGHT];
+    int to[IN_FLIGHT];
 #pragma unroll
     for (int u = 0; u < IN_FLIGHT; ++u) {
-      const int i = chunk + u * rows_a_pass + my_row;
-      const int from = my_row < rows_a_pass && i < places ? kept[i] : -1;
-      moves[u] = from > i && from < n;
-      if (moves[u]) held[u] = *unit_at(from);
+      const int2 move = my_row < rows_a_pass ? moves[turn][u * rows_a_pass + my_row] : make_int2(-1, 0);
+      to[u] = move.x >= 0 ? move.y : -1;
+      if (move.x >= 0) held[u] = base[(size_t)move.x * units];
     }
-    __syncthreads();                       // the whole chunk is read
+    if (chunk + chunk_rows < places) find(chunk + chunk_rows, moves[turn ^ 1]);
+    __syncthreads();                       // the whole chunk is read, and the next one's rows are found
 #pragma unroll
     for (int u = 0; u < IN_FLIGHT; ++u)
-      if (moves[u]) *unit_at(chunk + u * rows_a_pass + my_row) = held[u];
+      if (to[u] >= 0) base[(size_t)to[u] * units] = held[u];
   }
 }
 
-template <typename Unit>
-__global__ void __launch_bounds__(COMPACT_THREADS) compact_kernel(const CompactParams p) {
+template <int THREADS, typename Unit>
+__global__ void __launch_bounds__(THREADS) compact_kernel(const CompactParams p) {
   // The next kernel is not let go early: an attention that follows directly fetches keys of earlier tokens before it waits for
   // the kernel before it (common.cuh), and those are what is written here.
   dependent_launch_wait();
+  __shared__ int2 moves[2][MOST_ROWS];
   int strip = blockIdx.x;
   if (strip < p.strips[0]) {
-    compact_strip<Unit>(p, 0, strip);
+    compact_strip<THREADS, Unit>(p, 0, strip, moves);
   } else if ((strip -= p.strips[0]) < p.strips[1]) {
-    compact_strip<Unit>(p, 1, strip);
+    compact_strip<THREADS, Unit>(p, 1, strip, moves);
   } else {
-    compact_strip<uint32_t>(p, 2, 0);
+    compact_strip<THREADS, uint32_t>(p, 2, 0, moves);
   }
   __threadfence();
 }
@@ -244,14 +339,16 @@ PAE_EXPORT int pae_choose_kept(int* kept, const float* mass, const int* block_ta
                                int page_size, int budget, int keep_first, int keep_last, int max_kv_len, void* stream) {
   if (seqs < 1 || kv_heads < 1) return 0;
   if (kv_heads > 65535 || seqs > 65535) return fail(1, "choose_kept: %d requests of %d kv heads, at most 65535 of each", seqs, kv_heads);
+  // A cluster's barriers and counts cost some 2 us a pass: one block a row of up to 16,384 keys (9,000 keys, 2 rows: 12.3 us, in clusters of two 13.1, of four 16.4), more
+  // where all of them still have an SM each (64,000 keys: 8 rows 27.0 us in two blocks, 21.4 in four; 48 rows 31.5 and 40.6), and as many as hold the row.
   int ranks = 1;
-  while (ranks < 8 && (long long)seqs * kv_heads * ranks < 148 && max_kv_len > 2048 * ranks) ranks *= 2;
-  while (ranks < 8 && max_kv_len > 16384 * ranks) ranks *= 2;
-  ChooseParams p = {mass, block_table, kv_len, kept, table_width, kv_heads, page_size, budget, keep_first, keep_last, max_kv_len, 0};
-  p.staged = min(48 * 1024, (max_kv_len + ranks - 1) / ranks);
+  while (ranks < 8 && max_kv_len > 16384 * ranks && (long long)seqs * kv_heads * ranks * 2 <= 148) ranks *= 2;
+  while (ranks < 8 && max_kv_len > MOST_STAGED * ranks) ranks *= 2;
+  ChooseParams p = {mass, block_table, kv_len, kept, table_width, kv_heads, page_size, budget, keep_first, keep_last, max_kv_len, 0, page_size % 4 == 0 && (uintptr_t)mass % 16 == 0};
+  p.staged = min(MOST_STAGED, ((max_kv_len + ranks - 1) / ranks + 3) & ~3);      // fours, as a block's share is
   const size_t smem = (size_t)p.staged * 4;
   static DevicesSet devices;
-  if (int code = raise_shared_memory(devices, choose_kernel, 48 * 1024 * 4, "choose_kept")) return code;
+  if (int code = raise_shared_memory(devices, choose_kernel, MOST_STAGED * 4, "choose_kept")) return code;
   launch_kernel_cluster(choose_kernel, dim3(ranks, kv_heads, seqs), dim3(CHOOSE_THREADS), smem, (cudaStream_t)stream, ranks, p);
   return check_launch("choose_kept");
 }
@@ -273,17 +370,27 @@ PAE_EXPORT int pae_compact_kept(void* keys, void* values, float* mass, const int
   p.page_size = page_size;
   p.budget = budget;
   const int bytes[3] = {key_bytes, values != nullptr ? value_bytes : 0, mass != nullptr ? 4 : 0};
+  // A row's bytes in strips of 256: pieces of a row that are moved at different times cost the memory another row activation each. So blocks of 1,024 threads
+  // where 256 would leave too little under way; narrower strips only for launches of few rows.
+  const long long pairs = (long long)seqs * kv_heads;
+  auto strips_of = [&](int bytes) { return pairs * ((key_bytes + bytes - 1) / bytes + (value_bytes + bytes - 1) / bytes); };
+  int strip_bytes = 256;
+  bool wide = strips_of(256) < 296;
+  while (strip_bytes > 32 && strips_of(strip_bytes) < 74) strip_bytes /= 2;
+  if (strip_bytes < 64) wide = false;
   int blocks = 0;
   for (int i = 0; i < 3; ++i) {
     p.row_units[i] = bytes[i] / (i < 2 ? unit : 4);
-    p.strip_units[i] = min(i < 2 ? max(1, 64 / unit) : 1, max(1, p.row_units[i]));
+    p.strip_units[i] = min(i < 2 ? max(1, strip_bytes / unit) : 1, max(1, p.row_units[i]));
     p.strips[i] = (p.row_units[i] + p.strip_units[i] - 1) / p.strip_units[i];
     blocks += p.strips[i];
   }
   if (blocks == 0) return 0;
-  const dim3 grid(blocks, kv_heads, seqs), threads(COMPACT_THREADS);
-  if (unit == 16) launch_kernel(compact_kernel<uint4>, grid, threads, 0, (cudaStream_t)stream, p);
-  else if (unit == 4) launch_kernel(compact_kernel<uint32_t>, grid, threads, 0, (cudaStream_t)stream, p);
-  else launch_kernel(compact_kernel<uint16_t>, grid, threads, 0, (cudaStream_t)stream, p);
+  const dim3 grid(blocks, kv_heads, seqs);
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (unit == 16 && wide) launch_kernel(compact_kernel<1024, uint4>, grid, dim3(1024), 0, s, p);
+  else if (unit == 16) launch_kernel(compact_kernel<256, uint4>, grid, dim3(256), 0, s, p);
+  else if (unit == 4) launch_kernel(compact_kernel<256, uint32_t>, grid, dim3(256), 0, s, p);
+  else launch_kernel(compact_kernel<256, uint16_t>, grid, dim3(256), 0, s, p);
   return check_launch("compact_kept");
 }

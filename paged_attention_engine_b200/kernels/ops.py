@@ -2306,10 +2306,17 @@ def expert_combine(y, plan: ExpertPlan, weights, x, base=None, base_gate=None) -
 # ----------------------------------------------------------------------------------- #
 # attention over the paged cache of requests that share a prefix; attention that adds up its weights per key, and eviction by them
 
-def _here(what: str, **tensors) -> None:
+def _here(what: str, names: tuple, *tensors) -> None:
     """All of the tensors lie, contiguous, on the current device (whose stream the kernels are launched on)."""
+    device = tensors[0].get_device()
+    if device >= 0 and device == torch.cuda.current_device():
+        for t in tensors:
+            if t.get_device() != device or not t.is_contiguous():
+                break
+        else:
+            return
     device = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    for name, t in tensors.items():
+    for name, t in zip(names, tensors):
         if not t.is_cuda:
             raise KernelError(f"{what}: {name} is not on a CUDA device")
         if t.get_device() != device:
@@ -2326,15 +2333,25 @@ def _int32(what: str, **tensors) -> None:
 
 def _need_tables(what: str, block_table, kv_len) -> int:
     """The number of requests of a block table [requests, pages] and their lengths."""
-    _int32(what, block_table=block_table, kv_len=kv_len)
+    if block_table.dtype is not torch.int32 or kv_len.dtype is not torch.int32:
+        _int32(what, block_table=block_table, kv_len=kv_len)
     if block_table.dim() != 2 or block_table.shape[1] < 1 or kv_len.dim() != 1 or kv_len.shape[0] != block_table.shape[0]:
         raise KernelError(f"{what}: block tables {tuple(block_table.shape)} for lengths {tuple(kv_len.shape)}")
     return kv_len.shape[0]
 
 
+_STEP_TENSORS = ("qkv", "keys", "values", "block_table", "q_start", "q_pos0", "kv_len")
+
+
 def _need_attention(what: str, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads: int, num_kv_heads: int, head_dim: int,
                     page_size: int) -> int:
     """What an attention of a step over the paged cache is given: the number of its requests."""
+    dtype, i32, shape, seqs = qkv.dtype, torch.int32, keys.shape, kv_len.shape[0] if kv_len.dim() == 1 else -1
+    if (dtype in _DTYPE_CODE and keys.dtype is dtype and values.dtype is dtype and block_table.dtype is i32 and q_start.dtype is i32 and q_pos0.dtype is i32
+            and kv_len.dtype is i32 and num_kv_heads > 0 and num_heads >= num_kv_heads and num_heads % num_kv_heads == 0
+            and shape[1:] == (num_kv_heads, page_size, head_dim) and values.shape == shape and qkv.shape[1:] == ((num_heads + 2 * num_kv_heads) * head_dim,)
+            and block_table.dim() == 2 and block_table.shape[0] == seqs and block_table.shape[1] > 0 and q_start.shape == (seqs + 1,) and q_pos0.shape == (seqs,)):
+        return seqs
     _code(qkv)
     seqs = _need_tables(what, block_table, kv_len)
     _int32(what, q_start=q_start, q_pos0=q_pos0)
@@ -2356,6 +2373,17 @@ def _need_attention(what: str, qkv, keys, values, block_table, q_start, q_pos0, 
 PREFIX_ATTENTION_MAX_TOKENS = 63
 
 
+@functools.lru_cache(maxsize=64)
+def _prefix_supports(*sizes) -> bool:
+    return bool(_lib("attention_prefix").pae_attention_prefix_supports(*sizes))
+
+
+@functools.lru_cache(maxsize=1024)
+def _prefix_floats(*sizes) -> int:
+    """Floats of scratch, which follow from a step's sizes alone."""
+    return _lib("attention_prefix").pae_attention_prefix_floats(*sizes)
+
+
 def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_len, prefix_len, group_start, num_heads: int, num_kv_heads: int,
                            head_dim: int, page_size: int, max_q_len: int, max_prefix_len: int, max_own_len: int, max_group_tokens: int, scale: float,
                            num_single=None, info: dict | None = None) -> torch.Tensor:
@@ -2369,44 +2397,60 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     qkv = materialized(qkv)
     what = "paged_attention_prefix"
     seqs = _need_attention(what, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size)
-    _int32(what, prefix_len=prefix_len, group_start=group_start)
-    if prefix_len.shape != (seqs,) or group_start.dim() != 1 or not 2 <= group_start.shape[0] <= seqs + 1:
+    if prefix_len.dtype is not torch.int32 or group_start.dtype is not torch.int32:
+        _int32(what, prefix_len=prefix_len, group_start=group_start)
+    if prefix_len.shape != (seqs,) or group_start.dim() != 1 or not 2 <= group_start.numel() <= seqs + 1:
         raise KernelError(f"{what}: prefix_len {tuple(prefix_len.shape)} and group_start {tuple(group_start.shape)} for {seqs} requests")
-    tokens, groups = qkv.shape[0], group_start.shape[0] - 1
+    tokens, groups = qkv.shape[0], group_start.numel() - 1
     if max_prefix_len < 0 or max_own_len < 0 or max_prefix_len > block_table.shape[1] * page_size:
         raise KernelError(f"{what}: {max_prefix_len} shared and {max_own_len} own keys for tables of {block_table.shape[1]} pages of {page_size}")
     if not 0 <= max_q_len <= max_group_tokens <= tokens:
         raise KernelError(f"{what}: requests of up to {max_q_len} tokens in groups of up to {max_group_tokens}, of {tokens}")
-    _here(what, qkv=qkv, keys=keys, values=values, block_table=block_table, q_start=q_start, q_pos0=q_pos0, kv_len=kv_len, prefix_len=prefix_len,
-          group_start=group_start)
-    lib = _lib("attention_prefix")
-    if not (qkv.dtype == torch.bfloat16 and use_tensor_cores and 0 < max_q_len <= PREFIX_ATTENTION_MAX_TOKENS and max_prefix_len > 0
-            and max_group_tokens > max_q_len and lib.pae_attention_prefix_supports(num_heads, num_kv_heads, head_dim, page_size)
-            and not (qkv.data_ptr() | keys.data_ptr() | values.data_ptr()) & 15):
+    _here(what, (*_STEP_TENSORS, "prefix_len", "group_start"), qkv, keys, values, block_table, q_start, q_pos0, kv_len, prefix_len, group_start)
+    operands = qkv.data_ptr(), keys.data_ptr(), values.data_ptr()
+    if not (qkv.dtype is torch.bfloat16 and use_tensor_cores and 0 < max_q_len <= PREFIX_ATTENTION_MAX_TOKENS and max_prefix_len > 0
+            and max_group_tokens > max_q_len and _prefix_supports(num_heads, num_kv_heads, head_dim, page_size)
+            and not (operands[0] | operands[1] | operands[2]) & 15):
         return paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len,
                                min(max_prefix_len + max_own_len, block_table.shape[1] * page_size), scale, 0, num_single=num_single, info=info)
     if info is not None:
         info.update(kernel="shared")
-    out = torch.empty((tokens, num_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
-    scratch = torch.empty(lib.pae_attention_prefix_floats(tokens, seqs, groups, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_prefix_len,
-                                                          max_own_len, max_group_tokens), dtype=torch.float32, device=qkv.device)
-    _set_bounds("attention_prefix", keys)
+    lib = _lib("attention_prefix")
+    out = qkv.new_empty((tokens, num_heads * head_dim))
+    floats = _prefix_floats(tokens, seqs, groups, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_prefix_len, max_own_len, max_group_tokens)
+    scratch = qkv.new_empty(2 * floats)                   # bfloat16
+    if bounds_checked:
+        _set_bounds("attention_prefix", keys)
     _check(lib, lib.pae_paged_attention_prefix(
-        out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), keys.shape[0], block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
-        q_pos0.data_ptr(), kv_len.data_ptr(), prefix_len.data_ptr(), group_start.data_ptr(), tokens, seqs, groups, num_heads, num_kv_heads, head_dim,
-        page_size, max_q_len, max_prefix_len, max_own_len, max_group_tokens, scale, scratch.data_ptr(), _error_flag(qkv.device).data_ptr(), _stream()), 2)
+        out.data_ptr(), *operands, keys.shape[0], block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(),
+        prefix_len.data_ptr(), group_start.data_ptr(), tokens, seqs, groups, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_prefix_len,
+        max_own_len, max_group_tokens, scale, scratch.data_ptr(), _error_flag(qkv.device).data_ptr(), _stream()), 2)
     return out
+
+
+@functools.lru_cache(maxsize=64)
+def _mass_supports(*sizes) -> bool:
+    return bool(_lib("attention_mma").pae_attention_mma_supports(*sizes))
+
+
+@functools.lru_cache(maxsize=1024)
+def _mass_slicing(singles: int, seqs: int, num_heads: int, num_kv_heads: int, head_dim: int, max_kv_len: int) -> tuple[int, int, int]:
+    """(keys per slice, slices, floats of scratch) of a step of single tokens."""
+    plain = _lib("attention_mma")
+    slice_keys, max_slices = decode_slicing(singles, num_kv_heads, max_kv_len, wave_blocks=plain.pae_decode_blocks_per_wave(head_dim),
+                                            slices_per_block=plain.pae_decode_slices_per_block())
+    return slice_keys, max_slices, _lib("attention_mass").pae_decode_mass_floats(seqs, num_heads, head_dim, slice_keys, max_slices)
 
 
 def _decode_mass(out, qkv, keys, values, mass, block_table, q_start, kv_len, slots, sizes, max_kv_len: int, scale: float, keep_first: int, singles: int) -> None:
     """The requests of a step that bring one token: their rows of `out`, and their keys' weights."""
     num_heads, num_kv_heads, head_dim, page_size = sizes
     seqs = kv_len.shape[0]
-    plain, lib = _lib("attention_mma"), _lib("attention_mass")
-    slice_keys, max_slices = decode_slicing(singles, num_kv_heads, max_kv_len, wave_blocks=plain.pae_decode_blocks_per_wave(head_dim),
-                                            slices_per_block=plain.pae_decode_slices_per_block())
-    scratch = torch.empty(lib.pae_decode_mass_floats(seqs, num_heads, head_dim, slice_keys, max_slices), dtype=torch.float32, device=qkv.device)
-    _set_bounds("attention_mass", keys)
+    lib = _lib("attention_mass")
+    slice_keys, max_slices, floats = _mass_slicing(singles, seqs, num_heads, num_kv_heads, head_dim, max_kv_len)
+    scratch = qkv.new_empty(2 * floats)                   # bfloat16
+    if bounds_checked:
+        _set_bounds("attention_mass", keys)
     _check(lib, lib.pae_paged_attention_decode_mass(
         out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), mass.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
         kv_len.data_ptr(), _ptr(slots), seqs, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices, scratch.data_ptr(),
@@ -2457,20 +2501,19 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
         raise KernelError(f"paged_attention_mass: {keep_first} first keys")
     if not 0 <= max_kv_len <= block_table.shape[1] * page_size:
         raise KernelError(f"paged_attention_mass: {max_kv_len} keys for tables of {block_table.shape[1]} pages of {page_size}")
-    given = dict(qkv=qkv, keys=keys, values=values, mass=mass, block_table=block_table, q_start=q_start, q_pos0=q_pos0, kv_len=kv_len)
     if slots is not None:
         _int32("paged_attention_mass", slots=slots)
         if slots.shape != (tokens,):
             raise KernelError(f"paged_attention_mass: slots {tuple(slots.shape)} for {tokens} tokens")
-        given["slots"] = slots
-    _here("paged_attention_mass", **given)
+    _here("paged_attention_mass", (*_STEP_TENSORS, "mass", "slots"), qkv, keys, values, block_table, q_start, q_pos0, kv_len, mass,
+          *(() if slots is None else (slots,)))
     singles = num_single if num_single is not None else (seqs if max_q_len == 1 else -1)
     sizes = (num_heads, num_kv_heads, head_dim, page_size)
-    if max_kv_len > 0 and max_q_len > 0 and plain_attention_takes(*sizes, qkv.dtype):
+    if max_kv_len > 0 and max_q_len > 0 and qkv.dtype is torch.bfloat16 and use_tensor_cores and _mass_supports(*sizes):
         prompt = _lib("attention_mass_prompt") if max_q_len > 1 else None
         if prompt is None or (use_tcgen05_attention and prompt.pae_attention_mass_prompt_supports(*sizes)
                               and not (qkv.data_ptr() | keys.data_ptr() | values.data_ptr()) & 15):
-            out = torch.empty((tokens, num_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+            out = qkv.new_empty((tokens, num_heads * head_dim))
             if prompt is not None:
                 _prompt_mass(prompt, out, qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, slots, sizes, max_q_len, max_kv_len, scale, keep_first,
                              singles, multi_index)
@@ -2503,12 +2546,14 @@ def choose_kept(mass, block_table, kv_len, budget: int, keep_first: int, keep_la
         raise KernelError(f"choose_kept: {keep_first} first and {keep_last} last keys of a budget of {budget}")
     if not 0 <= max_kv_len <= block_table.shape[1] * mass.shape[2]:
         raise KernelError(f"choose_kept: {max_kv_len} keys for tables of {block_table.shape[1]} pages of {mass.shape[2]}")
-    _here("choose_kept", mass=mass, block_table=block_table, kv_len=kv_len)
-    kept = torch.empty((seqs, mass.shape[1], budget), dtype=torch.int32, device=mass.device)
+    _here("choose_kept", ("mass", "block_table", "kv_len"), mass, block_table, kv_len)
+    _, kv_heads, page_size = mass.shape
+    kept = kv_len.new_empty((seqs, kv_heads, budget))
     lib = _lib("evict")
-    _set_bounds("evict", mass)
-    _check(lib, lib.pae_choose_kept(kept.data_ptr(), mass.data_ptr(), block_table.data_ptr(), block_table.shape[1], kv_len.data_ptr(), seqs, mass.shape[1],
-                                    mass.shape[2], budget, keep_first, keep_last, max_kv_len, _stream()))
+    if bounds_checked:
+        _set_bounds("evict", mass)
+    _check(lib, lib.pae_choose_kept(kept.data_ptr(), mass.data_ptr(), block_table.data_ptr(), block_table.shape[1], kv_len.data_ptr(), seqs, kv_heads,
+                                    page_size, budget, keep_first, keep_last, max_kv_len, _stream()))
     return kept
 
 
@@ -2526,23 +2571,26 @@ def compact_kept(keys, values, mass, block_table, kv_len, kept) -> None:
     pages, kv_heads, page_size, key_dim = keys.shape
     if kept.dim() != 3 or kept.shape[0] != seqs or kept.shape[1] != kv_heads:
         raise KernelError(f"compact_kept: kept {tuple(kept.shape)} for {seqs} requests of {kv_heads} kv heads")
-    given = dict(keys=keys, block_table=block_table, kv_len=kv_len, kept=kept)
+    names, given = ["keys", "block_table", "kv_len", "kept"], [keys, block_table, kv_len, kept]
     if values is not None and values.data_ptr() == keys.data_ptr() and values.shape == keys.shape:
         values = None
     if values is not None:
         if values.dtype != keys.dtype or values.dim() != 4 or values.shape[:3] != keys.shape[:3]:
             raise KernelError(f"compact_kept: values {values.dtype} {tuple(values.shape)} beside keys {keys.dtype} {tuple(keys.shape)}")
-        given["values"] = values
+        names.append("values")
+        given.append(values)
     if mass is not None:
         if mass.dtype != torch.float32 or mass.shape != keys.shape[:3]:
             raise KernelError(f"compact_kept: mass {mass.dtype} {tuple(mass.shape)} beside keys {tuple(keys.shape)}")
-        given["mass"] = mass
-    _here("compact_kept", **given)
+        names.append("mass")
+        given.append(mass)
+    _here("compact_kept", names, *given)
     size = keys.element_size()
     key_bytes, value_bytes = key_dim * size, 0 if values is None else values.shape[3] * size
     together = key_bytes | value_bytes | keys.data_ptr() | (0 if values is None else values.data_ptr())
     unit = 16 if together % 16 == 0 else 4 if together % 4 == 0 else 2
     lib = _lib("evict")
-    _set_bounds("evict", keys)
+    if bounds_checked:
+        _set_bounds("evict", keys)
     _check(lib, lib.pae_compact_kept(keys.data_ptr(), _ptr(values), _ptr(mass), block_table.data_ptr(), block_table.shape[1], kv_len.data_ptr(),
                                      kept.data_ptr(), seqs, kv_heads, page_size, kept.shape[2], key_bytes, value_bytes, unit, _stream()))
