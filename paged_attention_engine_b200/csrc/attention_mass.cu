@@ -12,8 +12,12 @@
 //                   which leaves the scaled scores beside its partial outputs (4 bytes for each query head and key, where the keys and values
 //                   are 4 * head size bytes for each kv head and key), and one kernel that merges the slices and, in further blocks,
 //                   turns the scores into weights once a row's maximum and sum are known.
+//   slices, merge   the same on CUDA cores for single tokens of any other type and head size that is a multiple of 4 up to 256 (up to 16 query
+//                   heads a kv head): a block takes 64 keys a tile, one thread per key and half of the rows for the scores, one per four channels and a share
+//                   of the keys for the output.
 //   stats, columns  every other step: the rows' maxima and sums over runs of keys, then per tile of keys the
-//                   weights of all rows that see it, from scores that are computed again. CUDA cores, any type and head size.
+//                   weights of all rows that see it, from scores that are computed again. CUDA cores, any type and head size. (Portions in bfloat16 go
+//                   to attention_mass_prompt.cu where that takes their sizes.)
 #include "attention_mma.cuh"
 
 using namespace pae;
@@ -132,8 +136,50 @@ __global__ void __launch_bounds__(SLICE_WARPS * 32) mass_slices_kernel(const Dec
   }
 }
 
+constexpr int MASS_CHUNK = 512;          // keys per block of 128 threads, four a thread
+
+// The weights of keys key0 .. key0 + MASS_CHUNK - 1 of (request b, kv head g), from the scores and the slices' maxima and sums.
+__device__ __forceinline__ void add_chunk(const MassParams& m, const float* __restrict__ part_max, const float* __restrict__ part_sum, const float* __restrict__ scores, int b,
+                                          int g, int key0, int token, int n_kv, int slices, int slice_keys, int max_slices, int span, float* top_of, float* inverse_of) {
+  const int last = min(n_kv, slices * slice_keys);
+  if (key0 >= last || key0 + MASS_CHUNK <= m.keep_first || pads(m, token)) return;
+  const int groups = m.heads / m.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < groups; r += MERGE_WARPS) {
+    const size_t at = ((size_t)b * m.heads + g * groups + r) * max_slices;
+    float top = -FLT_MAX, total = 0.f;
+    for (int s = lane; s < slices; s += 32) top = fmaxf(top, part_max[at + s]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int s = lane; s < slices; s += 32) total += part_sum[at + s] * exp2f(part_max[at + s] - top);
+    total = warp_sum(total);
+    if (lane == 0) {
+      top_of[r] = top;
+      inverse_of[r] = total > 0.f ? 1.f / total : 0.f;
+    }
+  }
+  __syncthreads();
+  const int j0 = key0 + threadIdx.x * 4;
+  if (j0 >= last) return;
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  const float* from = scores + ((size_t)b * m.heads + g * groups) * span + j0;
+  for (int r = 0; r < groups; ++r) {
+    const float4 s = *(const float4*)(from + (size_t)r * span);
+    const float top = top_of[r], inverse = inverse_of[r];
+    w[0] += exp2f(s.x - top) * inverse;
+    w[1] += exp2f(s.y - top) * inverse;
+    w[2] += exp2f(s.z - top) * inverse;
+    w[3] += exp2f(s.w - top) * inverse;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = j0 + i;
+    if (j < m.keep_first || j >= last) continue;
+    float* to = mass_of(m, b, g, j);
+    *to = (j == n_kv - 1 ? 0.f : *to) + w[i];
+  }
+}
+
 // Blocks 0 .. heads - 1 of a request merge the slices of a head; the others add the weights of a chunk of one kv head's keys.
-constexpr int MASS_CHUNK = 512;          // keys per block, four a thread
 
 template <int D, int DEPTH>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) mass_merge_kernel(__nv_bfloat16* __restrict__ out, const DecodeParams p, const MassParams m,
@@ -153,42 +199,201 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) mass_merge_kernel(__nv_bfloa
     merge_parts<D, DEPTH>(out + ((size_t)token * p.heads + h) * D, p.part_out + at * D, p.part_max + at, p.part_sum + at, slices, p.max_slices, weights);
     return;
   }
-  const int g = ((int)blockIdx.x - p.heads) / chunks, key0 = (((int)blockIdx.x - p.heads) % chunks) * MASS_CHUNK;
-  const int last = min(n_kv, slices * p.slice_keys);
-  if (key0 >= last || key0 + MASS_CHUNK <= m.keep_first || pads(m, token)) return;
-  const int groups = p.heads / p.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int r = warp; r < groups; r += MERGE_WARPS) {
-    const size_t at = ((size_t)b * p.heads + g * groups + r) * p.max_slices;
-    float top = -FLT_MAX, total = 0.f;
-    for (int s = lane; s < slices; s += 32) top = fmaxf(top, p.part_max[at + s]);
+  add_chunk(m, p.part_max, p.part_sum, scores, b, ((int)blockIdx.x - p.heads) / chunks, (((int)blockIdx.x - p.heads) % chunks) * MASS_CHUNK, token, n_kv, slices,
+            p.slice_keys, p.max_slices, span, top_of, inverse_of);
+}
+
+// ---------------------------------------------------------------------------------------
+// single tokens, any type
+// ---------------------------------------------------------------------------------------
+constexpr int ANY_KEYS = 64;
+constexpr int ANY_THREADS = 128;
+constexpr int ANY_ROWS = 16;
+
+template <typename T>
+struct AnyParams {
+  MassParams m;
+  const T* qkv;
+  const T* keys;
+  const T* values;
+  T* out;
+  float* scores;                // [requests, heads, span]
+  float* part_out;              // [requests, heads, slices, d]
+  float* part_max;
+  float* part_sum;
+  int d, slice_keys, max_slices, span;
+  float scale_log2;
+};
+
+// Four neighbouring elements as float32 (a row starts on a multiple of four elements).
+__device__ __forceinline__ float4 load4(const float* from) { return *(const float4*)from; }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* from) {
+  const uint2 v = *(const uint2*)from;
+  const float2 a = __bfloat1622float2(*(const __nv_bfloat162*)&v.x), b = __bfloat1622float2(*(const __nv_bfloat162*)&v.y);
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ void fma4(float4& acc, float w, const float4& v) {
+  acc.x = fmaf(w, v.x, acc.x);
+  acc.y = fmaf(w, v.y, acc.y);
+  acc.z = fmaf(w, v.z, acc.z);
+  acc.w = fmaf(w, v.w, acc.w);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ANY_THREADS) any_slices_kernel(const AnyParams<T> p) {
+  extern __shared__ __align__(16) float any_smem[];
+  __shared__ float weight[ANY_KEYS][ANY_ROWS], top_of[ANY_ROWS], sum_of[ANY_ROWS], shrink_of[ANY_ROWS];
+  dependent_launch_prologue();
+  const int slice = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
+  const int token = p.m.q_start[b], n = p.m.kv_len[b], begin = slice * p.slice_keys, end = min(n, begin + p.slice_keys);
+  if (p.m.q_start[b + 1] - token != 1 || begin >= end) return;
+  const int groups = p.m.heads / p.m.kv_heads, units = p.d / 4, stride = p.d + 4, tid = threadIdx.x;
+  float* q = any_smem;                                   // [groups][d]
+  float* k = q + ANY_ROWS * p.d;                         // [ANY_KEYS][stride]: a quarter-warp's 16-byte reads of eight rows fall into different banks
+  float* v = k + ANY_KEYS * stride;                      // [ANY_KEYS][d]
+  const T* query = p.qkv + (size_t)token * (p.m.heads + 2 * p.m.kv_heads) * p.d + (size_t)g * groups * p.d;
+  for (int i = tid; i < groups * units; i += ANY_THREADS) *(float4*)(q + i * 4) = load4(query + i * 4);
+  if (tid < ANY_ROWS) {
+    top_of[tid] = -FLT_MAX;
+    sum_of[tid] = 0.f;
+  }
+  const int key = tid % ANY_KEYS, half = tid / ANY_KEYS;
+  const int shares = ANY_THREADS / units, unit = tid % units, share = tid / units;      // threads behind the last share have no part in the output
+  float4 acc[ANY_ROWS];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    for (int s = lane; s < slices; s += 32) total += p.part_sum[at + s] * exp2f(p.part_max[at + s] - top);
-    total = warp_sum(total);
-    if (lane == 0) {
-      top_of[r] = top;
-      inverse_of[r] = total > 0.f ? 1.f / total : 0.f;
+  for (int r = 0; r < ANY_ROWS; ++r) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float* row_scores = p.scores + ((size_t)b * p.m.heads + g * groups) * p.span;
+  for (int key0 = begin; key0 < end; key0 += ANY_KEYS) {
+    const int count = min(ANY_KEYS, end - key0);
+    __syncthreads();                                     // the tile before is read
+    for (int i = tid; i < ANY_KEYS * units; i += ANY_THREADS) {
+      const int row = i / units, c = (i % units) * 4;
+      float4 kv = make_float4(0.f, 0.f, 0.f, 0.f), vv = kv;
+      if (row < count) {
+        const int j = key0 + row, page = checked_page(p.m.block_table[(size_t)b * p.m.table_width + checked_table_index(j / p.m.page_size, p.m.table_width)]);
+        const size_t at = (((size_t)page * p.m.kv_heads + g) * p.m.page_size + j % p.m.page_size) * p.d + c;
+        kv = load4(p.keys + at);
+        vv = load4(p.values + at);
+      }
+      *(float4*)(k + row * stride + c) = kv;
+      *(float4*)(v + row * p.d + c) = vv;
+    }
+    __syncthreads();
+    {
+      float s[ANY_ROWS / 2];                             // of the key with rows half, half + 2, ...
+#pragma unroll
+      for (int i = 0; i < ANY_ROWS / 2; ++i) s[i] = 0.f;
+      for (int c = 0; c < p.d; c += 4) {
+        const float4 kv = *(const float4*)(k + key * stride + c);
+#pragma unroll
+        for (int i = 0; i < ANY_ROWS / 2; ++i)
+          if (half + 2 * i < groups) {
+            const float4 qv = *(const float4*)(q + (half + 2 * i) * p.d + c);
+            s[i] = fmaf(kv.x, qv.x, fmaf(kv.y, qv.y, fmaf(kv.z, qv.z, fmaf(kv.w, qv.w, s[i]))));
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < ANY_ROWS / 2; ++i)
+        if (half + 2 * i < groups) {
+          const float score = key < count ? s[i] * p.scale_log2 : -FLT_MAX;
+          weight[key][half + 2 * i] = score;
+          if (key < count) row_scores[(size_t)(half + 2 * i) * p.span + key0 + key] = score;
+        }
+    }
+    __syncthreads();
+    // A warp per row: the running maximum and sum, and the scores become weights.
+    for (int r = tid >> 5; r < groups; r += ANY_THREADS / 32) {
+      const int lane = tid & 31;
+      const float s0 = weight[lane][r], s1 = weight[lane + 32][r];
+      float top = fmaxf(s0, s1);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float before = top_of[r], higher = fmaxf(before, top);
+      const float e0 = lane < count ? exp2f(s0 - higher) : 0.f, e1 = lane + 32 < count ? exp2f(s1 - higher) : 0.f;
+      weight[lane][r] = e0;
+      weight[lane + 32][r] = e1;
+      const float sum = warp_sum(e0 + e1);
+      __syncwarp();
+      if (lane == 0) {
+        const float shrink = before == -FLT_MAX ? 0.f : exp2f(before - higher);
+        sum_of[r] = sum_of[r] * shrink + sum;
+        top_of[r] = higher;
+        shrink_of[r] = shrink;
+      }
+    }
+    __syncthreads();
+    if (share < shares) {
+#pragma unroll
+      for (int r = 0; r < ANY_ROWS; ++r)
+        if (r < groups) {
+          const float shrink = shrink_of[r];
+          acc[r].x *= shrink;
+          acc[r].y *= shrink;
+          acc[r].z *= shrink;
+          acc[r].w *= shrink;
+        }
+      for (int j = share; j < count; j += shares) {
+        const float4 vv = *(const float4*)(v + j * p.d + unit * 4);
+#pragma unroll
+        for (int r = 0; r < ANY_ROWS; r += 4)
+          if (r < groups) {
+            const float4 w = *(const float4*)&weight[j][r];
+            fma4(acc[r], w.x, vv);
+            if (r + 1 < groups) fma4(acc[r + 1], w.y, vv);
+            if (r + 2 < groups) fma4(acc[r + 2], w.z, vv);
+            if (r + 3 < groups) fma4(acc[r + 3], w.w, vv);
+          }
+      }
     }
   }
+  // ---- the shares of the keys, added in their order, over the tiles' memory
   __syncthreads();
-  const int j0 = key0 + threadIdx.x * 4;
-  if (j0 >= last) return;
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
-  const float* from = scores + ((size_t)b * p.heads + g * groups) * span + j0;
-  for (int r = 0; r < groups; ++r) {
-    const float4 s = *(const float4*)(from + (size_t)r * span);
-    const float top = top_of[r], inverse = inverse_of[r];
-    w[0] += exp2f(s.x - top) * inverse;
-    w[1] += exp2f(s.y - top) * inverse;
-    w[2] += exp2f(s.z - top) * inverse;
-    w[3] += exp2f(s.w - top) * inverse;
-  }
+  float* sums = k;                                       // [shares][groups][d]
+  if (share < shares) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = j0 + i;
-    if (j < m.keep_first || j >= last) continue;
-    float* to = mass_of(m, b, g, j);
-    *to = (j == n_kv - 1 ? 0.f : *to) + w[i];
+    for (int r = 0; r < ANY_ROWS; ++r)
+      if (r < groups) *(float4*)(sums + ((size_t)share * groups + r) * p.d + unit * 4) = acc[r];
+  }
+  __syncthreads();
+  const size_t first = ((size_t)b * p.m.heads + g * groups) * p.max_slices + slice;
+  for (int i = tid; i < groups * units; i += ANY_THREADS) {
+    const int r = i / units, c = (i % units) * 4;
+    float4 total = *(const float4*)(sums + r * p.d + c);
+    for (int s = 1; s < shares; ++s) fma4(total, 1.f, *(const float4*)(sums + ((size_t)s * groups + r) * p.d + c));
+    *(float4*)(p.part_out + (first + (size_t)r * p.max_slices) * p.d + c) = total;
+  }
+  if (tid < groups) {
+    p.part_max[first + (size_t)tid * p.max_slices] = top_of[tid];
+    p.part_sum[first + (size_t)tid * p.max_slices] = sum_of[tid];
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ANY_THREADS) any_merge_kernel(const AnyParams<T> p, int chunks) {
+  __shared__ float top_of[ANY_ROWS], inverse_of[ANY_ROWS];
+  dependent_launch_prologue();
+  const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const int token = p.m.q_start[b], n = p.m.kv_len[b];
+  if (p.m.q_start[b + 1] - token != 1) return;
+  const int slices = min(p.max_slices, (n + p.slice_keys - 1) / p.slice_keys);
+  if ((int)blockIdx.x >= p.m.heads) {
+    add_chunk(p.m, p.part_max, p.part_sum, p.scores, b, ((int)blockIdx.x - p.m.heads) / chunks, (((int)blockIdx.x - p.m.heads) % chunks) * MASS_CHUNK, token, n, slices,
+              p.slice_keys, p.max_slices, p.span, top_of, inverse_of);
+    return;
+  }
+  const size_t at = ((size_t)b * p.m.heads + blockIdx.x) * p.max_slices;
+  float top = -FLT_MAX, total = 0.f;
+  for (int s = lane; s < slices; s += 32) top = fmaxf(top, p.part_max[at + s]);           // every warp works them out for itself
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int s = lane; s < slices; s += 32) total += p.part_sum[at + s] * exp2f(p.part_max[at + s] - top);
+  total = warp_sum(total);
+  const float inverse = total > 0.f ? 1.f / total : 0.f;
+  for (int c = tid; c < p.d; c += ANY_THREADS) {
+    float sum = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < slices; ++s) sum = fmaf(exp2f(p.part_max[at + s] - top), p.part_out[(at + s) * p.d + c], sum);
+    p.out[((size_t)token * p.m.heads + blockIdx.x) * p.d + c] = from_float<T>(sum * inverse);
   }
 }
 
@@ -379,6 +584,20 @@ int launch_rows(RowParams<T> p, const void* qkv, const void* keys, int seqs, int
   return check_launch("attention_mass");
 }
 
+template <typename T>
+int launch_any(AnyParams<T> p, int seqs, cudaStream_t s) {
+  const int groups = p.m.heads / p.m.kv_heads;
+  size_t tiles = (size_t)ANY_KEYS * (2 * p.d + 4), shares = (size_t)(ANY_THREADS / (p.d / 4)) * groups * p.d;
+  const size_t bytes = ((size_t)ANY_ROWS * p.d + (tiles > shares ? tiles : shares)) * sizeof(float);
+  static DevicesSet devices;
+  if (int err = raise_shared_memory(devices, any_slices_kernel<T>, 160 * 1024, "paged_attention_mass")) return err;
+  launch_kernel(any_slices_kernel<T>, dim3(p.max_slices, p.m.kv_heads, seqs), dim3(ANY_THREADS), bytes, s, p);
+  if (int err = check_launch("paged_attention_mass")) return err;
+  const int chunks = (p.span + MASS_CHUNK - 1) / MASS_CHUNK;
+  launch_kernel(any_merge_kernel<T>, dim3(p.m.heads + p.m.kv_heads * chunks, seqs), dim3(ANY_THREADS), 0, s, p, chunks);
+  return check_launch("paged_attention_mass");
+}
+
 int runs_of(int tokens_rows_tiles, int kv_heads, int seqs, int max_kv_len) {
   const long long blocks = (long long)tokens_rows_tiles * kv_heads * seqs;
   int runs = 1;
@@ -431,6 +650,33 @@ PAE_EXPORT int pae_paged_attention_decode_mass(void* out, const void* qkv, const
   if (d == 32) return launch_decode_mass<32>(p, m, (__nv_bfloat16*)out, scores, span, seqs, s);
   if (d == 64) return launch_decode_mass<64>(p, m, (__nv_bfloat16*)out, scores, span, seqs, s);
   return launch_decode_mass<128>(p, m, (__nv_bfloat16*)out, scores, span, seqs, s);
+}
+
+// Steps of single tokens on CUDA cores (dtype 0 float32, 1 bfloat16): out and weights; requests of several tokens are skipped. `slice_keys` is a
+// multiple of 64; scratch as pae_decode_mass_floats.
+PAE_EXPORT int pae_paged_attention_any_mass(void* out, const void* qkv, const void* keys, const void* values, float* mass, const int* block_table, int table_width,
+                                            const int* q_start, const int* kv_len, const int* slots, int seqs, int heads, int kv_heads, int d, int page_size,
+                                            float scale, int keep_first, int slice_keys, int max_slices, int dtype, float* scratch, void* stream) {
+  if (seqs == 0) return 0;
+  if (d < 4 || d > 256 || d % 4) return fail(2, "paged_attention_mass: head_dim %d is not a multiple of 4 up to 256", d);
+  if (kv_heads < 1 || heads % kv_heads || heads / kv_heads > ANY_ROWS) return fail(2, "paged_attention_mass: %d heads over %d kv heads", heads, kv_heads);
+  if (slice_keys < ANY_KEYS || slice_keys % ANY_KEYS || max_slices < 1) return fail(2, "paged_attention_mass: slices of %d keys x %d", slice_keys, max_slices);
+  if (kv_heads > 65535 || seqs > 65535) return fail(1, "paged_attention_mass: %d requests of %d kv heads, at most 65535 of each", seqs, kv_heads);
+  const int align = dtype == kF32 ? 15 : 7;
+  if ((((uintptr_t)qkv | (uintptr_t)keys | (uintptr_t)values) & align) || ((uintptr_t)scratch & 15))
+    return fail(2, "paged_attention_mass: an operand does not start on a boundary of four elements");
+  const MassParams m = {mass, block_table, q_start, kv_len, slots, table_width, heads, kv_heads, page_size, keep_first};
+  const int span = slice_keys * max_slices;
+  const size_t rows = (size_t)seqs * heads * max_slices;
+  float* scores = scratch;
+  float* part_out = scratch + (size_t)seqs * heads * span;
+  const float scale_log2 = scale * LOG2E;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (dtype == kF32)
+    return launch_any<float>({m, (const float*)qkv, (const float*)keys, (const float*)values, (float*)out, scores, part_out, part_out + rows * d,
+                              part_out + rows * (d + 1), d, slice_keys, max_slices, span, scale_log2}, seqs, s);
+  return launch_any<__nv_bfloat16>({m, (const __nv_bfloat16*)qkv, (const __nv_bfloat16*)keys, (const __nv_bfloat16*)values, (__nv_bfloat16*)out, scores, part_out,
+                                    part_out + rows * d, part_out + rows * (d + 1), d, slice_keys, max_slices, span, scale_log2}, seqs, s);
 }
 
 // Floats of scratch for pae_attention_mass_rows.

@@ -9,8 +9,8 @@
 //
 //   warp 0      TMA: the keys once, by their pages; per tile one box of heads x tokens x 64 channels for each half of the head dimension
 //   warp 1      MMA: scores [128 keys x 128 rows] = K . Q^T into one of two buffers in tensor memory
-//   warps 2-5   one thread per key: reads its 128 scores, takes 128 exponentials and adds them to one sum. No shuffles, no second product.
-//   warp 6      the rows' l_r, negated, into shared memory beside the scores' buffers; -infinity where a tile's rows end
+//   warps 2-9   two threads per key, each for half of a tile's rows: 64 scores, 64 exponentials, one sum. No shuffles, no second product.
+//   warp 10     the rows' l_r, negated, into shared memory beside the scores' buffers; -infinity where a tile's rows end
 //
 // What bounds it are the exponentials: 16 a clock and SM, 128 x 128 of them a tile in 1,024 clocks, where the MMA takes 256 to 512; two blocks share an SM. The
 // rows are cut into chunks so that many blocks of nearly one length are there (a causal mask makes late key tiles short); their sums
@@ -27,8 +27,8 @@ namespace {
 constexpr int KEYS = 128;               // per block: the MMA's rows
 constexpr int TILE = 128;               // query rows per tile: its columns
 constexpr int STAGES = 2;
-constexpr int THREADS = 224;
-constexpr int SUM_WARPS = 4;
+constexpr int THREADS = 352;
+constexpr int SUM_WARPS = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Params {
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(THREADS, 2) column_sums_kernel(const __grid_co
       }
       __syncwarp();
     }
-  } else if (warp == 6) {
+  } else if (warp == 2 + SUM_WARPS) {
     // ------------------------------------------------------------------ the rows' logarithms
     for (int t = 0; t < n_tiles; ++t) {
       const int token0 = (tiles.first + t) * p.tile_tokens, rows = min(p.tile_tokens, tiles.tokens - token0) * groups;
@@ -206,8 +206,8 @@ __global__ void __launch_bounds__(THREADS, 2) column_sums_kernel(const __grid_co
       mbar_arrive(bar(L_FULL, t & 1));
     }
   } else {
-    // ------------------------------------------------------------------ one thread per key
-    const int quadrant = warp & 3, r = quadrant * 32 + lane;
+    // ------------------------------------------------------------------ two threads per key
+    const int quadrant = warp & 3, r = quadrant * 32 + lane, side = (warp - 2) >> 2;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quadrant * 32) << 16);
     const int j = key0 + r;
     uint64_t sum01 = 0, sum23 = 0;
@@ -222,27 +222,37 @@ __global__ void __launch_bounds__(THREADS, 2) column_sums_kernel(const __grid_co
       tcgen05_fence_after();
       // The tile's first `until` rows are the request's; of them the key is seen from row `from` on.
       const int until = min(p.tile_tokens, tiles.tokens - token0) * groups, from = max(0, j - tiles.pos0 - token0) * groups;
-      const bool all = until == TILE && key0 + KEYS - 1 <= tiles.pos0 + token0;
+      // (Rows that no box fills score 0 against an l_r of infinity: their weight is 0 without a mask.)
+      const bool all = until == tile_rows && key0 + KEYS - 1 <= tiles.pos0 + token0;
       const ulonglong2* negated = (const ulonglong2*)(generic_base + L::LSE_OFFSET + (t & 1) * TILE * 4);
+      const int column = side * (TILE / 2);
+      const uint32_t scores = lane_base + (t & 1) * TILE + column;
+      auto add = [&](const float (&s)[32], int c, auto counts) {
 #pragma unroll
-      for (int c = 0; c < TILE; c += 32) {
-        float s[32];
-        tmem_load32(lane_base + (t & 1) * TILE + c, s);
-        auto add = [&](auto counts) {
+        for (int i = 0; i < 32; i += 4) {
+          const ulonglong2 l = negated[(column + c + i) / 4];
+          float e[4];
+          unpack2(fma2(pack2(s[i], s[i + 1]), factor2, l.x), e[0], e[1]);
+          unpack2(fma2(pack2(s[i + 2], s[i + 3]), factor2, l.y), e[2], e[3]);
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const ulonglong2 l = negated[(c + i) / 4];
-            float e[4];
-            unpack2(fma2(pack2(s[i], s[i + 1]), factor2, l.x), e[0], e[1]);
-            unpack2(fma2(pack2(s[i + 2], s[i + 3]), factor2, l.y), e[2], e[3]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) e[k] = counts(c + i + k) ? fast_exp2(e[k]) : 0.f;
-            sum01 = add2(sum01, pack2(e[0], e[1]));
-            sum23 = add2(sum23, pack2(e[2], e[3]));
-          }
-        };
-        if (all) add([](int) { return true; });
-        else add([&](int row) { return row >= from && row < until; });
+          for (int k = 0; k < 4; ++k) e[k] = counts(column + c + i + k) ? fast_exp2(e[k]) : 0.f;
+          sum01 = add2(sum01, pack2(e[0], e[1]));
+          sum23 = add2(sum23, pack2(e[2], e[3]));
+        }
+      };
+      float s[32], behind[32];
+      tmem_ask32(scores, s);
+      tmem_arrived(s);
+      tmem_ask32(scores + 32, behind);
+      if (all) {
+        add(s, 0, [](int) { return true; });
+        tmem_arrived(behind);
+        add(behind, 32, [](int) { return true; });
+      } else {
+        auto seen = [&](int row) { return row >= from && row < until; };
+        add(s, 0, seen);
+        tmem_arrived(behind);
+        add(behind, 32, seen);
       }
       tcgen05_fence_before();
       __syncwarp();
@@ -251,12 +261,14 @@ __global__ void __launch_bounds__(THREADS, 2) column_sums_kernel(const __grid_co
         mbar_arrive(bar(L_EMPTY, t & 1));
       }
     }
-    if (ok && j < p.span) {
-      float e[4];
-      unpack2(sum01, e[0], e[1]);
-      unpack2(sum23, e[2], e[3]);
-      p.part[(((size_t)chunk * p.seqs + b) * p.kv_heads + g) * p.span + j] = (e[0] + e[1]) + (e[2] + e[3]);
-    }
+    float e[4];
+    unpack2(sum01, e[0], e[1]);
+    unpack2(sum23, e[2], e[3]);
+    const float sum = (e[0] + e[1]) + (e[2] + e[3]);
+    float* halves = (float*)(generic_base + L::K_OFFSET);       // the second halves' sums, where the keys lay: every product has read them
+    if (side == 1) halves[r] = sum;
+    asm volatile("bar.sync 1, 256;" ::: "memory");              // the sum warps
+    if (ok && side == 0 && j < p.span) p.part[(((size_t)chunk * p.seqs + b) * p.kv_heads + g) * p.span + j] = sum + halves[r];
   }
 
   tcgen05_fence_before();

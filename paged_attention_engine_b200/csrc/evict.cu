@@ -349,7 +349,8 @@ PAE_EXPORT int pae_choose_kept(int* kept, const float* mass, const int* block_ta
   const size_t smem = (size_t)p.staged * 4;
   static DevicesSet devices;
   if (int code = raise_shared_memory(devices, choose_kernel, MOST_STAGED * 4, "choose_kept")) return code;
-  launch_kernel_cluster(choose_kernel, dim3(ranks, kv_heads, seqs), dim3(CHOOSE_THREADS), smem, (cudaStream_t)stream, ranks, p);
+  if (ranks == 1) launch_kernel(choose_kernel, dim3(1, kv_heads, seqs), dim3(CHOOSE_THREADS), smem, (cudaStream_t)stream, p);
+  else launch_kernel_cluster(choose_kernel, dim3(ranks, kv_heads, seqs), dim3(CHOOSE_THREADS), smem, (cudaStream_t)stream, ranks, p);
   return check_launch("choose_kept");
 }
 

@@ -2442,6 +2442,16 @@ def _mass_slicing(singles: int, seqs: int, num_heads: int, num_kv_heads: int, he
     return slice_keys, max_slices, _lib("attention_mass").pae_decode_mass_floats(seqs, num_heads, head_dim, slice_keys, max_slices)
 
 
+@functools.lru_cache(maxsize=1024)
+def _any_slicing(seqs: int, num_heads: int, num_kv_heads: int, head_dim: int, max_kv_len: int) -> tuple[int, int, int]:
+    """The same on CUDA cores: slices of 64 keys while all blocks run at once, of more where they are more (up to 96 a row)."""
+    tiles = -(-max_kv_len // 64)
+    most = max(1, min(96, tiles, 1184 // (seqs * num_kv_heads)))
+    slice_keys = 64 * -(-tiles // most)
+    max_slices = -(-max_kv_len // slice_keys)
+    return slice_keys, max_slices, _lib("attention_mass").pae_decode_mass_floats(seqs, num_heads, head_dim, slice_keys, max_slices)
+
+
 def _decode_mass(out, qkv, keys, values, mass, block_table, q_start, kv_len, slots, sizes, max_kv_len: int, scale: float, keep_first: int, singles: int) -> None:
     """The requests of a step that bring one token: their rows of `out`, and their keys' weights."""
     num_heads, num_kv_heads, head_dim, page_size = sizes
@@ -2520,6 +2530,19 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
             if singles != 0:
                 _decode_mass(out, qkv, keys, values, mass, block_table, q_start, kv_len, slots, sizes, max_kv_len, scale, keep_first, seqs if singles < 0 else singles)
             return out
+    if max_q_len == 1 and max_kv_len > 0 and head_dim % 4 == 0 and head_dim <= 256 and num_heads // num_kv_heads <= 16 and not (
+            qkv.data_ptr() | keys.data_ptr() | values.data_ptr()) & (4 * qkv.element_size() - 1):
+        slice_keys, max_slices, floats = _any_slicing(seqs, num_heads, num_kv_heads, head_dim, max_kv_len)
+        out = qkv.new_empty((tokens, num_heads * head_dim))
+        scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device)
+        lib = _lib("attention_mass")
+        if bounds_checked:
+            _set_bounds("attention_mass", keys)
+        _check(lib, lib.pae_paged_attention_any_mass(
+            out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), mass.data_ptr(), block_table.data_ptr(), block_table.shape[1],
+            q_start.data_ptr(), kv_len.data_ptr(), _ptr(slots), seqs, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices,
+            _code(qkv), scratch.data_ptr(), _stream()), 2)
+        return out
     out = paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_kv_len, scale,
                           0, num_single=num_single, multi_index=multi_index)
     lib = _lib("attention_mass")
