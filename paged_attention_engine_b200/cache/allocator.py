@@ -8,9 +8,10 @@ or nothing and reports exhaustion as a value, not an exception
 (engine/cache.py:132-155,238-257); an unknown id, a second create and a second free are
 caller faults and raise (engine/cache.py:221-264).
 
-One thing is added for layers that see a window of keys only: `release_before` gives
+Two things are added. For layers that see a window of keys only, `release_before` gives
 back the blocks that lie wholly before a position, leaving holes (-1) at the front of
-the table.
+the table. For caches whose keys are evicted, `shorten_sequence` gives back the blocks
+behind the tokens that stay.
 """
 
 from __future__ import annotations
@@ -183,6 +184,20 @@ class BlockAllocator:
             t.released = upto
         self._free.extend(freed)
         return tuple(freed)
+
+    def shorten_sequence(self, seq_id, num_tokens: int) -> tuple[int, ...]:
+        """Leaves the sequence its first `num_tokens` tokens and gives back the blocks behind them: what remains
+        of a request whose keys were evicted and whose kept ones moved to the front of its blocks."""
+        t = self._tables[seq_id]
+        if not 0 <= num_tokens <= t.tokens:
+            raise ValueError(f"sequence {seq_id!r} has {t.tokens} tokens, it cannot be shortened to {num_tokens}")
+        left = self.blocks_needed(num_tokens)
+        freed = tuple(b for b in t.blocks[left:] if b != HOLE)
+        del t.blocks[left:]
+        t.tokens = num_tokens
+        t.released = min(t.released, left)
+        self._free.extend(freed)
+        return freed
 
     def free_sequence(self, seq_id) -> tuple[int, ...]:
         """Drops the table and gives back every block it still held, in table order."""

@@ -2391,7 +2391,7 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     Requests group_start[i] .. group_start[i + 1] - 1 (int32 [groups + 1], from 0 to the number of requests) are a group: their first
     prefix_len[b] keys (int32 [requests], the same for all of a group; 0: nothing is shared) are the same, and every token of the step stands behind
     them. They are read through the block table of the group's first request. The result is that of `paged_attention` but for the order of the sums.
-    The longest request brings `max_q_len` tokens, the largest group `max_group_tokens`; `max_prefix_len` and `max_own_len` bound the shared keys and the
+    The longest request brings at most `max_q_len` tokens, the largest group `max_group_tokens`; `max_prefix_len` and `max_own_len` bound the shared keys and the
     keys behind them. `info`, when given, receives which kernel ran ("kernel": "shared", or what `paged_attention` says where each request reads its
     keys by itself: other types, head sizes and page sizes than the tensor-core kernel's, long portions, groups of one request)."""
     qkv = materialized(qkv)
@@ -2404,8 +2404,9 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     tokens, groups = qkv.shape[0], group_start.numel() - 1
     if max_prefix_len < 0 or max_own_len < 0 or max_prefix_len > block_table.shape[1] * page_size:
         raise KernelError(f"{what}: {max_prefix_len} shared and {max_own_len} own keys for tables of {block_table.shape[1]} pages of {page_size}")
-    if not 0 <= max_q_len <= max_group_tokens <= tokens:
-        raise KernelError(f"{what}: requests of up to {max_q_len} tokens in groups of up to {max_group_tokens}, of {tokens}")
+    if not 0 <= max_q_len <= max_group_tokens:
+        raise KernelError(f"{what}: requests of up to {max_q_len} tokens in groups of up to {max_group_tokens}")
+    max_q_len, max_group_tokens = min(max_q_len, tokens), min(max_group_tokens, tokens)
     _here(what, (*_STEP_TENSORS, "prefix_len", "group_start"), qkv, keys, values, block_table, q_start, q_pos0, kv_len, prefix_len, group_start)
     operands = qkv.data_ptr(), keys.data_ptr(), values.data_ptr()
     if not (qkv.dtype is torch.bfloat16 and use_tensor_cores and 0 < max_q_len <= PREFIX_ATTENTION_MAX_TOKENS and max_prefix_len > 0
@@ -2518,6 +2519,8 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
     _here("paged_attention_mass", (*_STEP_TENSORS, "mass", "slots"), qkv, keys, values, block_table, q_start, q_pos0, kv_len, mass,
           *(() if slots is None else (slots,)))
     singles = num_single if num_single is not None else (seqs if max_q_len == 1 else -1)
+    if singles < 0 and tokens > (seqs - 1) * max_q_len + 1:
+        singles = 0                                       # a request of one token would leave more to the others than they can bring
     sizes = (num_heads, num_kv_heads, head_dim, page_size)
     if max_kv_len > 0 and max_q_len > 0 and qkv.dtype is torch.bfloat16 and use_tensor_cores and _mass_supports(*sizes):
         prompt = _lib("attention_mass_prompt") if max_q_len > 1 else None
@@ -2585,13 +2588,15 @@ def compact_kept(keys, values, mass, block_table, kv_len, kept) -> None:
     request and kv head gets the row of key kept[.., i], of `keys` and `values` [pages, kv_heads, page_size, head size] and of
     `mass` [pages, kv_heads, page_size] alike. values and mass may be None; values may have another head size, and may be the keys
     themselves (a latent's pages). A request then has min(kv_len, budget) keys; what lies behind them is left as it was. Rows that
-    stay where they are, such as a shared prefix of at most `keep_first` keys, are not written. The indices ascend in every
-    row, as `choose_kept` leaves them; one that is negative, not below kv_len, or below its place moves nothing."""
+    stay where they are, such as a shared prefix of at most `keep_first` keys, are not written. A page with rows that move belongs
+    to one request. The indices ascend in every row, as `choose_kept` leaves them; one that is negative, not below kv_len, or below its place moves nothing."""
     seqs = _need_tables("compact_kept", block_table, kv_len)
     _int32("compact_kept", kept=kept)
     if keys.dim() != 4:
         raise KernelError(f"compact_kept: keys {tuple(keys.shape)}, [pages, kv_heads, page_size, head size] is needed")
     pages, kv_heads, page_size, key_dim = keys.shape
+    if pages * kv_heads * page_size >= 0xFFFFFFFF:
+        raise KernelError(f"compact_kept: a pool of {pages * kv_heads * page_size} rows, fewer than 2^32 - 1 are taken")
     if kept.dim() != 3 or kept.shape[0] != seqs or kept.shape[1] != kv_heads:
         raise KernelError(f"compact_kept: kept {tuple(kept.shape)} for {seqs} requests of {kv_heads} kv heads")
     names, given = ["keys", "block_table", "kv_len", "kept"], [keys, block_table, kv_len, kept]

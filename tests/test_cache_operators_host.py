@@ -74,7 +74,7 @@ def test_mass_refuses(arguments, message):
 @pytest.mark.parametrize("arguments,message", STEP_REFUSALS + [
     (dict(prefix_len=_i32(2)), "prefix_len \\(2,\\)"), (dict(prefix_len=_i32(3).long()), "prefix_len is torch.int64"), (dict(group_start=_i32(1)), "group_start \\(1,\\)"),
     (dict(group_start=_i32(5)), "group_start \\(5,\\)"), (dict(group_start=torch.zeros(3)), "group_start is torch.float32"), (dict(max_prefix_len=-1), "-1 shared"),
-    (dict(max_own_len=-1), "-1 own keys"), (dict(max_prefix_len=65), "65 shared"), (dict(max_group_tokens=6), "groups of up to 6, of 5"), (dict(max_q_len=4), "up to 4 tokens in groups of up to 3")])
+    (dict(max_own_len=-1), "-1 own keys"), (dict(max_prefix_len=65), "65 shared"), (dict(max_q_len=4), "up to 4 tokens in groups of up to 3")])
 def test_prefix_refuses(arguments, message):
     a = dict(prefix_len=_i32(3), group_start=_i32(3), num_heads=HEADS, num_kv_heads=KV_HEADS, head_dim=DIM, page_size=PAGE, max_q_len=2, max_prefix_len=20, max_own_len=30,
              max_group_tokens=3, scale=1.0)
@@ -82,3 +82,32 @@ def test_prefix_refuses(arguments, message):
     a.update({k: v for k, v in arguments.items()})
     with pytest.raises(ops.KernelError, match=message):
         ops.paged_attention_prefix(**a)
+
+
+def test_a_shortened_sequence_gives_back_the_blocks_behind_its_tokens():
+    from paged_attention_engine_b200.cache.allocator import HOLE, BlockAllocator
+
+    pool = BlockAllocator(10, 4)
+    for name, count in (("a", 18), ("b", 9)):
+        pool.create_sequence(name)
+        assert pool.append_tokens(name, count).ok
+    table = pool.block_table("a")
+    assert pool.shorten_sequence("a", 9) == table[3:] and pool.block_table("a") == table[:3] and pool.num_tokens("a") == 9
+    assert pool.free_block_ids()[-2:] == table[3:] and pool.num_allocated == 6
+    assert pool.shorten_sequence("a", 9) == () and pool.append_tokens("a", 3).new_block_ids == ()
+    assert pool.append_tokens("a", 1).new_block_ids == (8,)
+    with pytest.raises(ValueError, match="13 tokens, it cannot be shortened to 14"):
+        pool.shorten_sequence("a", 14)
+    with pytest.raises(ValueError, match="-1"):
+        pool.shorten_sequence("a", -1)
+    with pytest.raises(KeyError):
+        pool.shorten_sequence("c", 0)
+    assert pool.shorten_sequence("a", 0) == (*table[:3], 8) and pool.block_table("a") == ()
+    # Behind a window's holes.
+    assert pool.append_tokens("a", 16).ok
+    freed = pool.release_before("a", 9)
+    held = pool.block_table("a")
+    assert len(freed) == 2 and held[:2] == (HOLE, HOLE) and pool.num_held("a") == 2
+    assert pool.shorten_sequence("a", 5) == held[2:] and pool.num_held("a") == 0
+    everything = pool.num_free
+    assert pool.free_sequence("a") == () and pool.num_free == everything and len(set(pool.free_block_ids())) == everything == 7
