@@ -36,9 +36,12 @@ struct MassParams {
 
 __device__ __forceinline__ bool pads(const MassParams& m, int token) { return m.slots != nullptr && m.slots[token] < 0; }
 
-__device__ __forceinline__ float* mass_of(const MassParams& m, int b, int g, int j) {
-  const int page = checked_page(m.block_table[(size_t)b * m.table_width + checked_table_index(j / m.page_size, m.table_width)]);
-  return m.mass + ((size_t)page * m.kv_heads + g) * m.page_size + j % m.page_size;
+// mass = (mass, or 0 for a key that starts from nothing) + w.
+__device__ __forceinline__ void add_mass(const MassParams& m, int b, int g, int j, bool fresh, float w) {
+  const int page = page_or_none(m.block_table + (size_t)b * m.table_width, j / m.page_size, m.table_width);
+  if (page < 0) return;
+  float* to = m.mass + ((size_t)page * m.kv_heads + g) * m.page_size + j % m.page_size;
+  *to = (fresh ? 0.f : *to) + w;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -174,8 +177,7 @@ __device__ __forceinline__ void add_chunk(const MassParams& m, const float* __re
   for (int i = 0; i < 4; ++i) {
     const int j = j0 + i;
     if (j < m.keep_first || j >= last) continue;
-    float* to = mass_of(m, b, g, j);
-    *to = (j == n_kv - 1 ? 0.f : *to) + w[i];
+    add_mass(m, b, g, j, j == n_kv - 1, w[i]);
   }
 }
 
@@ -552,8 +554,7 @@ __global__ void __launch_bounds__(THREADS) column_mass_kernel(const RowParams<T>
     float w = 0.f;
 #pragma unroll
     for (int i = 0; i < THREADS / 32; ++i) w += sums[i][lane];
-    float* to = mass_of(p.m, b, g, j);
-    *to = (j >= pos0 ? 0.f : *to) + w;
+    add_mass(p.m, b, g, j, j >= pos0, w);
   }
 }
 

@@ -293,7 +293,8 @@ __global__ void __launch_bounds__(KEYS) add_chunks_kernel(const Params p, int ch
     tiles = tiles_of(p, b, key0, c);
     if (tiles.first < tiles.last) w += p.part[(((size_t)c * p.seqs + b) * p.kv_heads + g) * p.span + j];
   }
-  const int page = checked_page(p.block_table[(size_t)b * p.table_width + checked_table_index(j / p.page_size, p.table_width)]);
+  const int page = page_or_none(p.block_table + (size_t)b * p.table_width, j / p.page_size, p.table_width);
+  if (page < 0) return;
   float* to = p.mass + ((size_t)page * p.kv_heads + g) * p.page_size + j % p.page_size;
   *to = (j >= tiles.pos0 ? 0.f : *to) + w;
 }

@@ -133,6 +133,21 @@ __device__ __forceinline__ int checked_page(int page) {
   return page;
 }
 
+// The page at `index` of a block table of `width` entries, for an access that is not made at all where either is out of range: -1 then.
+__device__ __forceinline__ int page_or_none(const int* table, int index, int width) {
+#ifdef PAE_BOUNDS
+  if (index < 0 || index >= width) {
+    bounds_violation(102);
+    return -1;
+  }
+  if (g_bounds.pages > 0 && (table[index] < 0 || (long long)table[index] >= g_bounds.pages)) {
+    bounds_violation(103);
+    return -1;
+  }
+#endif
+  return table[index];
+}
+
 // The gate of a gated linear unit, act(g) * u: SiLU, the rectifier, or the tanh form of GELU. The kernels that fold it
 // into a product's epilogue and the ones that run it alone all call this.
 enum GateKind : int { kGateSilu = 0, kGateRelu = 1, kGateGeluTanh = 2 };

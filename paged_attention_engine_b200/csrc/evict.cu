@@ -287,13 +287,15 @@ __device__ __forceinline__ void compact_strip(const CompactParams& p, int pool, 
   const int my_row = threadIdx.x / width, my_unit = strip * p.strip_units[pool] + threadIdx.x % width;
   Unit* base = (Unit*)p.pools[pool] + my_unit;
   auto row_of = [&](int i) {
-    const int page = checked_page(table[checked_table_index(i / p.page_size, p.table_width)]);
-    return ((uint32_t)page * p.kv_heads + g) * p.page_size + i % p.page_size;
+    const int page = page_or_none(table, i / p.page_size, p.table_width);
+    return page < 0 ? STAYS : ((uint32_t)page * p.kv_heads + g) * p.page_size + i % p.page_size;
   };
   auto find = [&](int chunk, uint2* to) {
     for (int r = threadIdx.x; r < chunk_rows; r += THREADS) {
       const int i = chunk + r, from = i < places ? kept[i] : -1;
-      to[r] = from > i && from < n ? make_uint2(row_of(from), row_of(i)) : make_uint2(STAYS, STAYS);
+      uint2 move = from > i && from < n ? make_uint2(row_of(from), row_of(i)) : make_uint2(STAYS, STAYS);
+      if (move.y == STAYS) move.x = STAYS;
+      to[r] = move;
     }
   };
   find(0, moves[0]);
@@ -304,7 +306,7 @@ __device__ __forceinline__ void compact_strip(const CompactParams& p, int pool, 
 #pragma unroll
     for (int u = 0; u < IN_FLIGHT; ++u) {
       const uint2 move = my_row < rows_a_pass ? moves[turn][u * rows_a_pass + my_row] : make_uint2(STAYS, STAYS);
-      to[u] = move.y;
+      to[u] = move.x != STAYS ? move.y : STAYS;
       if (move.x != STAYS) held[u] = base[(size_t)move.x * units];
     }
     if (chunk + chunk_rows < places) find(chunk + chunk_rows, moves[turn ^ 1]);
