@@ -2344,14 +2344,18 @@ _STEP_TENSORS = ("qkv", "keys", "values", "block_table", "q_start", "q_pos0", "k
 
 
 def _need_attention(what: str, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads: int, num_kv_heads: int, head_dim: int,
-                    page_size: int) -> int:
-    """What an attention of a step over the paged cache is given: the number of its requests."""
-    dtype, i32, shape, seqs = qkv.dtype, torch.int32, keys.shape, kv_len.shape[0] if kv_len.dim() == 1 else -1
-    if (dtype in _DTYPE_CODE and keys.dtype is dtype and values.dtype is dtype and block_table.dtype is i32 and q_start.dtype is i32 and q_pos0.dtype is i32
-            and kv_len.dtype is i32 and num_kv_heads > 0 and num_heads >= num_kv_heads and num_heads % num_kv_heads == 0
-            and shape[1:] == (num_kv_heads, page_size, head_dim) and values.shape == shape and qkv.shape[1:] == ((num_heads + 2 * num_kv_heads) * head_dim,)
-            and block_table.dim() == 2 and block_table.shape[0] == seqs and block_table.shape[1] > 0 and q_start.shape == (seqs + 1,) and q_pos0.shape == (seqs,)):
-        return seqs
+                    page_size: int) -> tuple[int, int, int, int]:
+    """What an attention of a step over the paged cache is given: (tokens, requests, pages a block table, pages of the pool)."""
+    dtype, i32 = qkv.dtype, torch.int32
+    try:
+        (tokens, width), (pages, *layout), (seqs, table_width) = qkv.shape, keys.shape, block_table.shape
+        if (dtype in _DTYPE_CODE and keys.dtype is dtype and values.dtype is dtype and block_table.dtype is i32 and q_start.dtype is i32 and q_pos0.dtype is i32
+                and kv_len.dtype is i32 and num_heads >= num_kv_heads > 0 and num_heads % num_kv_heads == 0 and layout == [num_kv_heads, page_size, head_dim]
+                and values.shape == keys.shape and width == (num_heads + 2 * num_kv_heads) * head_dim and table_width > 0
+                and kv_len.numel() == seqs and q_pos0.numel() == seqs and q_start.numel() == seqs + 1):
+            return tokens, seqs, table_width, pages
+    except ValueError:
+        pass                                              # another number of dimensions: said below
     _code(qkv)
     seqs = _need_tables(what, block_table, kv_len)
     _int32(what, q_start=q_start, q_pos0=q_pos0)
@@ -2365,12 +2369,23 @@ def _need_attention(what: str, qkv, keys, values, block_table, q_start, q_pos0, 
             raise KernelError(f"{what}: {name} {t.dtype} {tuple(t.shape)}, {qkv.dtype} [pages, {num_kv_heads}, {page_size}, {head_dim}] is needed")
     if q_start.shape != (seqs + 1,) or q_pos0.shape != (seqs,):
         raise KernelError(f"{what}: q_start {tuple(q_start.shape)} and q_pos0 {tuple(q_pos0.shape)} for {seqs} requests")
-    return seqs
+    raise KernelError(f"{what}: tensors of {qkv.dim()}, {keys.dim()} and {block_table.dim()} dimensions for qkv, keys and the block table")
 
 
 # From how many tokens a request on a step is an ordinary one: a query tile of one request fills the tensor cores then, and its keys are
 # read once for all of its tokens anyway.
 PREFIX_ATTENTION_MAX_TOKENS = 63
+
+
+_PREFIX_TENSORS = (*_STEP_TENSORS, "prefix_len", "group_start")
+
+
+def _aligned_operands(what: str, qkv, keys, values, head_dim: int) -> tuple[int, int, int]:
+    """Where the operands lie: on 16-byte boundaries wherever their rows are whole 16-byte pieces, which the kernels copy."""
+    operands = qkv.data_ptr(), keys.data_ptr(), values.data_ptr()
+    if (operands[0] | operands[1] | operands[2]) & 15 and head_dim * qkv.element_size() % 16 == 0:
+        raise KernelError(f"{what}: an operand does not start on a 16-byte boundary")
+    return operands
 
 
 @functools.lru_cache(maxsize=64)
@@ -2396,24 +2411,27 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     keys by itself: other types, head sizes and page sizes than the tensor-core kernel's, long portions, groups of one request)."""
     qkv = materialized(qkv)
     what = "paged_attention_prefix"
-    seqs = _need_attention(what, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size)
+    tokens, seqs, table_width, pages = _need_attention(what, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim,
+                                                       page_size)
     if prefix_len.dtype is not torch.int32 or group_start.dtype is not torch.int32:
         _int32(what, prefix_len=prefix_len, group_start=group_start)
-    if prefix_len.shape != (seqs,) or group_start.dim() != 1 or not 2 <= group_start.numel() <= seqs + 1:
+    groups = group_start.numel() - 1
+    if prefix_len.numel() != seqs or not 1 <= groups <= seqs:
         raise KernelError(f"{what}: prefix_len {tuple(prefix_len.shape)} and group_start {tuple(group_start.shape)} for {seqs} requests")
-    tokens, groups = qkv.shape[0], group_start.numel() - 1
-    if max_prefix_len < 0 or max_own_len < 0 or max_prefix_len > block_table.shape[1] * page_size:
-        raise KernelError(f"{what}: {max_prefix_len} shared and {max_own_len} own keys for tables of {block_table.shape[1]} pages of {page_size}")
+    if max_prefix_len < 0 or max_own_len < 0 or max_prefix_len > table_width * page_size:
+        raise KernelError(f"{what}: {max_prefix_len} shared and {max_own_len} own keys for tables of {table_width} pages of {page_size}")
     if not 0 <= max_q_len <= max_group_tokens:
         raise KernelError(f"{what}: requests of up to {max_q_len} tokens in groups of up to {max_group_tokens}")
-    max_q_len, max_group_tokens = min(max_q_len, tokens), min(max_group_tokens, tokens)
-    _here(what, (*_STEP_TENSORS, "prefix_len", "group_start"), qkv, keys, values, block_table, q_start, q_pos0, kv_len, prefix_len, group_start)
-    operands = qkv.data_ptr(), keys.data_ptr(), values.data_ptr()
+    if max_group_tokens > tokens:
+        max_q_len, max_group_tokens = min(max_q_len, tokens), tokens
+    _here(what, _PREFIX_TENSORS, qkv, keys, values, block_table, q_start, q_pos0, kv_len, prefix_len, group_start)
+    operands = _aligned_operands(what, qkv, keys, values, head_dim)
+    if tokens == 0:
+        return qkv.new_empty((0, num_heads * head_dim))
     if not (qkv.dtype is torch.bfloat16 and use_tensor_cores and 0 < max_q_len <= PREFIX_ATTENTION_MAX_TOKENS and max_prefix_len > 0
-            and max_group_tokens > max_q_len and _prefix_supports(num_heads, num_kv_heads, head_dim, page_size)
-            and not (operands[0] | operands[1] | operands[2]) & 15):
+            and max_group_tokens > max_q_len and _prefix_supports(num_heads, num_kv_heads, head_dim, page_size)):
         return paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len,
-                               min(max_prefix_len + max_own_len, block_table.shape[1] * page_size), scale, 0, num_single=num_single, info=info)
+                               min(max_prefix_len + max_own_len, table_width * page_size), scale, 0, num_single=num_single, info=info)
     if info is not None:
         info.update(kernel="shared")
     lib = _lib("attention_prefix")
@@ -2423,7 +2441,7 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     if bounds_checked:
         _set_bounds("attention_prefix", keys)
     _check(lib, lib.pae_paged_attention_prefix(
-        out.data_ptr(), *operands, keys.shape[0], block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(),
+        out.data_ptr(), *operands, pages, block_table.data_ptr(), table_width, q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(),
         prefix_len.data_ptr(), group_start.data_ptr(), tokens, seqs, groups, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_prefix_len,
         max_own_len, max_group_tokens, scale, scratch.data_ptr(), _error_flag(qkv.device).data_ptr(), _stream()), 2)
     return out
@@ -2453,19 +2471,21 @@ def _any_slicing(seqs: int, num_heads: int, num_kv_heads: int, head_dim: int, ma
     return slice_keys, max_slices, _lib("attention_mass").pae_decode_mass_floats(seqs, num_heads, head_dim, slice_keys, max_slices)
 
 
-def _decode_mass(out, qkv, keys, values, mass, block_table, q_start, kv_len, slots, sizes, max_kv_len: int, scale: float, keep_first: int, singles: int) -> None:
+_MASS_TENSORS = (*_STEP_TENSORS, "mass", "slots")
+
+
+def _decode_mass(out, qkv, keys, operands, mass, block_table, table_width: int, q_start, kv_len, slots, seqs: int, sizes, max_kv_len: int, scale: float,
+                 keep_first: int, singles: int) -> None:
     """The requests of a step that bring one token: their rows of `out`, and their keys' weights."""
     num_heads, num_kv_heads, head_dim, page_size = sizes
-    seqs = kv_len.shape[0]
     lib = _lib("attention_mass")
     slice_keys, max_slices, floats = _mass_slicing(singles, seqs, num_heads, num_kv_heads, head_dim, max_kv_len)
     scratch = qkv.new_empty(2 * floats)                   # bfloat16
     if bounds_checked:
         _set_bounds("attention_mass", keys)
     _check(lib, lib.pae_paged_attention_decode_mass(
-        out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), mass.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
-        kv_len.data_ptr(), _ptr(slots), seqs, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices, scratch.data_ptr(),
-        _stream()), 2)
+        out.data_ptr(), *operands, mass.data_ptr(), block_table.data_ptr(), table_width, q_start.data_ptr(), kv_len.data_ptr(), _ptr(slots), seqs, num_heads,
+        num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices, scratch.data_ptr(), _stream()), 2)
 
 
 def _prompt_mass(lib, out, qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, slots, sizes, max_q_len: int, max_kv_len: int, scale: float,
@@ -2504,37 +2524,40 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
     the pages that hold such keys only; every other page belongs to one request of the step. `slots` (int32 [tokens], as
     `qkv_projection` takes them): a request whose first slot is negative only pads the step and adds nothing."""
     qkv = materialized(qkv)
-    seqs = _need_attention("paged_attention_mass", qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size)
-    tokens = qkv.shape[0]
-    if mass.dtype != torch.float32 or mass.shape != keys.shape[:3]:
+    what = "paged_attention_mass"
+    tokens, seqs, table_width, pages = _need_attention(what, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim,
+                                                       page_size)
+    if mass.dtype is not torch.float32 or mass.shape != (pages, num_kv_heads, page_size):
         raise KernelError(f"paged_attention_mass: mass {mass.dtype} {tuple(mass.shape)} beside keys {tuple(keys.shape)}")
     if keep_first < 0:
         raise KernelError(f"paged_attention_mass: {keep_first} first keys")
-    if not 0 <= max_kv_len <= block_table.shape[1] * page_size:
-        raise KernelError(f"paged_attention_mass: {max_kv_len} keys for tables of {block_table.shape[1]} pages of {page_size}")
+    if not 0 <= max_kv_len <= table_width * page_size:
+        raise KernelError(f"paged_attention_mass: {max_kv_len} keys for tables of {table_width} pages of {page_size}")
     if slots is not None:
         _int32("paged_attention_mass", slots=slots)
         if slots.shape != (tokens,):
             raise KernelError(f"paged_attention_mass: slots {tuple(slots.shape)} for {tokens} tokens")
-    _here("paged_attention_mass", (*_STEP_TENSORS, "mass", "slots"), qkv, keys, values, block_table, q_start, q_pos0, kv_len, mass,
-          *(() if slots is None else (slots,)))
+    _here(what, _MASS_TENSORS, qkv, keys, values, block_table, q_start, q_pos0, kv_len, mass, *(() if slots is None else (slots,)))
+    operands = _aligned_operands(what, qkv, keys, values, head_dim)
+    if tokens == 0:
+        return qkv.new_empty((0, num_heads * head_dim))
     singles = num_single if num_single is not None else (seqs if max_q_len == 1 else -1)
     if singles < 0 and tokens > (seqs - 1) * max_q_len + 1:
         singles = 0                                       # a request of one token would leave more to the others than they can bring
     sizes = (num_heads, num_kv_heads, head_dim, page_size)
     if max_kv_len > 0 and max_q_len > 0 and qkv.dtype is torch.bfloat16 and use_tensor_cores and _mass_supports(*sizes):
         prompt = _lib("attention_mass_prompt") if max_q_len > 1 else None
-        if prompt is None or (use_tcgen05_attention and prompt.pae_attention_mass_prompt_supports(*sizes)
-                              and not (qkv.data_ptr() | keys.data_ptr() | values.data_ptr()) & 15):
+        if prompt is None or (use_tcgen05_attention and prompt.pae_attention_mass_prompt_supports(*sizes)):
             out = qkv.new_empty((tokens, num_heads * head_dim))
             if prompt is not None:
                 _prompt_mass(prompt, out, qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, slots, sizes, max_q_len, max_kv_len, scale, keep_first,
                              singles, multi_index)
             if singles != 0:
-                _decode_mass(out, qkv, keys, values, mass, block_table, q_start, kv_len, slots, sizes, max_kv_len, scale, keep_first, seqs if singles < 0 else singles)
+                _decode_mass(out, qkv, keys, operands, mass, block_table, table_width, q_start, kv_len, slots, seqs, sizes, max_kv_len, scale, keep_first,
+                             seqs if singles < 0 else singles)
             return out
     if max_q_len == 1 and max_kv_len > 0 and head_dim % 4 == 0 and head_dim <= 256 and num_heads // num_kv_heads <= 16 and not (
-            qkv.data_ptr() | keys.data_ptr() | values.data_ptr()) & (4 * qkv.element_size() - 1):
+            operands[0] | operands[1] | operands[2]) & (4 * qkv.element_size() - 1):
         slice_keys, max_slices, floats = _any_slicing(seqs, num_heads, num_kv_heads, head_dim, max_kv_len)
         out = qkv.new_empty((tokens, num_heads * head_dim))
         scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device)

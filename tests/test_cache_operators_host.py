@@ -57,6 +57,7 @@ STEP_REFUSALS = [
     (dict(keys=torch.zeros(9, KV_HEADS, PAGE, DIM, dtype=torch.bfloat16)), "keys torch.bfloat16"), (dict(values=torch.zeros(9, KV_HEADS, 8, DIM)), "values torch.float32 \\(9, 2, 8, 8\\)"),
     (dict(values=torch.zeros(8, KV_HEADS, PAGE, DIM)), "values"), (dict(q_start=_i32(3)), "q_start \\(3,\\)"), (dict(q_pos0=_i32(4)), "q_pos0 \\(4,\\)"),
     (dict(kv_len=_i32(3).long()), "kv_len is torch.int64"), (dict(q_start=torch.zeros(4)), "q_start is torch.float32"), (dict(block_table=_i32(2, 4)), "block tables"),
+    (dict(qkv=torch.zeros(5, 8, 8)), "qkv \\(5, 8, 8\\)"), (dict(keys=torch.zeros(9, KV_HEADS, PAGE * DIM)), "keys torch.float32 \\(9, 2, 128\\)"),
     (dict(num_heads=3), "3 heads over 2 kv heads"), (dict(num_kv_heads=0), "4 heads over 0 kv heads"), (dict(), "is not on a CUDA device")]
 
 

@@ -157,3 +157,20 @@ def test_two_streams_at_once(ops):
     torch.cuda.synchronize()
     ops.check_device_errors()
     assert all(torch.equal(o, wants[i]) for i in range(2) for o in outs[i])
+
+
+def test_a_step_without_tokens_and_operands_that_start_anywhere(ops):
+    step = _step(((2, 40),), [3, 9], [1, 1], 12, 2, 128, 16, BF16, 6)
+    pools, tables = step.on()
+    none = ops.paged_attention_prefix(pools[0][:0], *pools[1:], *tables, step.prefix_len.cuda(), step.groups.cuda(), *step.sizes, *_limits(step), step.scale)
+    assert none.shape == (0, 12 * 128)
+    shifted = torch.empty(pools[1].numel() + 4, dtype=BF16, device="cuda")[4:].view_as(pools[1]).copy_(pools[1])
+    with pytest.raises(ops.KernelError, match="16-byte boundary"):
+        ops.paged_attention_prefix(pools[0], shifted, pools[2], *tables, step.prefix_len.cuda(), step.groups.cuda(), *step.sizes, *_limits(step), step.scale)
+    mass = step.mass.cuda()
+    with pytest.raises(ops.KernelError, match="16-byte boundary"):
+        ops.paged_attention_mass(pools[0], pools[1], shifted, mass, *tables, *step.sizes, *step.longest, step.scale)
+    assert ops.paged_attention_mass(pools[0][:0], *pools[1:], mass, *tables, *step.sizes, *step.longest, step.scale).shape == (0, 12 * 128)
+    assert torch.equal(mass.cpu(), step.mass)
+    with pytest.raises(ops.KernelError, match="values is not contiguous"):
+        ops.paged_attention_mass(pools[0], pools[1], pools[2].transpose(0, 1).contiguous().transpose(0, 1), mass, *tables, *step.sizes, *step.longest, step.scale)
