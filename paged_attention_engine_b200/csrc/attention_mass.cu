@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) mass_merge_kernel(__nv_bfloa
 // ---------------------------------------------------------------------------------------
 constexpr int ANY_KEYS = 64;
 constexpr int ANY_THREADS = 128;
+constexpr int AT_ONCE = 8;               // pieces of keys and of values that a thread asks for before it waits for any
 constexpr int ANY_ROWS = 16;
 
 template <typename T>
@@ -268,17 +269,27 @@ __global__ void __launch_bounds__(ANY_THREADS) any_slices_kernel(const AnyParams
   for (int key0 = begin; key0 < end; key0 += ANY_KEYS) {
     const int count = min(ANY_KEYS, end - key0);
     __syncthreads();                                     // the tile before is read
-    for (int i = tid; i < ANY_KEYS * units; i += ANY_THREADS) {
-      const int row = i / units, c = (i % units) * 4;
-      float4 kv = make_float4(0.f, 0.f, 0.f, 0.f), vv = kv;
-      if (row < count) {
-        const int j = key0 + row, page = checked_page(p.m.block_table[(size_t)b * p.m.table_width + checked_table_index(j / p.m.page_size, p.m.table_width)]);
-        const size_t at = (((size_t)page * p.m.kv_heads + g) * p.m.page_size + j % p.m.page_size) * p.d + c;
-        kv = load4(p.keys + at);
-        vv = load4(p.values + at);
+    for (int i0 = tid; i0 < ANY_KEYS * units; i0 += ANY_THREADS * AT_ONCE) {
+      float4 kv[AT_ONCE], vv[AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = i0 + u * ANY_THREADS, row = i / units, c = (i % units) * 4;
+        kv[u] = vv[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row < count) {
+          const int j = key0 + row, page = checked_page(p.m.block_table[(size_t)b * p.m.table_width + checked_table_index(j / p.m.page_size, p.m.table_width)]);
+          const size_t at = (((size_t)page * p.m.kv_heads + g) * p.m.page_size + j % p.m.page_size) * p.d + c;
+          kv[u] = load4(p.keys + at);
+          vv[u] = load4(p.values + at);
+        }
       }
-      *(float4*)(k + row * stride + c) = kv;
-      *(float4*)(v + row * p.d + c) = vv;
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = i0 + u * ANY_THREADS, row = i / units, c = (i % units) * 4;
+        if (row < ANY_KEYS) {
+          *(float4*)(k + row * stride + c) = kv[u];
+          *(float4*)(v + row * p.d + c) = vv[u];
+        }
+      }
     }
     __syncthreads();
     {

@@ -15,6 +15,8 @@
 //            own keys, which few rows read, a tile costs little more than its bytes.
 //   merge    a row's slices, shared and own, in their order.
 //
+// Other types and sizes than those of the tensor-core kernel take the same slices of 16 rows on CUDA cores (any_slices_kernel).
+//
 // Scores are scaled in float32, maxima, sums and outputs are float32; probabilities are rounded to bfloat16 for the second
 // product, as the value operand is, and the result once. Every wait on an mbarrier is bounded and reports through `error`.
 #include <cfloat>
@@ -53,6 +55,7 @@ struct Params {
   int shared_blocks, row_tiles, shared_slices, shared_keys;      // keys per slice of the shared ones, a multiple of BKEYS
   int own_row_tiles, own_slices, own_keys;                       // likewise of the own ones
   int slots;                    // slices of a row at most: shared ones, then own ones
+  int box;                      // own slices start on multiples of it
   float scale_log2, slack;
   int* error;
 };
@@ -107,15 +110,16 @@ struct PageRun {
     return __shfl_sync(0xffffffffu, held, box & 31);
   }
 };
-// Where the own keys of a tile of ROWS rows begin and end; their slices start at `base`, where a box of rows does.
+// Where the own keys of a tile of TILE_ROWS rows begin and end; their slices start at `base`, where a box of rows does.
 struct OwnSpan {
   int first, base, end;
 };
+template <int TILE_ROWS>
 __device__ __forceinline__ OwnSpan own_span(const Params& p, int shared, int kv_len, int pos0, int tokens, int groups, int row_tile) {
   OwnSpan s;
   s.first = shared;
-  s.base = shared & -min(p.page_size, BKEYS);
-  s.end = min(kv_len, pos0 + min((row_tile * ROWS + ROWS - 1) / groups, tokens - 1) + 1);
+  s.base = shared / p.box * p.box;
+  s.end = min(kv_len, pos0 + min((row_tile * TILE_ROWS + TILE_ROWS - 1) / groups, tokens - 1) + 1);
   return s;
 }
 
@@ -125,6 +129,7 @@ struct Work {
   int b, g, first_token, row0, rows, begin, end, first, pos0, slot;
 };
 constexpr int EVERY_KEY = 1 << 30;       // pos0 of rows behind all keys
+template <int TILE_ROWS>
 __device__ __forceinline__ Work find_work(const Params& p, int index) {
   const int groups = p.heads / p.kv_heads;
   Work w = {0, 0, 0, 0, 0, 0, 0, 0, EVERY_KEY, 0};
@@ -140,8 +145,8 @@ __device__ __forceinline__ Work find_work(const Params& p, int index) {
     const int b_end = p.group_start[group + 1];
     if (w.b >= b_end) return w;
     w.first_token = p.q_start[w.b];
-    w.row0 = row_tile * ROWS;
-    w.rows = min(ROWS, (p.q_start[b_end] - w.first_token) * groups - w.row0);
+    w.row0 = row_tile * TILE_ROWS;
+    w.rows = min(TILE_ROWS, (p.q_start[b_end] - w.first_token) * groups - w.row0);
     w.begin = w.slot * p.shared_keys;
     w.end = min(min(p.prefix_len[w.b], p.max_prefix), w.begin + p.shared_keys);
     return w;
@@ -156,10 +161,10 @@ __device__ __forceinline__ Work find_work(const Params& p, int index) {
   w.first_token = p.q_start[w.b];
   const int tokens = p.q_start[w.b + 1] - w.first_token, shared = min(p.prefix_len[w.b], p.max_prefix);
   w.pos0 = p.q_pos0[w.b];
-  const OwnSpan span = own_span(p, shared, p.kv_len[w.b], w.pos0, tokens, groups, row_tile);
+  const OwnSpan span = own_span<TILE_ROWS>(p, shared, p.kv_len[w.b], w.pos0, tokens, groups, row_tile);
   if (span.end <= span.first) return w;
-  w.row0 = row_tile * ROWS;
-  w.rows = min(ROWS, tokens * groups - w.row0);
+  w.row0 = row_tile * TILE_ROWS;
+  w.rows = min(TILE_ROWS, tokens * groups - w.row0);
   w.first = shared;
   w.begin = span.base + slice * p.own_keys;
   w.end = min(span.end, w.begin + p.own_keys);
@@ -179,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
   volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
   auto bar = [&](int which, int i = 0) { return bars + 8u * (which + i); };
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  const Work work = find_work(p, blockIdx.x);
+  const Work work = find_work<ROWS>(p, blockIdx.x);
   if (work.rows <= 0 || work.begin >= work.end) {      // the same in every thread
     dependent_launch_trigger();
     dependent_launch_wait();
@@ -489,9 +494,10 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
 }
 
 // The slices of token i of a request and head r of a kv head: shared ones, then own ones.
+template <int TILE_ROWS>
 __device__ __forceinline__ int slices_of(const Params& p, int shared, int kv_len, int pos0, int tokens, int i, int r) {
   const int groups = p.heads / p.kv_heads;
-  const OwnSpan span = own_span(p, shared, kv_len, pos0, tokens, groups, (i * groups + r) / ROWS);
+  const OwnSpan span = own_span<TILE_ROWS>(p, shared, kv_len, pos0, tokens, groups, (i * groups + r) / TILE_ROWS);
   const int own = span.end > span.first ? (span.end - span.base + p.own_keys - 1) / p.own_keys : 0;
   return min((shared + p.shared_keys - 1) / p.shared_keys + own, p.slots);
 }
@@ -505,7 +511,7 @@ __global__ void __launch_bounds__(pae_attention::MERGE_WARPS * 32) prefix_merge_
   const int shared = min(p.prefix_len[b], p.max_prefix), kv_len = p.kv_len[b], pos0 = p.q_pos0[b];
   dependent_launch_wait();
   if (i >= tokens) return;
-  const int slices = slices_of(p, shared, kv_len, pos0, tokens, i, h % groups);
+  const int slices = slices_of<ROWS>(p, shared, kv_len, pos0, tokens, i, h % groups);
   const size_t row = (size_t)(token0 + i) * p.heads + h, at = row * p.slots;
   pae_attention::merge_parts<D, DEPTH>(out + row * D, p.part_out + at * D, p.part_max + at, p.part_sum + at, slices, p.slots, weights);
 }
@@ -520,7 +526,7 @@ __global__ void __launch_bounds__(128) prefix_merge_rows_kernel(__nv_bfloat16* _
   const int shared = min(p.prefix_len[b], p.max_prefix), kv_len = p.kv_len[b], pos0 = p.q_pos0[b];
   dependent_launch_wait();
   if (i >= tokens || h >= p.heads) return;
-  const int slices = slices_of(p, shared, kv_len, pos0, tokens, i, h % groups);
+  const int slices = slices_of<ROWS>(p, shared, kv_len, pos0, tokens, i, h % groups);
   const size_t row = (size_t)(token0 + i) * p.heads + h, at = row * p.slots;
   const float* maxima = p.part_max + at;
   float top = -FLT_MAX, total = 0.f;
@@ -560,26 +566,220 @@ __global__ void __launch_bounds__(128) prefix_merge_rows_kernel(__nv_bfloat16* _
 }
 
 // ---------------------------------------------------------------------------------------
+// any type and head size, on CUDA cores
+// ---------------------------------------------------------------------------------------
+constexpr int ANY_ROWS = 16;
+constexpr int ANY_THREADS = 128;
+constexpr int AT_ONCE = 8;               // pieces of keys and of values that a thread asks for before it waits for any
+
+// The operands and the result in their type; the Params' own pointers to them are not used.
+template <typename T>
+struct AnyOperands {
+  const T* qkv;
+  const T* keys;
+  const T* values;
+  T* out;
+  int d;                        // a multiple of 4 up to 256
+};
+
+__device__ __forceinline__ float4 load4(const float* from) { return *(const float4*)from; }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* from) {
+  const uint2 v = *(const uint2*)from;
+  const float2 a = __bfloat1622float2(*(const __nv_bfloat162*)&v.x), b = __bfloat1622float2(*(const __nv_bfloat162*)&v.y);
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ void fma4(float4& acc, float w, const float4& v) {
+  acc.x = fmaf(w, v.x, acc.x);
+  acc.y = fmaf(w, v.y, acc.y);
+  acc.z = fmaf(w, v.z, acc.z);
+  acc.w = fmaf(w, v.w, acc.w);
+}
+
+// 64 keys a tile: scores by one thread per key and half of the rows, the running softmax by a warp per row, the output by one thread per four channels and
+// a share of the keys; the shares are added in their order.
+template <typename T>
+__global__ void __launch_bounds__(ANY_THREADS) any_slices_kernel(const AnyOperands<T> x, const Params p) {
+  extern __shared__ __align__(16) float any_smem[];
+  __shared__ float weight[BKEYS][ANY_ROWS], top_of[ANY_ROWS], sum_of[ANY_ROWS], shrink_of[ANY_ROWS];
+  dependent_launch_prologue();
+  const Work work = find_work<ANY_ROWS>(p, blockIdx.x);
+  if (work.rows <= 0 || work.begin >= work.end) return;
+  const int rows = work.rows, groups = p.heads / p.kv_heads, units = x.d / 4, stride = x.d + 4, tid = threadIdx.x;
+  float* q = any_smem;                                   // [ANY_ROWS][d]
+  float* k = q + ANY_ROWS * x.d;                         // [BKEYS][stride]: eight rows' 16 bytes fall into different banks
+  float* v = k + BKEYS * stride;                         // [BKEYS][d]
+  auto token_of = [&](int r) { return work.first_token + (work.row0 + r) / groups; };
+  auto head_of = [&](int r) { return work.g * groups + (work.row0 + r) % groups; };
+  for (int i = tid; i < rows * units; i += ANY_THREADS) {
+    const int r = i / units, c = (i % units) * 4;
+    *(float4*)(q + r * x.d + c) = load4(x.qkv + ((size_t)token_of(r) * (p.heads + 2 * p.kv_heads) + head_of(r)) * x.d + c);
+  }
+  if (tid < ANY_ROWS) {
+    top_of[tid] = -FLT_MAX;
+    sum_of[tid] = 0.f;
+  }
+  const int key = tid % BKEYS, half = tid / BKEYS;
+  const int shares = ANY_THREADS / units, unit = tid % units, share = tid / units;      // threads behind the last share have no part in the output
+  float4 acc[ANY_ROWS];
+#pragma unroll
+  for (int r = 0; r < ANY_ROWS; ++r) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int* table = p.block_table + (size_t)work.b * p.table_width;
+  for (int key0 = work.begin; key0 < work.end; key0 += BKEYS) {
+    const int count = min(BKEYS, work.end - key0);
+    __syncthreads();                                     // the tile before is read
+    for (int i0 = tid; i0 < BKEYS * units; i0 += ANY_THREADS * AT_ONCE) {
+      float4 kv[AT_ONCE], vv[AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = i0 + u * ANY_THREADS, row = i / units, c = (i % units) * 4, j = key0 + row;
+        kv[u] = vv[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row < count && j >= work.first) {
+          const int page = checked_page(table[checked_table_index(j / p.page_size, p.table_width)]);
+          const size_t at = (((size_t)page * p.kv_heads + work.g) * p.page_size + j % p.page_size) * x.d + c;
+          kv[u] = load4(x.keys + at);
+          vv[u] = load4(x.values + at);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = i0 + u * ANY_THREADS, row = i / units, c = (i % units) * 4;
+        if (row < BKEYS) {
+          *(float4*)(k + row * stride + c) = kv[u];
+          *(float4*)(v + row * x.d + c) = vv[u];
+        }
+      }
+    }
+    __syncthreads();
+    {
+      float s[ANY_ROWS / 2];                             // of the key with rows half, half + 2, ...
+#pragma unroll
+      for (int i = 0; i < ANY_ROWS / 2; ++i) s[i] = 0.f;
+      for (int c = 0; c < x.d; c += 4) {
+        const float4 kv = *(const float4*)(k + key * stride + c);
+#pragma unroll
+        for (int i = 0; i < ANY_ROWS / 2; ++i)
+          if (half + 2 * i < rows) {
+            const float4 qv = *(const float4*)(q + (half + 2 * i) * x.d + c);
+            s[i] = fmaf(kv.x, qv.x, fmaf(kv.y, qv.y, fmaf(kv.z, qv.z, fmaf(kv.w, qv.w, s[i]))));
+          }
+      }
+      const int j = key0 + key;
+#pragma unroll
+      for (int i = 0; i < ANY_ROWS / 2; ++i) {
+        const int r = half + 2 * i;
+        if (r < rows) weight[key][r] = key < count && j >= work.first && j <= work.pos0 + (work.row0 + r) / groups ? s[i] * p.scale_log2 : -FLT_MAX;
+      }
+    }
+    __syncthreads();
+    // A warp per row: the running maximum and sum, and the scores become weights.
+    for (int r = tid >> 5; r < rows; r += ANY_THREADS / 32) {
+      const int lane = tid & 31;
+      const float s0 = weight[lane][r], s1 = weight[lane + 32][r];
+      float top = fmaxf(s0, s1);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float before = top_of[r], higher = fmaxf(before, top);
+      const float e0 = s0 == -FLT_MAX ? 0.f : exp2f(s0 - higher), e1 = s1 == -FLT_MAX ? 0.f : exp2f(s1 - higher);
+      weight[lane][r] = e0;
+      weight[lane + 32][r] = e1;
+      const float sum = warp_sum(e0 + e1);
+      __syncwarp();
+      if (lane == 0) {
+        const float shrink = before == -FLT_MAX ? 1.f : exp2f(before - higher);      // without a key all is 0, or not a number
+        sum_of[r] = sum_of[r] * shrink + sum;
+        top_of[r] = higher;
+        shrink_of[r] = shrink;
+      }
+    }
+    __syncthreads();
+    if (share < shares) {
+#pragma unroll
+      for (int r = 0; r < ANY_ROWS; ++r)
+        if (r < rows) {
+          const float shrink = shrink_of[r];
+          acc[r].x *= shrink;
+          acc[r].y *= shrink;
+          acc[r].z *= shrink;
+          acc[r].w *= shrink;
+        }
+      for (int j = share; j < count; j += shares) {
+        const float4 vv = *(const float4*)(v + j * x.d + unit * 4);
+#pragma unroll
+        for (int r = 0; r < ANY_ROWS; r += 4)
+          if (r < rows) {
+            const float4 w = *(const float4*)&weight[j][r];
+            fma4(acc[r], w.x, vv);
+            if (r + 1 < rows) fma4(acc[r + 1], w.y, vv);
+            if (r + 2 < rows) fma4(acc[r + 2], w.z, vv);
+            if (r + 3 < rows) fma4(acc[r + 3], w.w, vv);
+          }
+      }
+    }
+  }
+  __syncthreads();
+  float* sums = k;                                       // [shares][rows][d], over the tiles' memory
+  if (share < shares) {
+#pragma unroll
+    for (int r = 0; r < ANY_ROWS; ++r)
+      if (r < rows) *(float4*)(sums + ((size_t)share * rows + r) * x.d + unit * 4) = acc[r];
+  }
+  __syncthreads();
+  auto at = [&](int r) { return ((size_t)token_of(r) * p.heads + head_of(r)) * p.slots + work.slot; };
+  for (int i = tid; i < rows * units; i += ANY_THREADS) {
+    const int r = i / units, c = (i % units) * 4;
+    float4 total = *(const float4*)(sums + r * x.d + c);
+    for (int s = 1; s < shares; ++s) fma4(total, 1.f, *(const float4*)(sums + ((size_t)s * rows + r) * x.d + c));
+    *(float4*)(p.part_out + at(r) * x.d + c) = total;
+  }
+  if (tid < rows) {
+    p.part_max[at(tid)] = top_of[tid];
+    p.part_sum[at(tid)] = sum_of[tid];
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ANY_THREADS) any_merge_kernel(const AnyOperands<T> x, const Params p) {
+  dependent_launch_prologue();
+  const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0;
+  if (i >= tokens) return;
+  const int slices = slices_of<ANY_ROWS>(p, min(p.prefix_len[b], p.max_prefix), p.kv_len[b], p.q_pos0[b], tokens, i, h % groups);
+  const size_t row = (size_t)(token0 + i) * p.heads + h, at = row * p.slots;
+  float top = -FLT_MAX, total = 0.f;
+  for (int s = lane; s < slices; s += 32) top = fmaxf(top, p.part_max[at + s]);           // every warp works them out for itself
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int s = lane; s < slices; s += 32) total += p.part_sum[at + s] * exp2f(p.part_max[at + s] - top);
+  total = warp_sum(total);
+  const float inverse = total > 0.f ? 1.f / total : 0.f;
+  for (int c = threadIdx.x; c < x.d; c += ANY_THREADS) {
+    float sum = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < slices; ++s) sum = fmaf(exp2f(p.part_max[at + s] - top), p.part_out[(at + s) * x.d + c], sum);
+    x.out[row * x.d + c] = from_float<T>(sum * inverse);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
 // how the keys are cut
 // ---------------------------------------------------------------------------------------
 struct Cut {
   int row_tiles, shared_slices, shared_keys, own_row_tiles, own_slices, own_keys, slots;
   long long shared_blocks, own_blocks;
 };
-// Two blocks share an SM. Own keys are cut into as many slices as fill a wave, of one tile at least and OWN_TILES at most. The shared keys' blocks fill
+// Two blocks share an SM (three of the CUDA-core kernel). Own keys are cut into as many slices as fill a wave, of one tile at least and OWN_TILES at most. The shared keys' blocks fill
 // that share of one wave that their tiles are of all tiles (a request's own keys taken as half of the longest's), half of it at least: what is left
 // goes to the own blocks, which wait for memory while the others compute. 64 requests, 8,000 shared and 20 to 700 own keys, 28 heads over 4 of
 // 128, us with the merge: 37.6 with the wave full of shared blocks, 36.2 with three quarters, 33.5 with half; 24 requests of five
 // tokens, 30,011 shared and 100 to 900 own keys, 40 heads over 8: 94.8, 112 and 154.
-constexpr int SHARED_TILES = 2;   // of a slice at least
 constexpr int OWN_TILES = 12;
-Cut cut_keys(int seqs, int groups, int heads, int kv_heads, int page_size, int max_q_len, int max_prefix, int max_own, int max_group_tokens) {
-  const int share = heads / kv_heads, wave = 2 * pae_attention::multiprocessors();
+Cut cut_keys(int seqs, int groups, int heads, int kv_heads, int box, int max_q_len, int max_prefix, int max_own, int max_group_tokens, bool any) {
+  const int share = heads / kv_heads, wave = (any ? 3 : 2) * pae_attention::multiprocessors(), rows = any ? ANY_ROWS : ROWS;
   Cut c;
-  c.row_tiles = (int)(((long long)max_group_tokens * share + ROWS - 1) / ROWS);
-  c.own_row_tiles = (int)(((long long)max_q_len * share + ROWS - 1) / ROWS);
+  c.row_tiles = (int)(((long long)max_group_tokens * share + rows - 1) / rows);
+  c.own_row_tiles = (int)(((long long)max_q_len * share + rows - 1) / rows);
   const long long pairs = (long long)seqs * kv_heads * c.own_row_tiles;
-  const int own_tiles = (max_own + (page_size < BKEYS ? page_size : BKEYS) - 1 + BKEYS - 1) / BKEYS;     // a span may begin inside a box
+  const int own_tiles = (max_own + box - 1 + BKEYS - 1) / BKEYS;     // a span may begin inside a box
   long long most = wave / pairs;
   if (most < (own_tiles + OWN_TILES - 1) / OWN_TILES) most = (own_tiles + OWN_TILES - 1) / OWN_TILES;
   if (most > own_tiles) most = own_tiles;
@@ -593,7 +793,8 @@ Cut cut_keys(int seqs, int groups, int heads, int kv_heads, int page_size, int m
   const double blocks = wave * fmax(0.5, shared_work / fmax(1.0, shared_work + own_work));
   long long slices = (long long)(blocks / per_slice + 0.5);
   while (slices > 1 && slices * per_slice > wave) --slices;
-  if (slices > (tiles + SHARED_TILES - 1) / SHARED_TILES) slices = (tiles + SHARED_TILES - 1) / SHARED_TILES;
+  const int least = any ? 1 : 2;                         // tiles of a shared slice
+  if (slices > (tiles + least - 1) / least) slices = (tiles + least - 1) / least;
   if (slices < 1) slices = 1;
   const int slice_tiles = tiles > 0 ? (int)((tiles + slices - 1) / slices) : 1;
   c.shared_keys = slice_tiles * BKEYS;
@@ -621,39 +822,31 @@ int launch(const Params& p, void* out, long long pages, int blocks, int seqs, in
   return check_launch("paged_attention_prefix");
 }
 
-}  // namespace
-
-PAE_DEFINE_LAST_ERROR()
-
-PAE_EXPORT int pae_attention_prefix_supports(int heads, int kv_heads, int d, int page_size) {
-  return (d == 64 || d == 128) && (page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128) && kv_heads >= 1 && heads % kv_heads == 0;
+template <typename T>
+int launch_any(const AnyOperands<T>& x, const Params& p, int blocks, int seqs, int max_q_len, cudaStream_t s) {
+  const size_t tiles = (size_t)BKEYS * (2 * x.d + 4), shares = (size_t)(ANY_THREADS / (x.d / 4)) * ANY_ROWS * x.d;
+  const size_t bytes = ((size_t)ANY_ROWS * x.d + (tiles > shares ? tiles : shares)) * sizeof(float);
+  static DevicesSet devices;
+  if (int err = raise_shared_memory(devices, any_slices_kernel<T>, 160 * 1024, "paged_attention_prefix")) return err;
+  launch_kernel(any_slices_kernel<T>, dim3(blocks), dim3(ANY_THREADS), bytes, s, x, p);
+  if (int err = check_launch("paged_attention_prefix")) return err;
+  launch_kernel(any_merge_kernel<T>, dim3(p.heads, max_q_len, seqs), dim3(ANY_THREADS), 0, s, x, p);
+  return check_launch("paged_attention_prefix");
 }
 
-// Floats of scratch that pae_paged_attention_prefix needs for the same sizes.
-PAE_EXPORT long long pae_attention_prefix_floats(int tokens, int seqs, int groups, int heads, int kv_heads, int d, int page_size, int max_q_len, int max_prefix,
-                                                 int max_own, int max_group_tokens) {
-  const Cut c = cut_keys(seqs, groups, heads, kv_heads, page_size, max_q_len, max_prefix, max_own, max_group_tokens);
-  return (long long)tokens * heads * c.slots * (d + 2);
-}
+int box_of(int page_size, bool any) { return any ? 1 : (page_size < BKEYS ? page_size : BKEYS); }
 
-PAE_EXPORT int pae_paged_attention_prefix(void* out, const void* qkv, const void* keys, const void* values, long long pages, const int* block_table,
-                                          int table_width, const int* q_start, const int* q_pos0, const int* kv_len, const int* prefix_len,
-                                          const int* group_start, int tokens, int seqs, int groups, int heads, int kv_heads, int d, int page_size,
-                                          int max_q_len, int max_prefix, int max_own, int max_group_tokens, float scale, float* scratch, int* error,
-                                          void* stream) {
-  if (tokens == 0 || seqs == 0) return 0;
-  if (!pae_attention_prefix_supports(heads, kv_heads, d, page_size))
-    return fail(2, "paged_attention_prefix: head_dim %d with pages of %d is not taken (64 or 128; 16, 32, 64 or 128)", d, page_size);
+// What the kernels are told of a step, but for its operands.
+int set_up(Params* to, long long* blocks, const int* block_table, int table_width, const int* q_start, const int* q_pos0, const int* kv_len, const int* prefix_len,
+           const int* group_start, int tokens, int seqs, int groups, int heads, int kv_heads, int d, int page_size, int max_q_len, int max_prefix, int max_own,
+           int max_group_tokens, float scale, float* scratch, bool any) {
   if (seqs > 65535 || max_q_len > 65535) return fail(3, "paged_attention_prefix: %d requests of up to %d tokens exceed one launch", seqs, max_q_len);
-  if ((((uintptr_t)qkv | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)out | (uintptr_t)scratch) & 15) != 0)
-    return fail(2, "paged_attention_prefix: an operand does not start on a 16-byte boundary");
-  const Cut c = cut_keys(seqs, groups, heads, kv_heads, page_size, max_q_len, max_prefix, max_own, max_group_tokens);
-  if ((size_t)(c.slots + pae_attention::MERGE_WARPS * d) * sizeof(float) > 40 * 1024 || c.shared_blocks + c.own_blocks > 0x7fffffffll)
+  if ((uintptr_t)scratch & 15) return fail(2, "paged_attention_prefix: the scratch does not start on a 16-byte boundary");
+  const Cut c = cut_keys(seqs, groups, heads, kv_heads, box_of(page_size, any), max_q_len, max_prefix, max_own, max_group_tokens, any);
+  if ((size_t)(c.slots + pae_attention::MERGE_WARPS * d) * sizeof(float) > 40 * 1024 || c.shared_blocks + c.own_blocks > 0x7fffffffll ||
+      (long long)tokens * heads * c.slots > 0xffffffffll)
     return fail(3, "paged_attention_prefix: %d slices a row, %lld + %lld blocks exceed one launch", c.slots, c.shared_blocks, c.own_blocks);
   Params p = {};
-  p.qkv = (const __nv_bfloat16*)qkv;
-  p.keys = (const __nv_bfloat16*)keys;
-  p.values = (const __nv_bfloat16*)values;
   p.block_table = block_table;
   p.q_start = q_start;
   p.q_pos0 = q_pos0;
@@ -677,9 +870,68 @@ PAE_EXPORT int pae_paged_attention_prefix(void* out, const void* qkv, const void
   p.own_slices = c.own_slices;
   p.own_keys = c.own_keys;
   p.slots = c.slots;
+  p.box = box_of(page_size, any);
   p.scale_log2 = scale * LOG2E;
   p.slack = REFERENCE_SLACK;
+  *to = p;
+  *blocks = c.shared_blocks + c.own_blocks;
+  return 0;
+}
+
+}  // namespace
+
+PAE_DEFINE_LAST_ERROR()
+
+PAE_EXPORT int pae_attention_prefix_supports(int heads, int kv_heads, int d, int page_size) {
+  return (d == 64 || d == 128) && (page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128) && kv_heads >= 1 && heads % kv_heads == 0;
+}
+
+// Floats of scratch that pae_paged_attention_prefix (any = 0) or pae_paged_attention_prefix_any (any = 1) needs for the same sizes.
+PAE_EXPORT long long pae_attention_prefix_floats(int tokens, int seqs, int groups, int heads, int kv_heads, int d, int page_size, int max_q_len, int max_prefix,
+                                                 int max_own, int max_group_tokens, int any) {
+  const Cut c = cut_keys(seqs, groups, heads, kv_heads, box_of(page_size, any), max_q_len, max_prefix, max_own, max_group_tokens, any);
+  return (long long)tokens * heads * c.slots * (d + 2);
+}
+
+PAE_EXPORT int pae_paged_attention_prefix(void* out, const void* qkv, const void* keys, const void* values, long long pages, const int* block_table,
+                                          int table_width, const int* q_start, const int* q_pos0, const int* kv_len, const int* prefix_len,
+                                          const int* group_start, int tokens, int seqs, int groups, int heads, int kv_heads, int d, int page_size,
+                                          int max_q_len, int max_prefix, int max_own, int max_group_tokens, float scale, float* scratch, int* error,
+                                          void* stream) {
+  if (tokens == 0 || seqs == 0) return 0;
+  if (!pae_attention_prefix_supports(heads, kv_heads, d, page_size))
+    return fail(2, "paged_attention_prefix: head_dim %d with pages of %d is not taken (64 or 128; 16, 32, 64 or 128)", d, page_size);
+  if ((((uintptr_t)qkv | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)out) & 15) != 0)
+    return fail(2, "paged_attention_prefix: an operand does not start on a 16-byte boundary");
+  Params p;
+  long long blocks;
+  if (int err = set_up(&p, &blocks, block_table, table_width, q_start, q_pos0, kv_len, prefix_len, group_start, tokens, seqs, groups, heads, kv_heads, d, page_size,
+                       max_q_len, max_prefix, max_own, max_group_tokens, scale, scratch, false))
+    return err;
+  p.qkv = (const __nv_bfloat16*)qkv;
+  p.keys = (const __nv_bfloat16*)keys;
+  p.values = (const __nv_bfloat16*)values;
   p.error = error;
-  if (d == 64) return launch<64>(p, out, pages, (int)(c.shared_blocks + c.own_blocks), seqs, max_q_len, (cudaStream_t)stream);
-  return launch<128>(p, out, pages, (int)(c.shared_blocks + c.own_blocks), seqs, max_q_len, (cudaStream_t)stream);
+  if (d == 64) return launch<64>(p, out, pages, (int)blocks, seqs, max_q_len, (cudaStream_t)stream);
+  return launch<128>(p, out, pages, (int)blocks, seqs, max_q_len, (cudaStream_t)stream);
+}
+
+// The same on CUDA cores: dtype 0 float32, 1 bfloat16; head sizes that are multiples of 4 up to 256, pages of any size.
+PAE_EXPORT int pae_paged_attention_prefix_any(void* out, const void* qkv, const void* keys, const void* values, const int* block_table, int table_width,
+                                              const int* q_start, const int* q_pos0, const int* kv_len, const int* prefix_len, const int* group_start, int tokens,
+                                              int seqs, int groups, int heads, int kv_heads, int d, int page_size, int max_q_len, int max_prefix, int max_own,
+                                              int max_group_tokens, float scale, int dtype, float* scratch, void* stream) {
+  if (tokens == 0 || seqs == 0) return 0;
+  if (d < 4 || d > 256 || d % 4) return fail(2, "paged_attention_prefix: head_dim %d is not a multiple of 4 up to 256", d);
+  if (kv_heads < 1 || heads % kv_heads) return fail(2, "paged_attention_prefix: %d heads over %d kv heads", heads, kv_heads);
+  if (((uintptr_t)qkv | (uintptr_t)keys | (uintptr_t)values) & (dtype == kF32 ? 15 : 7))
+    return fail(2, "paged_attention_prefix: an operand does not start on a boundary of four elements");
+  Params p;
+  long long blocks;
+  if (int err = set_up(&p, &blocks, block_table, table_width, q_start, q_pos0, kv_len, prefix_len, group_start, tokens, seqs, groups, heads, kv_heads, d, page_size,
+                       max_q_len, max_prefix, max_own, max_group_tokens, scale, scratch, true))
+    return err;
+  if (dtype == kF32) return launch_any<float>({(const float*)qkv, (const float*)keys, (const float*)values, (float*)out, d}, p, (int)blocks, seqs, max_q_len, (cudaStream_t)stream);
+  return launch_any<__nv_bfloat16>({(const __nv_bfloat16*)qkv, (const __nv_bfloat16*)keys, (const __nv_bfloat16*)values, (__nv_bfloat16*)out, d}, p, (int)blocks, seqs,
+                                   max_q_len, (cudaStream_t)stream);
 }

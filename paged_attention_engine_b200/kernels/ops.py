@@ -2375,6 +2375,10 @@ def _need_attention(what: str, qkv, keys, values, block_table, q_start, q_pos0, 
 # From how many tokens a request on a step is an ordinary one: a query tile of one request fills the tensor cores then, and its keys are
 # read once for all of its tokens anyway.
 PREFIX_ATTENTION_MAX_TOKENS = 63
+# From how many shared keys on the CUDA-core kernel takes them once for all. us a pass, captured, shared and each request by itself, float32, 12 heads over 2 of 64:
+# 2 requests behind 200 keys 15 and 8, 16 behind 1,000 20.3 and 19.5, 64 behind 2,000 56 and 92, 4 behind 8,000 35 and 106; 32 of 28 heads over 4 of 128
+# behind 4,000 293 and 416.
+PREFIX_SIMT_MIN_KEYS = 1024
 
 
 _PREFIX_TENSORS = (*_STEP_TENSORS, "prefix_len", "group_start")
@@ -2407,8 +2411,10 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     prefix_len[b] keys (int32 [requests], the same for all of a group; 0: nothing is shared) are the same, and every token of the step stands behind
     them. They are read through the block table of the group's first request. The result is that of `paged_attention` but for the order of the sums.
     The longest request brings at most `max_q_len` tokens, the largest group `max_group_tokens`; `max_prefix_len` and `max_own_len` bound the shared keys and the
-    keys behind them. `info`, when given, receives which kernel ran ("kernel": "shared", or what `paged_attention` says where each request reads its
-    keys by itself: other types, head sizes and page sizes than the tensor-core kernel's, long portions, groups of one request)."""
+    keys behind them. `info`, when given, receives which kernel ran ("kernel"): "shared", on tensor cores (bfloat16, head sizes 64 and 128, pages
+    of 16, 32, 64 or 128 keys), "shared simt" (long prefixes in float32 and of what no tensor-core attention takes; head sizes that are multiples of 4 up
+    to 256), or what
+    `paged_attention` says where each request reads its keys by itself (other sizes, long portions, groups of one request)."""
     qkv = materialized(qkv)
     what = "paged_attention_prefix"
     tokens, seqs, table_width, pages = _need_attention(what, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim,
@@ -2428,22 +2434,33 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     operands = _aligned_operands(what, qkv, keys, values, head_dim)
     if tokens == 0:
         return qkv.new_empty((0, num_heads * head_dim))
-    if not (qkv.dtype is torch.bfloat16 and use_tensor_cores and 0 < max_q_len <= PREFIX_ATTENTION_MAX_TOKENS and max_prefix_len > 0
-            and max_group_tokens > max_q_len and _prefix_supports(num_heads, num_kv_heads, head_dim, page_size)):
+    sizes = (tokens, seqs, groups, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_prefix_len, max_own_len, max_group_tokens)
+    form = None
+    if 0 < max_q_len <= PREFIX_ATTENTION_MAX_TOKENS and max_prefix_len > 0 and max_group_tokens > max_q_len:
+        if qkv.dtype is torch.bfloat16 and use_tensor_cores and _prefix_supports(num_heads, num_kv_heads, head_dim, page_size):
+            form = "shared"
+        elif max_prefix_len >= PREFIX_SIMT_MIN_KEYS and head_dim % 4 == 0 and head_dim <= 256 and not plain_attention_takes(num_heads, num_kv_heads, head_dim, page_size, qkv.dtype) and not (
+                operands[0] | operands[1] | operands[2]) & (4 * qkv.element_size() - 1):
+            form = "shared simt"
+    if form is None:
         return paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len,
                                min(max_prefix_len + max_own_len, table_width * page_size), scale, 0, num_single=num_single, info=info)
     if info is not None:
-        info.update(kernel="shared")
+        info.update(kernel=form)
     lib = _lib("attention_prefix")
     out = qkv.new_empty((tokens, num_heads * head_dim))
-    floats = _prefix_floats(tokens, seqs, groups, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_prefix_len, max_own_len, max_group_tokens)
-    scratch = qkv.new_empty(2 * floats)                   # bfloat16
     if bounds_checked:
         _set_bounds("attention_prefix", keys)
-    _check(lib, lib.pae_paged_attention_prefix(
-        out.data_ptr(), *operands, pages, block_table.data_ptr(), table_width, q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(),
-        prefix_len.data_ptr(), group_start.data_ptr(), tokens, seqs, groups, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_prefix_len,
-        max_own_len, max_group_tokens, scale, scratch.data_ptr(), _error_flag(qkv.device).data_ptr(), _stream()), 2)
+    if form == "shared":
+        scratch = qkv.new_empty(2 * _prefix_floats(*sizes, 0))            # bfloat16
+        _check(lib, lib.pae_paged_attention_prefix(
+            out.data_ptr(), *operands, pages, block_table.data_ptr(), table_width, q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(),
+            prefix_len.data_ptr(), group_start.data_ptr(), *sizes, scale, scratch.data_ptr(), _error_flag(qkv.device).data_ptr(), _stream()), 2)
+        return out
+    scratch = torch.empty(_prefix_floats(*sizes, 1), dtype=torch.float32, device=qkv.device)
+    _check(lib, lib.pae_paged_attention_prefix_any(
+        out.data_ptr(), *operands, block_table.data_ptr(), table_width, q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(), prefix_len.data_ptr(),
+        group_start.data_ptr(), *sizes, scale, _code(qkv), scratch.data_ptr(), _stream()), 2)
     return out
 
 

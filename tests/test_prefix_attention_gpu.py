@@ -15,7 +15,9 @@ F32, BF16 = torch.float32, torch.bfloat16
 def ops():
     from paged_attention_engine_b200.kernels import ops as kernel_ops
 
-    return kernel_ops
+    least, kernel_ops.PREFIX_SIMT_MIN_KEYS = kernel_ops.PREFIX_SIMT_MIN_KEYS, 1        # every case by the kernel that shares
+    yield kernel_ops
+    kernel_ops.PREFIX_SIMT_MIN_KEYS = least
 
 
 def _limits(step):
@@ -44,7 +46,7 @@ def _step(shared, own, tokens, heads, kv_heads, dim, page, dtype, seed, **more):
 
 
 SIZES = [(12, 2, 128, 16, BF16), (28, 4, 128, 32, BF16), (14, 2, 64, 64, BF16), (8, 8, 64, 128, BF16), (40, 2, 128, 16, BF16), (3, 1, 32, 16, BF16), (12, 2, 64, 48, BF16),
-         (4, 2, 64, 16, F32), (6, 3, 48, 7, F32)]
+         (4, 2, 64, 16, F32), (6, 3, 48, 7, F32), (40, 2, 128, 16, F32)]
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", SIZES)
@@ -60,7 +62,8 @@ def test_groups(ops, heads, kv_heads, dim, page, dtype, shared, own, tokens):
     step = _step(shared, own, tokens, heads, kv_heads, dim, page, dtype, heads + len(own))
     info = {}
     out = _run(ops, step, info=info)
-    assert (info["kernel"] == "shared") == (dtype == BF16 and dim in (64, 128) and page != 48)
+    takes = "shared" if dtype == BF16 and dim in (64, 128) and page != 48 else "shared simt" if dtype == F32 else "mma"
+    assert info["kernel"] == takes
     _check(step, out)
 
 
@@ -174,3 +177,22 @@ def test_a_step_without_tokens_and_operands_that_start_anywhere(ops):
     assert torch.equal(mass.cpu(), step.mass)
     with pytest.raises(ops.KernelError, match="values is not contiguous"):
         ops.paged_attention_mass(pools[0], pools[1], pools[2].transpose(0, 1).contiguous().transpose(0, 1), mass, *tables, *step.sizes, *step.longest, step.scale)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", [(12, 2, 64, 16, F32), (8, 2, 256, 16, F32), (5, 1, 20, 16, BF16), (3, 3, 4, 5, F32), (20, 1, 100, 48, BF16)])
+def test_many_keys_on_cuda_cores(ops, heads, kv_heads, dim, page, dtype):
+    step = _step(((9, 1500), (3, 2100)), [1 + 37 * b % 150 for b in range(12)], [1] * 12, heads, kv_heads, dim, page, dtype, dim)
+    info = {}
+    out = _run(ops, step, info=info)
+    assert info["kernel"] == "shared simt"
+    _check(step, out)
+    ops.PREFIX_SIMT_MIN_KEYS = 1 << 30
+    try:
+        if dim % 8:                            # no attention of a request by itself takes it
+            with pytest.raises(ops.KernelError, match="not a multiple of 8"):
+                _run(ops, step)
+        else:
+            _run(ops, step, info=info)
+            assert info["kernel"] == "simt"
+    finally:
+        ops.PREFIX_SIMT_MIN_KEYS = 1
