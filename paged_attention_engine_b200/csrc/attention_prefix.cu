@@ -15,6 +15,10 @@
 //            own keys, which few rows read, a tile costs little more than its bytes.
 //   merge    a row's slices, shared and own, in their order.
 //
+// The same kernel without shared keys is the attention of paged_attention_mass for steps of few tokens: it leaves its scores besides (4 bytes for each query
+// head and key, where keys and values are 4 * head size bytes for each kv head and key), and further blocks of the merge turn them into
+// weights once a row's maximum and sum are known, and add them up per key (attention_mass.cu says what is computed).
+//
 // Other types and sizes than those of the tensor-core kernel take the same slices of 16 rows on CUDA cores (any_slices_kernel).
 //
 // Scores are scaled in float32, maxima, sums and outputs are float32; probabilities are rounded to bfloat16 for the second
@@ -56,6 +60,8 @@ struct Params {
   int own_row_tiles, own_slices, own_keys;                       // likewise of the own ones
   int slots;                    // slices of a row at most: shared ones, then own ones
   int box;                      // own slices start on multiples of it
+  float* scores;                // [tokens, heads, span], not scaled, of own keys
+  int span;
   float scale_log2, slack;
   int* error;
 };
@@ -159,7 +165,7 @@ __device__ __forceinline__ Work find_work(const Params& p, int index) {
   w.g = index % p.kv_heads;
   w.b = index / p.kv_heads;
   w.first_token = p.q_start[w.b];
-  const int tokens = p.q_start[w.b + 1] - w.first_token, shared = min(p.prefix_len[w.b], p.max_prefix);
+  const int tokens = p.q_start[w.b + 1] - w.first_token, shared = p.max_prefix > 0 ? min(p.prefix_len[w.b], p.max_prefix) : 0;
   w.pos0 = p.q_pos0[w.b];
   const OwnSpan span = own_span<TILE_ROWS>(p, shared, p.kv_len[w.b], w.pos0, tokens, groups, row_tile);
   if (span.end <= span.first) return w;
@@ -172,7 +178,7 @@ __device__ __forceinline__ Work find_work(const Params& p, int index) {
   return w;
 }
 
-template <int D>
+template <int D, bool SCORES>
 __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constant__ PageMaps maps, const Params p) {
   using L = Layout<D>;
   extern __shared__ uint8_t raw_smem[];
@@ -389,7 +395,16 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
         return (sums[0] + sums[1]) + (sums[2] + sums[3]);
       };
       const uint32_t scores = lane_base + st * L::S_COLUMNS;
-      bool taken = false;
+      auto leave = [&](const float* s, int first, int count) {
+        if constexpr (SCORES) {
+          if (r < rows) {
+            float* to = p.scores + (token * p.heads + head) * p.span + key0 + first;
+#pragma unroll
+            for (int i = 0; i < count; i += 4) *(float4*)(to + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+          }
+        }
+      };
+      bool taken = false, left = false;
       float slack = p.slack;
       if (p.slack > 0.f && !__any_sync(0xffffffffu, r < rows && reference == -FLT_MAX)) {
         // Against the references as they are; should a sum come out above REFERENCE_LIMIT (or not a number), the tile is taken again below.
@@ -401,6 +416,9 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
         take32(s, 0);
         tmem_arrived(behind);
         take32(behind, 32);
+        leave(s, 0, 32);
+        leave(behind, 32, 32);
+        left = true;
         const float sum = tile_sum();
         taken = __all_sync(0xffffffffu, sum <= REFERENCE_LIMIT);
         if (taken) row_sum += sum;
@@ -409,6 +427,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
       if (!taken) {
         float s[BKEYS];
         tmem_load64(scores, s);
+        if (!left) leave(s, 0, BKEYS);
         float m4[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX};
         if (unmasked) {
 #pragma unroll
@@ -516,18 +535,10 @@ __global__ void __launch_bounds__(pae_attention::MERGE_WARPS * 32) prefix_merge_
   pae_attention::merge_parts<D, DEPTH>(out + row * D, p.part_out + at * D, p.part_max + at, p.part_sum + at, slices, p.slots, weights);
 }
 
-// The same by one warp a row, for launches of so many rows that warps are there for all SMs: every row is in flight at once.
+// A row's merge by one warp.
 template <int D>
-__global__ void __launch_bounds__(128) prefix_merge_rows_kernel(__nv_bfloat16* __restrict__ out, const Params p) {
-  dependent_launch_trigger();
+__device__ __forceinline__ void merge_row(__nv_bfloat16* __restrict__ out, const Params& p, size_t at, int slices, int lane) {
   constexpr int PER_LANE = D / 32, DEPTH = 8;
-  const int h = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, i = blockIdx.y, b = blockIdx.z;
-  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0;
-  const int shared = min(p.prefix_len[b], p.max_prefix), kv_len = p.kv_len[b], pos0 = p.q_pos0[b];
-  dependent_launch_wait();
-  if (i >= tokens || h >= p.heads) return;
-  const int slices = slices_of<ROWS>(p, shared, kv_len, pos0, tokens, i, h % groups);
-  const size_t row = (size_t)(token0 + i) * p.heads + h, at = row * p.slots;
   const float* maxima = p.part_max + at;
   float top = -FLT_MAX, total = 0.f;
   for (int s = lane; s < slices; s += 32) top = fmaxf(top, maxima[s]);
@@ -561,8 +572,94 @@ __global__ void __launch_bounds__(128) prefix_merge_rows_kernel(__nv_bfloat16* _
   }
   const float inv = total > 0.f ? 1.f / total : 0.f;
 #pragma unroll
-  for (int j = 0; j < PER_LANE; j += 2)
-    *(__nv_bfloat162*)(out + row * D + lane * PER_LANE + j) = __floats2bfloat162_rn(acc[j] * inv, acc[j + 1] * inv);
+  for (int j = 0; j < PER_LANE; j += 2) *(__nv_bfloat162*)(out + lane * PER_LANE + j) = __floats2bfloat162_rn(acc[j] * inv, acc[j + 1] * inv);
+}
+
+// The same by one warp a row, for launches of so many rows that warps are there for all SMs: every row is in flight at once.
+template <int D>
+__global__ void __launch_bounds__(128) prefix_merge_rows_kernel(__nv_bfloat16* __restrict__ out, const Params p) {
+  dependent_launch_trigger();
+  const int h = blockIdx.x * 4 + (threadIdx.x >> 5), i = blockIdx.y, b = blockIdx.z;
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0;
+  const int shared = min(p.prefix_len[b], p.max_prefix), kv_len = p.kv_len[b], pos0 = p.q_pos0[b];
+  dependent_launch_wait();
+  if (i >= tokens || h >= p.heads) return;
+  const size_t row = (size_t)(token0 + i) * p.heads + h;
+  merge_row<D>(out + row * D, p, row * p.slots, slices_of<ROWS>(p, shared, kv_len, pos0, tokens, i, h % groups), threadIdx.x & 31);
+}
+
+// ---------------------------------------------------------------------------------------
+// attention weights added up per key
+// ---------------------------------------------------------------------------------------
+struct MassParams {
+  float* mass;                  // [pages, kv_heads, page_size]
+  const int* slots;             // [tokens] or null: a request whose first slot is negative pads the step
+  int keep_first, row_blocks, chunks;
+};
+constexpr int MASS_CHUNK = 512;          // keys per block of 128 threads, four a thread
+constexpr int MASS_ROWS = 32;            // rows at a time
+
+// Blocks 0 .. row_blocks - 1 of a request merge its rows (a block each, or a warp each where WARPS); the others add the weights of a chunk of one kv head's keys.
+template <int D, bool WARPS>
+__global__ void __launch_bounds__(128) mass_merge_kernel(__nv_bfloat16* __restrict__ out, const Params p, const MassParams m) {
+  dependent_launch_trigger();
+  extern __shared__ float weights[];     // [slots], then [MERGE_WARPS][D]
+  __shared__ float logarithm[MASS_ROWS];
+  const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0, n = p.kv_len[b], pos0 = p.q_pos0[b];
+  dependent_launch_wait();
+  if ((int)blockIdx.x < m.row_blocks) {
+    const int index = WARPS ? (int)blockIdx.x * 4 + warp : (int)blockIdx.x, i = index / p.heads, h = index % p.heads;
+    if (i >= tokens) return;
+    const int slices = slices_of<ROWS>(p, 0, n, pos0, tokens, i, h % groups);
+    const size_t row = (size_t)(token0 + i) * p.heads + h;
+    if constexpr (WARPS) merge_row<D>(out + row * D, p, row * p.slots, slices, lane);
+    else
+      pae_attention::merge_parts<D, 24>(out + row * D, p.part_out + row * p.slots * D, p.part_max + row * p.slots, p.part_sum + row * p.slots, slices, p.slots, weights);
+    return;
+  }
+  const int g = ((int)blockIdx.x - m.row_blocks) / m.chunks, key0 = (((int)blockIdx.x - m.row_blocks) % m.chunks) * MASS_CHUNK;
+  const int last = min(min(n, pos0 + tokens), p.span), rows = tokens * groups;
+  if (rows <= 0 || key0 >= last || key0 + MASS_CHUNK <= m.keep_first || (m.slots != nullptr && m.slots[token0] < 0)) return;
+  const int j0 = key0 + threadIdx.x * 4;
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int first = 0; first < rows; first += MASS_ROWS) {
+    __syncthreads();
+    for (int u = warp; u < min(MASS_ROWS, rows - first); u += 4) {
+      const int i = (first + u) / groups, r = (first + u) % groups;
+      const int slices = slices_of<ROWS>(p, 0, n, pos0, tokens, i, r);
+      const size_t at = ((size_t)(token0 + i) * p.heads + g * groups + r) * p.slots;
+      float top = -FLT_MAX, total = 0.f;
+      for (int s = lane; s < slices; s += 32) top = fmaxf(top, p.part_max[at + s]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int s = lane; s < slices; s += 32) total += p.part_sum[at + s] * exp2f(p.part_max[at + s] - top);
+      total = warp_sum(total);
+      if (lane == 0) logarithm[u] = total == 0.f ? INFINITY : top + log2f(total);      // of a row without a key the weights are 0
+    }
+    __syncthreads();
+    if (j0 < last) {
+      const int count = min(MASS_ROWS, rows - first);
+#pragma unroll 4
+      for (int u = 0; u < count; ++u) {
+        const int i = (first + u) / groups, seen = pos0 + i;
+        const float4 s = *(const float4*)(p.scores + ((size_t)(token0 + i) * p.heads + g * groups + (first + u) % groups) * p.span + j0);
+        const float l = logarithm[u];
+        if (j0 <= seen) w[0] += exp2f(fmaf(s.x, p.scale_log2, -l));
+        if (j0 + 1 <= seen) w[1] += exp2f(fmaf(s.y, p.scale_log2, -l));
+        if (j0 + 2 <= seen) w[2] += exp2f(fmaf(s.z, p.scale_log2, -l));
+        if (j0 + 3 <= seen) w[3] += exp2f(fmaf(s.w, p.scale_log2, -l));
+      }
+    }
+  }
+  for (int k = 0; k < 4; ++k) {
+    const int j = j0 + k;
+    if (j < m.keep_first || j >= last) continue;
+    const int page = page_or_none(p.block_table + (size_t)b * p.table_width, j / p.page_size, p.table_width);
+    if (page < 0) continue;
+    float* to = m.mass + ((size_t)page * p.kv_heads + g) * p.page_size + j % p.page_size;
+    *to = (j >= pos0 ? 0.f : *to) + w[k];
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -809,8 +906,8 @@ int launch(const Params& p, void* out, long long pages, int blocks, int seqs, in
   PageMaps maps;
   if (int err = encode_page_maps(&maps, p.keys, p.values, pages, p.kv_heads, p.page_size, D, BKEYS)) return err;
   static DevicesSet devices;
-  if (int err = raise_shared_memory(devices, prefix_kernel<D>, Layout<D>::SMEM_BYTES, "paged_attention_prefix")) return err;
-  launch_kernel(prefix_kernel<D>, dim3(blocks), dim3(THREADS), Layout<D>::SMEM_BYTES, s, maps, p);
+  if (int err = raise_shared_memory(devices, prefix_kernel<D, false>, Layout<D>::SMEM_BYTES, "paged_attention_prefix")) return err;
+  launch_kernel(prefix_kernel<D, false>, dim3(blocks), dim3(THREADS), Layout<D>::SMEM_BYTES, s, maps, p);
   if (int err = check_launch("paged_attention_prefix")) return err;
   if ((long long)p.heads * max_q_len * seqs >= 8LL * pae_attention::multiprocessors()) {
     launch_kernel(prefix_merge_rows_kernel<D>, dim3((p.heads + 3) / 4, max_q_len, seqs), dim3(128), 0, s, (__nv_bfloat16*)out, p);
@@ -820,6 +917,19 @@ int launch(const Params& p, void* out, long long pages, int blocks, int seqs, in
   launch_kernel(merge, dim3(p.heads, max_q_len, seqs), dim3(pae_attention::MERGE_WARPS * 32),
                 (p.slots + pae_attention::MERGE_WARPS * D) * sizeof(float), s, (__nv_bfloat16*)out, p);
   return check_launch("paged_attention_prefix");
+}
+
+template <int D, bool WARPS>
+int launch_mass(const Params& p, const MassParams& m, void* out, long long pages, int blocks, int seqs, cudaStream_t s) {
+  PageMaps maps;
+  if (int err = encode_page_maps(&maps, p.keys, p.values, pages, p.kv_heads, p.page_size, D, BKEYS)) return err;
+  static DevicesSet devices;
+  if (int err = raise_shared_memory(devices, prefix_kernel<D, true>, Layout<D>::SMEM_BYTES, "paged_attention_mass")) return err;
+  launch_kernel(prefix_kernel<D, true>, dim3(blocks), dim3(THREADS), Layout<D>::SMEM_BYTES, s, maps, p);
+  if (int err = check_launch("paged_attention_mass")) return err;
+  launch_kernel(mass_merge_kernel<D, WARPS>, dim3(m.row_blocks + p.kv_heads * m.chunks, seqs), dim3(128),
+                WARPS ? 0 : (p.slots + pae_attention::MERGE_WARPS * D) * sizeof(float), s, (__nv_bfloat16*)out, p, m);
+  return check_launch("paged_attention_mass");
 }
 
 template <typename T>
@@ -934,4 +1044,42 @@ PAE_EXPORT int pae_paged_attention_prefix_any(void* out, const void* qkv, const 
   if (dtype == kF32) return launch_any<float>({(const float*)qkv, (const float*)keys, (const float*)values, (float*)out, d}, p, (int)blocks, seqs, max_q_len, (cudaStream_t)stream);
   return launch_any<__nv_bfloat16>({(const __nv_bfloat16*)qkv, (const __nv_bfloat16*)keys, (const __nv_bfloat16*)values, (__nv_bfloat16*)out, d}, p, (int)blocks, seqs,
                                    max_q_len, (cudaStream_t)stream);
+}
+
+// Floats of scratch that pae_paged_attention_few_mass needs.
+PAE_EXPORT long long pae_attention_few_mass_floats(int tokens, int seqs, int heads, int kv_heads, int d, int page_size, int max_q_len, int max_kv_len) {
+  const Cut c = cut_keys(seqs, 1, heads, kv_heads, box_of(page_size, false), max_q_len, 0, max_kv_len, max_q_len, false);
+  return (long long)tokens * heads * (c.slots * (d + 2) + (long long)c.own_slices * c.own_keys);
+}
+
+// Attention of a step whose requests bring few tokens, and the weights of their keys; `slots` and `keep_first` as pae_paged_attention_any_mass (attention_mass.cu) takes them.
+PAE_EXPORT int pae_paged_attention_few_mass(void* out, const void* qkv, const void* keys, const void* values, float* mass, long long pages, const int* block_table,
+                                            int table_width, const int* q_start, const int* q_pos0, const int* kv_len, const int* slots, int tokens, int seqs,
+                                            int heads, int kv_heads, int d, int page_size, int max_q_len, int max_kv_len, float scale, int keep_first,
+                                            float* scratch, int* error, void* stream) {
+  if (tokens == 0 || seqs == 0 || max_kv_len < 1) return 0;
+  if (!pae_attention_prefix_supports(heads, kv_heads, d, page_size))
+    return fail(2, "paged_attention_mass: head_dim %d with pages of %d is not taken (64 or 128; 16, 32, 64 or 128)", d, page_size);
+  if ((((uintptr_t)qkv | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)out) & 15) != 0)
+    return fail(2, "paged_attention_mass: an operand does not start on a 16-byte boundary");
+  Params p;
+  long long blocks;
+  if (int err = set_up(&p, &blocks, block_table, table_width, q_start, q_pos0, kv_len, nullptr, nullptr, tokens, seqs, 1, heads, kv_heads, d, page_size, max_q_len, 0,
+                       max_kv_len, max_q_len, scale, scratch, false))
+    return err;
+  p.qkv = (const __nv_bfloat16*)qkv;
+  p.keys = (const __nv_bfloat16*)keys;
+  p.values = (const __nv_bfloat16*)values;
+  p.error = error;
+  p.span = p.own_slices * p.own_keys;
+  p.scores = scratch;                                    // rows of a multiple of 64 floats
+  p.part_out = scratch + (size_t)tokens * heads * p.span;
+  p.part_max = p.part_out + (size_t)tokens * heads * p.slots * d;
+  p.part_sum = p.part_max + (size_t)tokens * heads * p.slots;
+  const int rows = heads * max_q_len;
+  const bool warps = (long long)rows * seqs >= 8LL * pae_attention::multiprocessors();
+  const MassParams m = {mass, slots, keep_first, warps ? (rows + 3) / 4 : rows, (p.span + MASS_CHUNK - 1) / MASS_CHUNK};
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (d == 64) return warps ? launch_mass<64, true>(p, m, out, pages, (int)blocks, seqs, s) : launch_mass<64, false>(p, m, out, pages, (int)blocks, seqs, s);
+  return warps ? launch_mass<128, true>(p, m, out, pages, (int)blocks, seqs, s) : launch_mass<128, false>(p, m, out, pages, (int)blocks, seqs, s);
 }

@@ -2464,6 +2464,34 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     return out
 
 
+# Up to how many tokens a request of a step of several go by slices of the keys, whose scores are kept until the weights are known; longer portions by the
+# attention of prompts and a second pass over the scores. us a pass, captured, the one and the other: 48 requests of five tokens over 300 to 6,000 keys, 28 heads
+# over 4 of 128, 154 and 431, four requests 39 and 92, 16 of 16 tokens 196 and 195. (Single tokens go by slices of their own, csrc/attention_mass.cu: 77 and 90.)
+MASS_FEW_TOKENS = 16
+
+
+@functools.lru_cache(maxsize=64)
+def _prompt_mass_supports(*sizes) -> bool:
+    return bool(_lib("attention_mass_prompt").pae_attention_mass_prompt_supports(*sizes))
+
+
+@functools.lru_cache(maxsize=1024)
+def _few_mass_floats(*sizes) -> int:
+    return _lib("attention_prefix").pae_attention_few_mass_floats(*sizes)
+
+
+def _few_mass(out, qkv, keys, operands, mass, pages: int, block_table, table_width: int, q_start, q_pos0, kv_len, slots, tokens: int, seqs: int, sizes,
+              max_q_len: int, max_kv_len: int, scale: float, keep_first: int) -> None:
+    """A step whose requests bring few tokens: `out`, and the keys' weights."""
+    lib = _lib("attention_prefix")
+    scratch = qkv.new_empty(2 * _few_mass_floats(tokens, seqs, *sizes, max_q_len, max_kv_len))            # bfloat16
+    if bounds_checked:
+        _set_bounds("attention_prefix", keys)
+    _check(lib, lib.pae_paged_attention_few_mass(
+        out.data_ptr(), *operands, mass.data_ptr(), pages, block_table.data_ptr(), table_width, q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(),
+        _ptr(slots), tokens, seqs, *sizes, max_q_len, max_kv_len, scale, keep_first, scratch.data_ptr(), _error_flag(qkv.device).data_ptr(), _stream()), 2)
+
+
 @functools.lru_cache(maxsize=64)
 def _mass_supports(*sizes) -> bool:
     return bool(_lib("attention_mma").pae_attention_mma_supports(*sizes))
@@ -2562,13 +2590,17 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
     if singles < 0 and tokens > (seqs - 1) * max_q_len + 1:
         singles = 0                                       # a request of one token would leave more to the others than they can bring
     sizes = (num_heads, num_kv_heads, head_dim, page_size)
-    if max_kv_len > 0 and max_q_len > 0 and qkv.dtype is torch.bfloat16 and use_tensor_cores and _mass_supports(*sizes):
-        prompt = _lib("attention_mass_prompt") if max_q_len > 1 else None
-        if prompt is None or (use_tcgen05_attention and prompt.pae_attention_mass_prompt_supports(*sizes)):
+    if max_kv_len > 0 and qkv.dtype is torch.bfloat16 and use_tensor_cores and max_q_len > 0:
+        few = 1 < max_q_len <= MASS_FEW_TOKENS and _prefix_supports(*sizes)
+        if few or (_mass_supports(*sizes) and (max_q_len == 1 or (use_tcgen05_attention and _prompt_mass_supports(*sizes)))):
             out = qkv.new_empty((tokens, num_heads * head_dim))
-            if prompt is not None:
-                _prompt_mass(prompt, out, qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, slots, sizes, max_q_len, max_kv_len, scale, keep_first,
-                             singles, multi_index)
+            if few:
+                _few_mass(out, qkv, keys, operands, mass, pages, block_table, table_width, q_start, q_pos0, kv_len, slots, tokens, seqs, sizes, max_q_len,
+                          max_kv_len, scale, keep_first)
+                return out
+            if max_q_len > 1:
+                _prompt_mass(_lib("attention_mass_prompt"), out, qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, slots, sizes, max_q_len, max_kv_len,
+                             scale, keep_first, singles, multi_index)
             if singles != 0:
                 _decode_mass(out, qkv, keys, operands, mass, block_table, table_width, q_start, kv_len, slots, seqs, sizes, max_kv_len, scale, keep_first,
                              seqs if singles < 0 else singles)

@@ -134,3 +134,13 @@ def test_a_mixed_step_as_the_engine_describes_it(ops):
     _check(step, *_run(ops, step, num_single=2, multi_index=i32([1, 3], "cuda")))
     step = Step([300, 500], [64, 130], 12, 2, 128, 16, BF16, 9)
     _check(step, *_run(ops, step, num_single=0))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(28, 4, 128, 16), (12, 2, 64, 128), (40, 2, 128, 32), (8, 8, 64, 64)])
+@pytest.mark.parametrize("lengths,tokens", [([900, 33, 2000, 5, 64], [5, 5, 5, 5, 5]), ([700, 300, 17], [16, 1, 9]), ([3, 2], [3, 2]), ([128, 4000], [2, 2])])
+def test_few_tokens(ops, heads, kv_heads, dim, page, lengths, tokens):
+    """Drafted tokens: slices of the keys that keep their scores."""
+    step = Step(lengths, tokens, heads, kv_heads, dim, page, BF16, heads + sum(tokens))
+    for keep_first in (0, 50):
+        _check(step, *_run(ops, step, keep_first), keep_first)
+    ops.check_device_errors()
