@@ -15,9 +15,9 @@
 //   slices, merge   the same on CUDA cores for single tokens of any other type and head size that is a multiple of 4 up to 256 (up to 16 query
 //                   heads a kv head): a block takes 64 keys a tile, one thread per key and half of the rows for the scores, one per four channels and a share
 //                   of the keys for the output.
-//   stats, columns  every other step: the rows' maxima and sums over runs of keys, then per tile of keys the
-//                   weights of all rows that see it, from scores that are computed again. CUDA cores, any type and head size. (Portions in bfloat16 go
-//                   to attention_mass_prompt.cu where that takes their sizes.)
+//   stats, columns  every other step: the rows' maxima and sums over runs of keys, then per tile of keys and chunk of rows the
+//                   weights, from scores that are computed again, and the chunks' sums in their order. CUDA cores, any type and head size. (Steps of several tokens in
+//                   bfloat16 go to attention_prefix.cu and attention_mass_prompt.cu where those take their sizes.)
 #include "attention_mma.cuh"
 
 using namespace pae;
@@ -413,9 +413,8 @@ __global__ void __launch_bounds__(ANY_THREADS) any_merge_kernel(const AnyParams<
 // ---------------------------------------------------------------------------------------
 // every other step
 // ---------------------------------------------------------------------------------------
-constexpr int ROWS = 16;                 // (token, head) pairs a tile, four a warp
-constexpr int KEYS = 32;                 // keys a tile, one a lane
-constexpr int THREADS = 128;
+// Tiles of 16 rows (token, head of a kv head) x 64 keys; a thread has one key and eight of the rows.
+constexpr int ROWS = 16;
 constexpr int MOST_RUNS = 16;            // of keys, that a request's maxima and sums are taken over
 
 template <typename T>
@@ -426,33 +425,58 @@ struct RowParams {
   const int* q_pos0;
   float* part_max;              // [runs, tokens * heads], in units of log2
   float* part_sum;
-  int d, runs, run_keys, row_tiles;
+  float* part;                  // [chunks, requests, kv_heads, span]
+  int d, runs, run_keys, row_tiles, chunk_tiles, span, seqs;
   long long rows;               // tokens * heads
   float scale_log2;
 };
 
-// A tile of rows, row r from row_ptr(r) (null: zeros), as float32 with `stride` floats a row.
+// Elements c .. c + 3 of a row of d: zeros behind the last. (Rows of a multiple of four start on a boundary of four: `vector`.)
+template <typename T>
+__device__ __forceinline__ float4 load4_of(const T* row, int c, int d, bool vector) {
+  if (vector) return load4(row + c);
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = c + i < d ? to_float<T>(row[c + i]) : 0.f;
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// Rows 0 .. rows - 1 of a tile, row r from row_ptr(r) (null: zeros), `stride` floats each.
 template <typename T, typename RowPtr>
-__device__ __forceinline__ void load_tile(float* tile, int rows, int d, int stride, RowPtr row_ptr) {
-  for (int r = threadIdx.x >> 5; r < rows; r += THREADS / 32) {
-    const T* from = row_ptr(r);
-    for (int i = threadIdx.x & 31; i < d; i += 32) tile[r * stride + i] = from != nullptr ? to_float<T>(from[i]) : 0.f;
+__device__ __forceinline__ void load_tile(float* tile, int rows, int d, int stride, bool vector, RowPtr row_ptr) {
+  const int units = (d + 3) / 4;
+  for (int i0 = threadIdx.x; i0 < rows * units; i0 += ANY_THREADS * AT_ONCE) {
+    float4 v[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = i0 + u * ANY_THREADS;
+      const T* from = i < rows * units ? row_ptr(i / units) : nullptr;
+      v[u] = from != nullptr ? load4_of<T>(from, (i % units) * 4, d, vector) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = i0 + u * ANY_THREADS;
+      if (i < rows * units) *(float4*)(tile + (i / units) * stride + (i % units) * 4) = v[u];
+    }
   }
 }
 
-// The scores of this thread's key (its lane) with the four rows of its warp, scaled, in units of log2.
-__device__ __forceinline__ void four_scores(float (&s)[4], const float* q_tile, const float* k_tile, int d, int stride, float scale_log2) {
-  const float* k = k_tile + (threadIdx.x & 31) * stride;
-  const float* q = q_tile + (threadIdx.x >> 5) * 4 * stride;
+// The scores of this thread's key with rows half, half + 2, ... of the tile, scaled, in units of log2.
+__device__ __forceinline__ void eight_scores(float (&s)[ROWS / 2], const float* q_tile, const float* k_tile, int d, int stride, float scale_log2) {
+  const float* k = k_tile + (threadIdx.x % ANY_KEYS) * stride;
+  const float* q = q_tile + (threadIdx.x / ANY_KEYS) * stride;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) s[i] = 0.f;
-  for (int c = 0; c < d; ++c) {
-    const float v = k[c];
+  for (int i = 0; i < ROWS / 2; ++i) s[i] = 0.f;
+  for (int c = 0; c < d; c += 4) {
+    const float4 kv = *(const float4*)(k + c);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = fmaf(q[i * stride + c], v, s[i]);
+    for (int i = 0; i < ROWS / 2; ++i) {
+      const float4 qv = *(const float4*)(q + 2 * i * stride + c);
+      s[i] = fmaf(kv.x, qv.x, fmaf(kv.y, qv.y, fmaf(kv.z, qv.z, fmaf(kv.w, qv.w, s[i]))));
+    }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) s[i] *= scale_log2;
+  for (int i = 0; i < ROWS / 2; ++i) s[i] *= scale_log2;
 }
 
 template <typename T>
@@ -460,113 +484,147 @@ __device__ __forceinline__ const T* key_row(const RowParams<T>& p, int b, int g,
   const int page = checked_page(p.m.block_table[(size_t)b * p.m.table_width + checked_table_index(j / p.m.page_size, p.m.table_width)]);
   return p.keys + (((size_t)page * p.m.kv_heads + g) * p.m.page_size + j % p.m.page_size) * p.d;
 }
+template <typename T>
+__device__ __forceinline__ const T* query_row(const RowParams<T>& p, int token0, int g, int groups, int i) {
+  return p.qkv + ((size_t)(token0 + i / groups) * (p.m.heads + 2 * p.m.kv_heads) + g * groups + i % groups) * p.d;
+}
+// How many keys some row of the tile that begins with row0 sees.
+__device__ __forceinline__ int seen_by(int row0, int count, int groups, int pos0, int n) { return min(n, pos0 + (min(row0 + ROWS, count) - 1) / groups + 1); }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) row_stats_kernel(const RowParams<T> p) {
-  extern __shared__ float shared[];
+__global__ void __launch_bounds__(ANY_THREADS) row_stats_kernel(const RowParams<T> p, bool vector) {
+  extern __shared__ __align__(16) float shared[];
+  __shared__ float tops[2][2][ROWS / 2], sums[2][2][ROWS / 2];       // [half of the keys][parity of the row][row / 2]
   dependent_launch_prologue();
   const int tile = blockIdx.x % p.row_tiles, run = blockIdx.x / p.row_tiles, g = blockIdx.y, b = blockIdx.z;
   const int groups = p.m.heads / p.m.kv_heads, token0 = p.m.q_start[b];
   const int count = (p.m.q_start[b + 1] - token0) * groups;
   const int row0 = tile * ROWS;
   if (row0 >= count || pads(p.m, token0)) return;
-  const int pos0 = p.q_pos0[b], n = p.m.kv_len[b];
-  const int visible = min(n, pos0 + (min(row0 + ROWS, count) - 1) / groups + 1);        // keys that some row of the tile sees
+  const int pos0 = p.q_pos0[b], visible = seen_by(row0, count, groups, pos0, p.m.kv_len[b]);
   const int begin = run * p.run_keys, end = min(visible, begin + p.run_keys);
-  const int stride = p.d + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stride = (p.d + 3) / 4 * 4 + 4, key = threadIdx.x % ANY_KEYS, half = threadIdx.x / ANY_KEYS, lane = threadIdx.x & 31;
   float* q_tile = shared;
   float* k_tile = shared + ROWS * stride;
-  load_tile<T>(q_tile, ROWS, p.d, stride, [&](int r) -> const T* {
-    const int i = row0 + r;
-    return i < count ? p.qkv + (size_t)(token0 + i / groups) * (p.m.heads + 2 * p.m.kv_heads) * p.d + (size_t)(g * groups + i % groups) * p.d : nullptr;
-  });
-  float top[4], sum[4];
+  load_tile<T>(q_tile, ROWS, p.d, stride, vector, [&](int r) -> const T* { return row0 + r < count ? query_row(p, token0, g, groups, row0 + r) : nullptr; });
+  float top[ROWS / 2], sum[ROWS / 2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < ROWS / 2; ++i) {
     top[i] = -FLT_MAX;
     sum[i] = 0.f;
   }
-  for (int key0 = begin; key0 < end; key0 += KEYS) {
+  for (int key0 = begin; key0 < end; key0 += ANY_KEYS) {
     __syncthreads();
-    load_tile<T>(k_tile, KEYS, p.d, stride, [&](int r) -> const T* { return key0 + r < end ? key_row(p, b, g, key0 + r) : nullptr; });
+    load_tile<T>(k_tile, ANY_KEYS, p.d, stride, vector, [&](int r) -> const T* { return key0 + r < end ? key_row(p, b, g, key0 + r) : nullptr; });
     __syncthreads();
-    float s[4];
-    four_scores(s, q_tile, k_tile, p.d, stride, p.scale_log2);
-    const int j = key0 + lane;
+    float s[ROWS / 2];
+    eight_scores(s, q_tile, k_tile, p.d, stride, p.scale_log2);
+    const int j = key0 + key;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (j >= end || j > pos0 + (row0 + warp * 4 + i) / groups) continue;
+    for (int i = 0; i < ROWS / 2; ++i) {
+      if (j >= end || j > pos0 + (row0 + half + 2 * i) / groups) continue;
       const float higher = fmaxf(top[i], s[i]);
-      sum[i] = (top[i] == -FLT_MAX ? 0.f : sum[i] * exp2f(top[i] - higher)) + exp2f(s[i] - higher);
+      sum[i] = (top[i] == -FLT_MAX ? sum[i] : sum[i] * exp2f(top[i] - higher)) + exp2f(s[i] - higher);
       top[i] = higher;
     }
   }
+  const int part = key / 32;                 // this warp's half of the tile's keys
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < ROWS / 2; ++i) {
     float both = top[i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) both = fmaxf(both, __shfl_xor_sync(0xffffffffu, both, o));
-    const float total = warp_sum(top[i] == -FLT_MAX ? 0.f : sum[i] * exp2f(top[i] - both));
-    const int r = row0 + warp * 4 + i;
-    if (lane == 0 && r < count) {
-      const size_t at = (size_t)run * p.rows + (size_t)(token0 + r / groups) * p.m.heads + g * groups + r % groups;
-      p.part_max[at] = both;
-      p.part_sum[at] = total;
+    const float total = warp_sum(top[i] == -FLT_MAX ? sum[i] : sum[i] * exp2f(top[i] - both));
+    if (lane == 0) {
+      tops[part][half][i] = both;
+      sums[part][half][i] = total;
     }
+  }
+  __syncthreads();
+  const int r = threadIdx.x;
+  if (r < ROWS && row0 + r < count) {
+    const float a = tops[0][r & 1][r >> 1], c = tops[1][r & 1][r >> 1], both = fmaxf(a, c);
+    const float total = (a == -FLT_MAX ? sums[0][r & 1][r >> 1] : sums[0][r & 1][r >> 1] * exp2f(a - both)) +
+                        (c == -FLT_MAX ? sums[1][r & 1][r >> 1] : sums[1][r & 1][r >> 1] * exp2f(c - both));
+    const int i = row0 + r;
+    const size_t at = (size_t)run * p.rows + (size_t)(token0 + i / groups) * p.m.heads + g * groups + i % groups;
+    p.part_max[at] = both;
+    p.part_sum[at] = total;
   }
 }
 
+// Which row tiles a block of column_sums_kernel takes: those of its chunk that see its keys. Empty: first >= last.
+struct ChunkTiles {
+  int first, last, pos0, tokens, n;
+};
 template <typename T>
-__global__ void __launch_bounds__(THREADS) column_mass_kernel(const RowParams<T> p) {
-  extern __shared__ float shared[];
-  __shared__ float top_of[ROWS], inverse_of[ROWS], sums[THREADS / 32][KEYS];
-  dependent_launch_prologue();
-  const int g = blockIdx.y, b = blockIdx.z, key0 = blockIdx.x * KEYS;
+__device__ __forceinline__ ChunkTiles chunk_tiles(const RowParams<T>& p, int b, int key0, int chunk) {
+  ChunkTiles t;
   const int groups = p.m.heads / p.m.kv_heads, token0 = p.m.q_start[b];
-  const int tokens = p.m.q_start[b + 1] - token0, count = tokens * groups;
-  const int pos0 = p.q_pos0[b], n = min(p.m.kv_len[b], pos0 + tokens);
-  if (key0 >= n || key0 + KEYS <= p.m.keep_first || tokens < 1 || pads(p.m, token0)) return;
-  const int stride = p.d + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = key0 + lane;
+  t.tokens = p.m.q_start[b + 1] - token0;
+  t.pos0 = p.q_pos0[b];
+  t.n = min(p.m.kv_len[b], t.pos0 + t.tokens);
+  const int all = (t.tokens * groups + ROWS - 1) / ROWS;
+  t.first = max(chunk * p.chunk_tiles, max(0, key0 - t.pos0) * groups / ROWS);
+  t.last = min((chunk + 1) * p.chunk_tiles, all);
+  if (t.tokens < 1 || key0 >= t.n || key0 + ANY_KEYS <= p.m.keep_first || pads(p.m, token0)) t.last = t.first;
+  return t;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ANY_THREADS) column_sums_kernel(const RowParams<T> p, bool vector) {
+  extern __shared__ __align__(16) float shared[];
+  __shared__ float logarithm[ROWS], halves[ANY_KEYS];
+  dependent_launch_prologue();
+  const int g = blockIdx.y % p.m.kv_heads, chunk = blockIdx.y / p.m.kv_heads, b = blockIdx.z, key0 = blockIdx.x * ANY_KEYS;
+  const ChunkTiles tiles = chunk_tiles(p, b, key0, chunk);
+  if (tiles.first >= tiles.last) return;
+  const int groups = p.m.heads / p.m.kv_heads, token0 = p.m.q_start[b], count = tiles.tokens * groups;
+  const int stride = (p.d + 3) / 4 * 4 + 4, key = threadIdx.x % ANY_KEYS, half = threadIdx.x / ANY_KEYS, j = key0 + key;
   float* q_tile = shared;
   float* k_tile = shared + ROWS * stride;
-  load_tile<T>(k_tile, KEYS, p.d, stride, [&](int r) -> const T* { return key0 + r < n ? key_row(p, b, g, key0 + r) : nullptr; });
+  load_tile<T>(k_tile, ANY_KEYS, p.d, stride, vector, [&](int r) -> const T* { return key0 + r < tiles.n ? key_row(p, b, g, key0 + r) : nullptr; });
   float sum = 0.f;
-  const int first_row = max(0, key0 - pos0) * groups;            // rows before it see none of the tile
-  for (int row0 = first_row / ROWS * ROWS; row0 < count; row0 += ROWS) {
+  for (int tile = tiles.first; tile < tiles.last; ++tile) {
+    const int row0 = tile * ROWS;
     __syncthreads();
-    load_tile<T>(q_tile, ROWS, p.d, stride, [&](int r) -> const T* {
-      const int i = row0 + r;
-      return i < count ? p.qkv + (size_t)(token0 + i / groups) * (p.m.heads + 2 * p.m.kv_heads) * p.d + (size_t)(g * groups + i % groups) * p.d : nullptr;
-    });
+    load_tile<T>(q_tile, ROWS, p.d, stride, vector, [&](int r) -> const T* { return row0 + r < count ? query_row(p, token0, g, groups, row0 + r) : nullptr; });
     if (threadIdx.x < ROWS && row0 + (int)threadIdx.x < count) {
-      const int r = row0 + threadIdx.x;
-      const size_t at = (size_t)(token0 + r / groups) * p.m.heads + g * groups + r % groups;
-      // Only the runs that a row's tile reached left something.
-      const int visible = min(p.m.kv_len[b], pos0 + (min(row0 + ROWS, count) - 1) / groups + 1);
-      const int runs = min(p.runs, (visible + p.run_keys - 1) / p.run_keys);
+      const int i = row0 + threadIdx.x;
+      const size_t at = (size_t)(token0 + i / groups) * p.m.heads + g * groups + i % groups;
+      const int runs = min(p.runs, (seen_by(row0, count, groups, tiles.pos0, p.m.kv_len[b]) + p.run_keys - 1) / p.run_keys);      // only these left something
       float top = -FLT_MAX, total = 0.f;
       for (int k = 0; k < runs; ++k) top = fmaxf(top, p.part_max[(size_t)k * p.rows + at]);
       for (int k = 0; k < runs; ++k) total += p.part_sum[(size_t)k * p.rows + at] * exp2f(p.part_max[(size_t)k * p.rows + at] - top);
-      top_of[threadIdx.x] = top;
-      inverse_of[threadIdx.x] = total > 0.f ? 1.f / total : 0.f;
+      logarithm[threadIdx.x] = total == 0.f ? INFINITY : top + log2f(total);
     }
     __syncthreads();
-    float s[4];
-    four_scores(s, q_tile, k_tile, p.d, stride, p.scale_log2);
+    float s[ROWS / 2];
+    eight_scores(s, q_tile, k_tile, p.d, stride, p.scale_log2);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = row0 + warp * 4 + i;
-      if (r < count && j <= pos0 + r / groups) sum += exp2f(s[i] - top_of[warp * 4 + i]) * inverse_of[warp * 4 + i];
+    for (int i = 0; i < ROWS / 2; ++i) {
+      const int r = row0 + half + 2 * i;
+      if (r < count && j <= tiles.pos0 + r / groups) sum += exp2f(s[i] - logarithm[half + 2 * i]);
     }
   }
-  sums[warp][lane] = sum;
+  if (half == 1) halves[key] = sum;
   __syncthreads();
-  if (warp == 0 && j >= p.m.keep_first && j < n) {
-    float w = 0.f;
-#pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) w += sums[i][lane];
-    add_mass(p.m, b, g, j, j >= pos0, w);
+  if (half == 0 && j < p.span) p.part[(((size_t)chunk * p.seqs + b) * p.m.kv_heads + g) * p.span + j] = sum + halves[key];
+}
+
+// The chunks' sums in their order, into the mass.
+template <typename T>
+__global__ void __launch_bounds__(ANY_KEYS) add_chunks_kernel(const RowParams<T> p, int chunks) {
+  dependent_launch_prologue();
+  const int g = blockIdx.y, b = blockIdx.z, key0 = blockIdx.x * ANY_KEYS, j = key0 + threadIdx.x;
+  ChunkTiles tiles = chunk_tiles(p, b, key0, 0);
+  if (j < p.m.keep_first || j >= min(tiles.n, p.span) || tiles.tokens < 1 || pads(p.m, p.m.q_start[b])) return;
+  float w = 0.f;
+  for (int c = 0; c < chunks; ++c) {
+    tiles = chunk_tiles(p, b, key0, c);
+    if (tiles.first < tiles.last) w += p.part[(((size_t)c * p.seqs + b) * p.m.kv_heads + g) * p.span + j];
   }
+  add_mass(p.m, b, g, j, j >= tiles.pos0, w);
 }
 
 template <int D>
@@ -582,17 +640,41 @@ int launch_decode_mass(const DecodeParams& p, const MassParams& m, __nv_bfloat16
   return check_launch("paged_attention_mass");
 }
 
+// How a step's rows and keys are cut: the stats into runs of keys, the columns into chunks of rows, until some 600 blocks are there.
+struct RowCut {
+  int row_tiles, runs, run_keys, chunk_tiles, chunks;
+};
+RowCut cut_rows(int seqs, int heads, int kv_heads, int max_q_len, int max_kv_len) {
+  RowCut c;
+  const long long pairs = (long long)seqs * kv_heads;
+  const int key_tiles = (max_kv_len + ANY_KEYS - 1) / ANY_KEYS;
+  c.row_tiles = (int)(((long long)max_q_len * (heads / kv_heads) + ROWS - 1) / ROWS);
+  long long runs = 592 / (pairs * c.row_tiles), chunks = 592 / (pairs * key_tiles);
+  if (runs > MOST_RUNS) runs = MOST_RUNS;
+  if (runs > key_tiles) runs = key_tiles;
+  if (runs < 1) runs = 1;
+  c.run_keys = (int)((key_tiles + runs - 1) / runs) * ANY_KEYS;
+  c.runs = (max_kv_len + c.run_keys - 1) / c.run_keys;
+  if (chunks > (c.row_tiles + 1) / 2) chunks = (c.row_tiles + 1) / 2;
+  if (chunks < 1) chunks = 1;
+  c.chunk_tiles = (int)((c.row_tiles + chunks - 1) / chunks);
+  c.chunks = (c.row_tiles + c.chunk_tiles - 1) / c.chunk_tiles;
+  return c;
+}
+
 template <typename T>
-int launch_rows(RowParams<T> p, const void* qkv, const void* keys, int seqs, int max_q_len, int max_kv_len, cudaStream_t s) {
-  p.qkv = (const T*)qkv;
-  p.keys = (const T*)keys;
-  const size_t stats_bytes = (size_t)(ROWS + KEYS) * (p.d + 1) * sizeof(float);
+int launch_rows(RowParams<T> p, const RowCut& c, int max_kv_len, cudaStream_t s) {
+  const size_t bytes = (size_t)(ROWS + ANY_KEYS) * ((p.d + 3) / 4 * 4 + 4) * sizeof(float);
+  const bool vector = p.d % 4 == 0 && (((uintptr_t)p.qkv | (uintptr_t)p.keys) & (4 * sizeof(T) - 1)) == 0;
   static DevicesSet stats_devices, column_devices;
   if (int err = raise_shared_memory(stats_devices, row_stats_kernel<T>, 200 * 1024, "attention_mass")) return err;
-  if (int err = raise_shared_memory(column_devices, column_mass_kernel<T>, 200 * 1024, "attention_mass")) return err;
-  launch_kernel(row_stats_kernel<T>, dim3(p.row_tiles * p.runs, p.m.kv_heads, seqs), dim3(THREADS), stats_bytes, s, p);
+  if (int err = raise_shared_memory(column_devices, column_sums_kernel<T>, 200 * 1024, "attention_mass")) return err;
+  const int key_tiles = (max_kv_len + ANY_KEYS - 1) / ANY_KEYS;
+  launch_kernel(row_stats_kernel<T>, dim3(c.row_tiles * c.runs, p.m.kv_heads, p.seqs), dim3(ANY_THREADS), bytes, s, p, vector);
   if (int err = check_launch("attention_mass")) return err;
-  launch_kernel(column_mass_kernel<T>, dim3((max_kv_len + KEYS - 1) / KEYS, p.m.kv_heads, seqs), dim3(THREADS), stats_bytes, s, p);
+  launch_kernel(column_sums_kernel<T>, dim3(key_tiles, p.m.kv_heads * c.chunks, p.seqs), dim3(ANY_THREADS), bytes, s, p, vector);
+  if (int err = check_launch("attention_mass")) return err;
+  launch_kernel(add_chunks_kernel<T>, dim3(key_tiles, p.m.kv_heads, p.seqs), dim3(ANY_KEYS), 0, s, p, c.chunks);
   return check_launch("attention_mass");
 }
 
@@ -608,13 +690,6 @@ int launch_any(AnyParams<T> p, int seqs, cudaStream_t s) {
   const int chunks = (p.span + MASS_CHUNK - 1) / MASS_CHUNK;
   launch_kernel(any_merge_kernel<T>, dim3(p.m.heads + p.m.kv_heads * chunks, seqs), dim3(ANY_THREADS), 0, s, p, chunks);
   return check_launch("paged_attention_mass");
-}
-
-int runs_of(int tokens_rows_tiles, int kv_heads, int seqs, int max_kv_len) {
-  const long long blocks = (long long)tokens_rows_tiles * kv_heads * seqs;
-  int runs = 1;
-  while (runs < MOST_RUNS && blocks * runs < 4 * 148 && max_kv_len > runs * 4 * KEYS) runs *= 2;
-  return runs;
 }
 
 }  // namespace
@@ -692,24 +767,29 @@ PAE_EXPORT int pae_paged_attention_any_mass(void* out, const void* qkv, const vo
 }
 
 // Floats of scratch for pae_attention_mass_rows.
-PAE_EXPORT long long pae_attention_mass_floats(int tokens, int heads) { return 2ll * MOST_RUNS * tokens * heads; }
+PAE_EXPORT long long pae_attention_mass_floats(int tokens, int seqs, int heads, int kv_heads, int max_q_len, int max_kv_len) {
+  if (seqs < 1 || max_q_len < 1 || max_kv_len < 1) return 1;
+  return 2ll * MOST_RUNS * tokens * heads + (long long)cut_rows(seqs, heads, kv_heads, max_q_len, max_kv_len).chunks * seqs * kv_heads * max_kv_len;
+}
 
 // The weights of any step's keys, whatever its rows, type (0 float32, 1 bfloat16) and head size; the attention's output is not computed.
 PAE_EXPORT int pae_attention_mass_rows(float* mass, const void* qkv, const void* keys, const int* block_table, int table_width, const int* q_start,
                                        const int* q_pos0, const int* kv_len, const int* slots, int tokens, int seqs, int max_q_len, int max_kv_len, int heads,
                                        int kv_heads, int d, int page_size, float scale, int keep_first, int dtype, float* scratch, void* stream) {
-  if (seqs == 0 || max_kv_len < 1) return 0;
-  if (kv_heads > 65535 || seqs > 65535) return fail(1, "paged_attention_mass: %d requests of %d kv heads, at most 65535 of each", seqs, kv_heads);
-  if (d < 1 || d > 1024) return fail(2, "paged_attention_mass: head_dim %d is not 1 to 1024", d);
+  if (seqs < 1 || tokens < 1 || max_q_len < 1 || max_kv_len < 1) return 0;
+  if (d < 1 || d > 512) return fail(2, "paged_attention_mass: head_dim %d is not 1 to 512", d);
+  const RowCut c = cut_rows(seqs, heads, kv_heads, max_q_len, max_kv_len);
+  if ((long long)kv_heads * c.chunks > 65535 || seqs > 65535 || (long long)c.row_tiles * c.runs > 0x7fffffffll)
+    return fail(1, "paged_attention_mass: %d requests of %d kv heads x %d chunks exceed one launch", seqs, kv_heads, c.chunks);
   const MassParams m = {mass, block_table, q_start, kv_len, slots, table_width, heads, kv_heads, page_size, keep_first};
-  const int groups = heads / kv_heads, row_tiles = (int)(((long long)max_q_len * groups + ROWS - 1) / ROWS);
-  const int runs = runs_of(row_tiles, kv_heads, seqs, max_kv_len);
-  const int run_keys = ((max_kv_len + runs - 1) / runs + KEYS - 1) / KEYS * KEYS;
   const long long rows = (long long)tokens * heads;
-  float* part_max = scratch;
   float* part_sum = scratch + (long long)MOST_RUNS * rows;
+  float* part = part_sum + (long long)MOST_RUNS * rows;
   const float scale_log2 = scale * LOG2E;
   const cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == kF32) return launch_rows<float>({m, nullptr, nullptr, q_pos0, part_max, part_sum, d, runs, run_keys, row_tiles, rows, scale_log2}, qkv, keys, seqs, max_q_len, max_kv_len, s);
-  return launch_rows<__nv_bfloat16>({m, nullptr, nullptr, q_pos0, part_max, part_sum, d, runs, run_keys, row_tiles, rows, scale_log2}, qkv, keys, seqs, max_q_len, max_kv_len, s);
+  if (dtype == kF32)
+    return launch_rows<float>({m, (const float*)qkv, (const float*)keys, q_pos0, scratch, part_sum, part, d, c.runs, c.run_keys, c.row_tiles, c.chunk_tiles, max_kv_len, seqs,
+                               rows, scale_log2}, c, max_kv_len, s);
+  return launch_rows<__nv_bfloat16>({m, (const __nv_bfloat16*)qkv, (const __nv_bfloat16*)keys, q_pos0, scratch, part_sum, part, d, c.runs, c.run_keys, c.row_tiles,
+                                     c.chunk_tiles, max_kv_len, seqs, rows, scale_log2}, c, max_kv_len, s);
 }

@@ -2621,7 +2621,7 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
     out = paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_kv_len, scale,
                           0, num_single=num_single, multi_index=multi_index)
     lib = _lib("attention_mass")
-    scratch = torch.empty(lib.pae_attention_mass_floats(tokens, num_heads), dtype=torch.float32, device=qkv.device)
+    scratch = torch.empty(lib.pae_attention_mass_floats(tokens, seqs, num_heads, num_kv_heads, max_q_len, max_kv_len), dtype=torch.float32, device=qkv.device)
     _set_bounds("attention_mass", keys)
     _check(lib, lib.pae_attention_mass_rows(
         mass.data_ptr(), qkv.data_ptr(), keys.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(),
