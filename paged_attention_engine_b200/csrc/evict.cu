@@ -272,11 +272,10 @@ struct CompactParams {
   int table_width, kv_heads, page_size, budget;
 };
 
-// Where a chunk's rows come from and go to, as row numbers of the pool (pages * kv_heads * page_size of them, fewer than 2^32 - 1), found by one
-// thread a row while the chunk before is on its way; STAYS: the row does not move.
-constexpr uint32_t STAYS = 0xFFFFFFFFu;
+// Where a chunk's rows come from and go to, as row numbers of the pool (pages * kv_heads * page_size of them, fewer than 2^31), found by one thread
+// a row while the chunk before is on its way; -1: the row does not move. (With unsigned numbers and another mark, the kernel of 1,024 threads took a tenth more.)
 template <int THREADS, typename Unit>
-__device__ __forceinline__ void compact_strip(const CompactParams& p, int pool, int strip, uint2 (*moves)[MOST_ROWS]) {
+__device__ __forceinline__ void compact_strip(const CompactParams& p, int pool, int strip, int2 (*moves)[MOST_ROWS]) {
   const int g = blockIdx.y, b = blockIdx.z;
   const int n = min(p.kv_len[b], p.table_width * p.page_size);
   const int places = min(n, p.budget);
@@ -288,13 +287,13 @@ __device__ __forceinline__ void compact_strip(const CompactParams& p, int pool, 
   Unit* base = (Unit*)p.pools[pool] + my_unit;
   auto row_of = [&](int i) {
     const int page = page_or_none(table, i / p.page_size, p.table_width);
-    return page < 0 ? STAYS : ((uint32_t)page * p.kv_heads + g) * p.page_size + i % p.page_size;
+    return page < 0 ? -1 : (page * p.kv_heads + g) * p.page_size + i % p.page_size;
   };
-  auto find = [&](int chunk, uint2* to) {
+  auto find = [&](int chunk, int2* to) {
     for (int r = threadIdx.x; r < chunk_rows; r += THREADS) {
       const int i = chunk + r, from = i < places ? kept[i] : -1;
-      uint2 move = from > i && from < n ? make_uint2(row_of(from), row_of(i)) : make_uint2(STAYS, STAYS);
-      if (move.y == STAYS) move.x = STAYS;
+      int2 move = from > i && from < n ? make_int2(row_of(from), row_of(i)) : make_int2(-1, 0);
+      if (move.y < 0) move.x = -1;
       to[r] = move;
     }
   };
@@ -302,18 +301,18 @@ __device__ __forceinline__ void compact_strip(const CompactParams& p, int pool, 
   __syncthreads();
   for (int chunk = 0, turn = 0; chunk < places; chunk += chunk_rows, turn ^= 1) {
     Unit held[IN_FLIGHT];
-    uint32_t to[IN_FLIGHT];
+    int to[IN_FLIGHT];
 #pragma unroll
     for (int u = 0; u < IN_FLIGHT; ++u) {
-      const uint2 move = my_row < rows_a_pass ? moves[turn][u * rows_a_pass + my_row] : make_uint2(STAYS, STAYS);
-      to[u] = move.x != STAYS ? move.y : STAYS;
-      if (move.x != STAYS) held[u] = base[(size_t)move.x * units];
+      const int2 move = my_row < rows_a_pass ? moves[turn][u * rows_a_pass + my_row] : make_int2(-1, 0);
+      to[u] = move.x >= 0 ? move.y : -1;
+      if (move.x >= 0) held[u] = base[(size_t)move.x * units];
     }
     if (chunk + chunk_rows < places) find(chunk + chunk_rows, moves[turn ^ 1]);
     __syncthreads();                       // the whole chunk is read, and the next one's rows are found
 #pragma unroll
     for (int u = 0; u < IN_FLIGHT; ++u)
-      if (to[u] != STAYS) base[(size_t)to[u] * units] = held[u];
+      if (to[u] >= 0) base[(size_t)to[u] * units] = held[u];
   }
 }
 
@@ -322,7 +321,7 @@ __global__ void __launch_bounds__(THREADS) compact_kernel(const CompactParams p)
   // The next kernel is not let go early: an attention that follows directly fetches keys of earlier tokens before it waits for
   // the kernel before it (common.cuh), and those are what is written here.
   dependent_launch_wait();
-  __shared__ uint2 moves[2][MOST_ROWS];
+  __shared__ int2 moves[2][MOST_ROWS];
   int strip = blockIdx.x;
   if (strip < p.strips[0]) {
     compact_strip<THREADS, Unit>(p, 0, strip, moves);

@@ -2667,8 +2667,8 @@ def compact_kept(keys, values, mass, block_table, kv_len, kept) -> None:
     if keys.dim() != 4:
         raise KernelError(f"compact_kept: keys {tuple(keys.shape)}, [pages, kv_heads, page_size, head size] is needed")
     pages, kv_heads, page_size, key_dim = keys.shape
-    if pages * kv_heads * page_size >= 0xFFFFFFFF:
-        raise KernelError(f"compact_kept: a pool of {pages * kv_heads * page_size} rows, fewer than 2^32 - 1 are taken")
+    if pages * kv_heads * page_size >= 1 << 31:
+        raise KernelError(f"compact_kept: a pool of {pages * kv_heads * page_size} rows, fewer than 2^31 are taken")
     if kept.dim() != 3 or kept.shape[0] != seqs or kept.shape[1] != kv_heads:
         raise KernelError(f"compact_kept: kept {tuple(kept.shape)} for {seqs} requests of {kv_heads} kv heads")
     names, given = ["keys", "block_table", "kv_len", "kept"], [keys, block_table, kv_len, kept]

@@ -35,7 +35,7 @@ def _compact(keys=None, values=None, mass=None, block_table=None, kv_len=None, k
     (dict(keys=torch.zeros(9, 2, 16)), "head size\\] is needed"), (dict(kept=_i32(3, 2, 5).long()), "kept is torch.int64"), (dict(kept=_i32(3, 1, 5)), "kept \\(3, 1, 5\\) for 3 requests of 2 kv heads"),
     (dict(kept=_i32(2, 2, 5)), "kept \\(2, 2, 5\\)"), (dict(values=torch.zeros(9, 2, 8, 8)), "beside keys"), (dict(values=torch.zeros(9, 2, 16, 8, dtype=torch.bfloat16)), "beside keys"),
     (dict(mass=torch.zeros(9, 2, 16, 8)), "mass torch.float32"), (dict(mass=torch.zeros(9, 2, 16, dtype=torch.float64)), "mass torch.float64"),
-    (dict(kv_len=_i32(2)), "block tables"), (dict(), "keys is not on a CUDA device")])
+    (dict(kv_len=_i32(2)), "block tables"), (dict(keys=torch.zeros(1).expand(1 << 20, 2, 1024, 8)), "a pool of 2147483648 rows"), (dict(), "keys is not on a CUDA device")])
 def test_compaction_refuses(arguments, message):
     with pytest.raises(ops.KernelError, match=message):
         _compact(**arguments)
