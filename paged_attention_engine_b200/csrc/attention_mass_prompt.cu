@@ -381,7 +381,7 @@ PAE_EXPORT int pae_attention_mass_prompt(float* mass, const void* qkv, const voi
   p.scale_log2 = scale * LOG2E;
   p.error = error;
   const int chunks = chunk_count(seqs, kv_heads, max_q_len, max_kv_len, p.tile_tokens);
-  if (seqs > 65535 || (long long)kv_heads * chunks > 65535) return fail(3, "attention_mass: %d requests, %d kv heads x %d chunks exceed one launch", seqs, kv_heads, chunks);
+  if ((long long)kv_heads * seqs > 65535 || chunks > 65535) return fail(3, "attention_mass: %d requests of %d kv heads, %d chunks exceed one launch", seqs, kv_heads, chunks);
   if (d == 64) return launch<64>(p, qkv, keys, pages, tokens, chunks, (cudaStream_t)stream);
   return launch<128>(p, qkv, keys, pages, tokens, chunks, (cudaStream_t)stream);
 }

@@ -2428,6 +2428,8 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
         raise KernelError(f"{what}: {max_prefix_len} shared and {max_own_len} own keys for tables of {table_width} pages of {page_size}")
     if not 0 <= max_q_len <= max_group_tokens:
         raise KernelError(f"{what}: requests of up to {max_q_len} tokens in groups of up to {max_group_tokens}")
+    if not scale >= 0:
+        raise KernelError(f"{what}: scores scaled by {scale}")
     if max_group_tokens > tokens:
         max_q_len, max_group_tokens = min(max_q_len, tokens), tokens
     _here(what, _PREFIX_TENSORS, qkv, keys, values, block_table, q_start, q_pos0, kv_len, prefix_len, group_start)
@@ -2576,6 +2578,8 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
         raise KernelError(f"paged_attention_mass: mass {mass.dtype} {tuple(mass.shape)} beside keys {tuple(keys.shape)}")
     if keep_first < 0:
         raise KernelError(f"paged_attention_mass: {keep_first} first keys")
+    if not scale >= 0:
+        raise KernelError(f"paged_attention_mass: scores scaled by {scale}")
     if not 0 <= max_kv_len <= table_width * page_size:
         raise KernelError(f"paged_attention_mass: {max_kv_len} keys for tables of {table_width} pages of {page_size}")
     if slots is not None:
@@ -2584,8 +2588,8 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
             raise KernelError(f"paged_attention_mass: slots {tuple(slots.shape)} for {tokens} tokens")
     _here(what, _MASS_TENSORS, qkv, keys, values, block_table, q_start, q_pos0, kv_len, mass, *(() if slots is None else (slots,)))
     operands = _aligned_operands(what, qkv, keys, values, head_dim)
-    if tokens == 0:
-        return qkv.new_empty((0, num_heads * head_dim))
+    if tokens == 0 or seqs == 0:
+        return qkv.new_empty((tokens, num_heads * head_dim))
     singles = num_single if num_single is not None else (seqs if max_q_len == 1 else -1)
     if singles < 0 and tokens > (seqs - 1) * max_q_len + 1:
         singles = 0                                       # a request of one token would leave more to the others than they can bring
@@ -2684,10 +2688,12 @@ def compact_kept(keys, values, mass, block_table, kv_len, kept) -> None:
             raise KernelError(f"compact_kept: mass {mass.dtype} {tuple(mass.shape)} beside keys {tuple(keys.shape)}")
         names.append("mass")
         given.append(mass)
-    _here("compact_kept", names, *given)
     size = keys.element_size()
     key_bytes, value_bytes = key_dim * size, 0 if values is None else values.shape[3] * size
     together = key_bytes | value_bytes | keys.data_ptr() | (0 if values is None else values.data_ptr())
+    if together & 1:
+        raise KernelError(f"compact_kept: rows of {key_bytes} and {value_bytes} bytes, whole pieces of two bytes are moved")
+    _here("compact_kept", names, *given)
     unit = 16 if together % 16 == 0 else 4 if together % 4 == 0 else 2
     lib = _lib("evict")
     if bounds_checked:

@@ -144,3 +144,23 @@ def test_few_tokens(ops, heads, kv_heads, dim, page, lengths, tokens):
     for keep_first in (0, 50):
         _check(step, *_run(ops, step, keep_first), keep_first)
     ops.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(BF16, 128, 16), (BF16, 64, 64), (F32, 64, 16)])
+@pytest.mark.parametrize("tokens,max_q_len", [(1, 1), (3, 3), (90, 90)])
+def test_requests_without_keys(ops, dtype, dim, page, tokens, max_q_len):
+    """Steps that padding alone makes up, and a step without requests: rows without a key are zeros, no weight changes."""
+    step = Step([70, 100], [1, 1], 12, 2, dim, page, dtype, 3)
+    pools, (table, *_) = step.on()
+    qkv = torch.randn(2 * tokens, 16 * dim, device="cuda").to(dtype)
+    mass = step.mass.cuda()
+    zeros = i32([0, 0], "cuda")
+    for longest in (0, 64):
+        for slots in (None, torch.full((2 * tokens,), -1, dtype=torch.int32, device="cuda")):
+            out = ops.paged_attention_mass(qkv, pools[1], pools[2], mass, table, i32([0, tokens, 2 * tokens], "cuda"), zeros, zeros, *step.sizes, max_q_len, longest, step.scale,
+                                           slots=slots)
+            assert torch.equal(out, torch.zeros_like(out))
+    assert ops.paged_attention_mass(qkv, pools[1], pools[2], mass, table[:0], i32([0], "cuda"), zeros[:0], zeros[:0], *step.sizes, max_q_len, 64, step.scale).shape == (2 * tokens, 12 * dim)
+    assert torch.equal(mass.cpu(), step.mass)
+    assert torch.equal(ops.choose_kept(mass, table, zeros, 5, 1, 1, 64), torch.full((2, 2, 5), -1, dtype=torch.int32, device="cuda"))
+    ops.check_device_errors()

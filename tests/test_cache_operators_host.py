@@ -35,7 +35,9 @@ def _compact(keys=None, values=None, mass=None, block_table=None, kv_len=None, k
     (dict(keys=torch.zeros(9, 2, 16)), "head size\\] is needed"), (dict(kept=_i32(3, 2, 5).long()), "kept is torch.int64"), (dict(kept=_i32(3, 1, 5)), "kept \\(3, 1, 5\\) for 3 requests of 2 kv heads"),
     (dict(kept=_i32(2, 2, 5)), "kept \\(2, 2, 5\\)"), (dict(values=torch.zeros(9, 2, 8, 8)), "beside keys"), (dict(values=torch.zeros(9, 2, 16, 8, dtype=torch.bfloat16)), "beside keys"),
     (dict(mass=torch.zeros(9, 2, 16, 8)), "mass torch.float32"), (dict(mass=torch.zeros(9, 2, 16, dtype=torch.float64)), "mass torch.float64"),
-    (dict(kv_len=_i32(2)), "block tables"), (dict(keys=torch.zeros(1).expand(1 << 20, 2, 1024, 8)), "a pool of 2147483648 rows"), (dict(), "keys is not on a CUDA device")])
+    (dict(kv_len=_i32(2)), "block tables"), (dict(keys=torch.zeros(1).expand(1 << 20, 2, 1024, 8)), "a pool of 2147483648 rows"),
+    (dict(keys=torch.zeros(9, 2, 16, 5, dtype=torch.uint8)), "rows of 5 and 0 bytes"),
+    (dict(keys=torch.zeros(9, 2, 16, 4, dtype=torch.uint8), values=torch.zeros(9, 2, 16, 3, dtype=torch.uint8)), "rows of 4 and 3 bytes"), (dict(), "keys is not on a CUDA device")])
 def test_compaction_refuses(arguments, message):
     with pytest.raises(ops.KernelError, match=message):
         _compact(**arguments)
@@ -63,7 +65,7 @@ STEP_REFUSALS = [
 
 @pytest.mark.parametrize("arguments,message", STEP_REFUSALS + [
     (dict(mass=torch.zeros(9, KV_HEADS, PAGE, dtype=torch.bfloat16)), "mass torch.bfloat16"), (dict(mass=torch.zeros(9, KV_HEADS, 8)), "mass torch.float32 \\(9, 2, 8\\)"),
-    (dict(keep_first=-1), "-1 first keys"), (dict(max_kv_len=65), "65 keys"), (dict(slots=_i32(4)), "slots \\(4,\\) for 5 tokens"), (dict(slots=_i32(5).long()), "slots is torch.int64")])
+    (dict(scale=-0.5), "scaled by -0.5"), (dict(scale=float("nan")), "scaled by nan"), (dict(keep_first=-1), "-1 first keys"), (dict(max_kv_len=65), "65 keys"), (dict(slots=_i32(4)), "slots \\(4,\\) for 5 tokens"), (dict(slots=_i32(5).long()), "slots is torch.int64")])
 def test_mass_refuses(arguments, message):
     a = dict(mass=torch.zeros(9, KV_HEADS, PAGE), num_heads=HEADS, num_kv_heads=KV_HEADS, head_dim=DIM, page_size=PAGE, max_q_len=3, max_kv_len=64, scale=1.0)
     a.update(_attention(**arguments))
@@ -75,7 +77,7 @@ def test_mass_refuses(arguments, message):
 @pytest.mark.parametrize("arguments,message", STEP_REFUSALS + [
     (dict(prefix_len=_i32(2)), "prefix_len \\(2,\\)"), (dict(prefix_len=_i32(3).long()), "prefix_len is torch.int64"), (dict(group_start=_i32(1)), "group_start \\(1,\\)"),
     (dict(group_start=_i32(5)), "group_start \\(5,\\)"), (dict(group_start=torch.zeros(3)), "group_start is torch.float32"), (dict(max_prefix_len=-1), "-1 shared"),
-    (dict(max_own_len=-1), "-1 own keys"), (dict(max_prefix_len=65), "65 shared"), (dict(max_q_len=4), "up to 4 tokens in groups of up to 3")])
+    (dict(scale=-0.5), "scaled by -0.5"), (dict(scale=float("nan")), "scaled by nan"), (dict(max_own_len=-1), "-1 own keys"), (dict(max_prefix_len=65), "65 shared"), (dict(max_q_len=4), "up to 4 tokens in groups of up to 3")])
 def test_prefix_refuses(arguments, message):
     a = dict(prefix_len=_i32(3), group_start=_i32(3), num_heads=HEADS, num_kv_heads=KV_HEADS, head_dim=DIM, page_size=PAGE, max_q_len=2, max_prefix_len=20, max_own_len=30,
              max_group_tokens=3, scale=1.0)
