@@ -868,7 +868,9 @@ struct Cut {
 // that share of one wave that their tiles are of all tiles (a request's own keys taken as half of the longest's), half of it at least: what is left
 // goes to the own blocks, which wait for memory while the others compute. 64 requests, 8,000 shared and 20 to 700 own keys, 28 heads over 4 of
 // 128, us with the merge: 37.6 with the wave full of shared blocks, 36.2 with three quarters, 33.5 with half; 24 requests of five
-// tokens, 30,011 shared and 100 to 900 own keys, 40 heads over 8: 94.8, 112 and 154.
+// tokens, 30,011 shared and 100 to 900 own keys, 40 heads over 8: 94.8, 112 and 154. With 4 and 32 tiles at most in place of 12: the former 39.2 and
+// 35.1 (35.1), with 3,000 to 5,000 own keys 153 and 104 (110); the latter 100.4 and 95.8 (97.1); the weights of 48 requests of five tokens over 300 to
+// 6,000 keys, 28 heads over 4, whose slices follow the same rule, 192 and 164 (154).
 constexpr int OWN_TILES = 12;
 Cut cut_keys(int seqs, int groups, int heads, int kv_heads, int box, int max_q_len, int max_prefix, int max_own, int max_group_tokens, bool any) {
   const int share = heads / kv_heads, wave = (any ? 3 : 2) * pae_attention::multiprocessors(), rows = any ? ANY_ROWS : ROWS;
@@ -909,6 +911,8 @@ int launch(const Params& p, void* out, long long pages, int blocks, int seqs, in
   if (int err = raise_shared_memory(devices, prefix_kernel<D, false>, Layout<D>::SMEM_BYTES, "paged_attention_prefix")) return err;
   launch_kernel(prefix_kernel<D, false>, dim3(blocks), dim3(THREADS), Layout<D>::SMEM_BYTES, s, maps, p);
   if (int err = check_launch("paged_attention_prefix")) return err;
+  // A warp a row where the rows fill the SMs with warps, a block a row below that. 12 heads of 4 requests 8.3 us a pass with warps and 7.7 with blocks,
+  // 28 heads of 64 35.1 and 35.7, 14 heads of 123 18.8 and 19.8; the rows of mass_merge_kernel, 28 heads of 48 requests of five tokens, 154 and 199.
   if ((long long)p.heads * max_q_len * seqs >= 8LL * pae_attention::multiprocessors()) {
     launch_kernel(prefix_merge_rows_kernel<D>, dim3((p.heads + 3) / 4, max_q_len, seqs), dim3(128), 0, s, (__nv_bfloat16*)out, p);
     return check_launch("paged_attention_prefix");

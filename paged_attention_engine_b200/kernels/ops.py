@@ -2372,9 +2372,11 @@ def _need_attention(what: str, qkv, keys, values, block_table, q_start, q_pos0, 
     raise KernelError(f"{what}: tensors of {qkv.dim()}, {keys.dim()} and {block_table.dim()} dimensions for qkv, keys and the block table")
 
 
-# From how many tokens a request on a step is an ordinary one: a query tile of one request fills the tensor cores then, and its keys are
-# read once for all of its tokens anyway.
-PREFIX_ATTENTION_MAX_TOKENS = 63
+# Up to how many tokens a request the shared keys are taken once for all; from there on a query tile of one request fills the tensor cores and its keys are
+# read once for all of its tokens anyway. us a pass, captured, shared and each request by itself: 24 requests behind 30,011 keys, 40 heads over 8 of 128, 48
+# tokens each 949 and 4,916, 64 1,060 and 2,006, 96 1,570 and 2,052, 128 2,063 and 2,032; 16 behind 8,000, 28 heads over 4, 48 145 and 854, 64 159 and 253,
+# 96 283 and 253.
+PREFIX_ATTENTION_MAX_TOKENS = 64
 # From how many shared keys on the CUDA-core kernel takes them once for all. us a pass, captured, shared and each request by itself, float32, 12 heads over 2 of 64:
 # 2 requests behind 200 keys 15 and 8, 16 behind 1,000 20.3 and 19.5, 64 behind 2,000 56 and 92, 4 behind 8,000 35 and 106; 32 of 28 heads over 4 of 128
 # behind 4,000 293 and 416.

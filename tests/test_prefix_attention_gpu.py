@@ -100,7 +100,7 @@ def test_maxima_that_grow_along_the_shared_keys(ops, dim, requests):
 
 
 def test_a_long_portion_and_a_lone_request_read_their_keys_themselves(ops):
-    step = _step(((2, 100),), [70, 5], [64, 1], 12, 2, 128, 16, BF16, 6)
+    step = _step(((2, 100),), [70, 5], [65, 1], 12, 2, 128, 16, BF16, 6)
     info = {}
     _check(step, _run(ops, step, info=info))
     assert info["kernel"] != "shared"
@@ -177,6 +177,15 @@ def test_a_step_without_tokens_and_operands_that_start_anywhere(ops):
     assert torch.equal(mass.cpu(), step.mass)
     with pytest.raises(ops.KernelError, match="values is not contiguous"):
         ops.paged_attention_mass(pools[0], pools[1], pools[2].transpose(0, 1).contiguous().transpose(0, 1), mass, *tables, *step.sizes, *step.longest, step.scale)
+
+
+@pytest.mark.parametrize("tokens", [16, 63, 64, 65])
+def test_up_to_64_tokens_a_request_share(ops, tokens):
+    step = _step(((3, 500), (2, 90)), [tokens + 9, 150, tokens, 130, 77], [tokens, 1, 5, tokens, 64], 12, 2, 128, 16, BF16, tokens)
+    info = {}
+    out = _run(ops, step, info=info)
+    assert info["kernel"] == ("shared" if max(step.tokens) <= 64 else "tcgen05")
+    _check(step, out)
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", [(12, 2, 64, 16, F32), (8, 2, 256, 16, F32), (5, 1, 20, 16, BF16), (3, 3, 4, 5, F32), (20, 1, 100, 48, BF16)])
