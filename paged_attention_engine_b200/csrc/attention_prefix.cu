@@ -535,35 +535,51 @@ __global__ void __launch_bounds__(pae_attention::MERGE_WARPS * 32) prefix_merge_
   pae_attention::merge_parts<D, DEPTH>(out + row * D, p.part_out + at * D, p.part_max + at, p.part_sum + at, slices, p.slots, weights);
 }
 
-// A row's merge by one warp.
-template <int D>
+template <int N>
+__device__ __forceinline__ void load_floats(float (&to)[N], const float* from) {       // of a boundary of N floats
+  if constexpr (N == 4) {
+    const float4 v = *(const float4*)from;
+    to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+  } else {
+    const float2 v = *(const float2*)from;
+    to[0] = v.x, to[1] = v.y;
+  }
+}
+
+// A row's merge by one warp. The first slices' outputs are asked for together with the maxima and sums that weigh them.
+template <int D, int DEPTH>
 __device__ __forceinline__ void merge_row(__nv_bfloat16* __restrict__ out, const Params& p, size_t at, int slices, int lane) {
-  constexpr int PER_LANE = D / 32, DEPTH = 8;
+  constexpr int PER_LANE = D / 32;
+  static_assert(32 % DEPTH == 0, "a lane holds the weight of one of 32 slices");
   const float* maxima = p.part_max + at;
-  float top = -FLT_MAX, total = 0.f;
-  for (int s = lane; s < slices; s += 32) top = fmaxf(top, maxima[s]);
+  const float* sums = p.part_sum + at;
+  const float* outputs = p.part_out + at * D + lane * PER_LANE;
+  const float my_max = lane < slices ? maxima[lane] : -FLT_MAX, my_sum = lane < slices ? sums[lane] : 0.f;
+  float part[DEPTH][PER_LANE];
+  auto ask = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u)
+      if (s0 + u < slices) load_floats(part[u], outputs + (size_t)(s0 + u) * D);
+  };
+  ask(0);
+  float top = my_max, total = 0.f;
+  for (int s = lane + 32; s < slices; s += 32) top = fmaxf(top, maxima[s]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  for (int s = lane; s < slices; s += 32) total += p.part_sum[at + s] * exp2f(maxima[s] - top);
+  if (lane < slices) total = my_sum * exp2f(my_max - top);
+  for (int s = lane + 32; s < slices; s += 32) total += sums[s] * exp2f(maxima[s] - top);
   total = warp_sum(total);
   float acc[PER_LANE];
 #pragma unroll
   for (int j = 0; j < PER_LANE; ++j) acc[j] = 0.f;
   for (int s0 = 0; s0 < slices; s0 += 32) {
-    const float weight = s0 + lane < slices ? exp2f(maxima[s0 + lane] - top) : 0.f;
-    const int count = min(32, slices - s0);
-    for (int k = 0; k < count; k += DEPTH) {
-      float part[DEPTH][PER_LANE];
+    const float weight = s0 + lane < slices ? exp2f((s0 == 0 ? my_max : maxima[s0 + lane]) - top) : 0.f;
+    for (int k = 0; k < min(32, slices - s0); k += DEPTH) {
+      if (s0 + k > 0) ask(s0 + k);
 #pragma unroll
       for (int u = 0; u < DEPTH; ++u) {
-        const float* from = p.part_out + (at + s0 + k + u) * D + lane * PER_LANE;
-#pragma unroll
-        for (int j = 0; j < PER_LANE; ++j) part[u][j] = k + u < count ? from[j] : 0.f;
-      }
-#pragma unroll
-      for (int u = 0; u < DEPTH; ++u) {
-        const float w = __shfl_sync(0xffffffffu, weight, (k + u) & 31);
-        if (k + u < count) {
+        const float w = __shfl_sync(0xffffffffu, weight, k + u);
+        if (s0 + k + u < slices) {
 #pragma unroll
           for (int j = 0; j < PER_LANE; ++j) acc[j] += part[u][j] * w;
         }
@@ -575,8 +591,8 @@ __device__ __forceinline__ void merge_row(__nv_bfloat16* __restrict__ out, const
   for (int j = 0; j < PER_LANE; j += 2) *(__nv_bfloat162*)(out + lane * PER_LANE + j) = __floats2bfloat162_rn(acc[j] * inv, acc[j + 1] * inv);
 }
 
-// The same by one warp a row, for launches of so many rows that warps are there for all SMs: every row is in flight at once.
-template <int D>
+// The same by one warp a row, for launches of so many rows that warps are there for all SMs.
+template <int D, int DEPTH>
 __global__ void __launch_bounds__(128) prefix_merge_rows_kernel(__nv_bfloat16* __restrict__ out, const Params p) {
   dependent_launch_trigger();
   const int h = blockIdx.x * 4 + (threadIdx.x >> 5), i = blockIdx.y, b = blockIdx.z;
@@ -585,7 +601,7 @@ __global__ void __launch_bounds__(128) prefix_merge_rows_kernel(__nv_bfloat16* _
   dependent_launch_wait();
   if (i >= tokens || h >= p.heads) return;
   const size_t row = (size_t)(token0 + i) * p.heads + h;
-  merge_row<D>(out + row * D, p, row * p.slots, slices_of<ROWS>(p, shared, kv_len, pos0, tokens, i, h % groups), threadIdx.x & 31);
+  merge_row<D, DEPTH>(out + row * D, p, row * p.slots, slices_of<ROWS>(p, shared, kv_len, pos0, tokens, i, h % groups), threadIdx.x & 31);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -600,7 +616,7 @@ constexpr int MASS_CHUNK = 512;          // keys per block of 128 threads, four 
 constexpr int MASS_ROWS = 32;            // rows at a time
 
 // Blocks 0 .. row_blocks - 1 of a request merge its rows (a block each, or a warp each where WARPS); the others add the weights of a chunk of one kv head's keys.
-template <int D, bool WARPS>
+template <int D, bool WARPS, int DEPTH>
 __global__ void __launch_bounds__(128) mass_merge_kernel(__nv_bfloat16* __restrict__ out, const Params p, const MassParams m) {
   dependent_launch_trigger();
   extern __shared__ float weights[];     // [slots], then [MERGE_WARPS][D]
@@ -613,9 +629,9 @@ __global__ void __launch_bounds__(128) mass_merge_kernel(__nv_bfloat16* __restri
     if (i >= tokens) return;
     const int slices = slices_of<ROWS>(p, 0, n, pos0, tokens, i, h % groups);
     const size_t row = (size_t)(token0 + i) * p.heads + h;
-    if constexpr (WARPS) merge_row<D>(out + row * D, p, row * p.slots, slices, lane);
+    if constexpr (WARPS) merge_row<D, DEPTH>(out + row * D, p, row * p.slots, slices, lane);
     else
-      pae_attention::merge_parts<D, 24>(out + row * D, p.part_out + row * p.slots * D, p.part_max + row * p.slots, p.part_sum + row * p.slots, slices, p.slots, weights);
+      pae_attention::merge_parts<D, DEPTH>(out + row * D, p.part_out + row * p.slots * D, p.part_max + row * p.slots, p.part_sum + row * p.slots, slices, p.slots, weights);
     return;
   }
   const int g = ((int)blockIdx.x - m.row_blocks) / m.chunks, key0 = (((int)blockIdx.x - m.row_blocks) % m.chunks) * MASS_CHUNK;
@@ -903,6 +919,11 @@ Cut cut_keys(int seqs, int groups, int heads, int kv_heads, int box, int max_q_l
   return c;
 }
 
+// Whether the merge of so many rows, a warp each, asks for 16 slices of a row at once: the registers leave an SM some 20 warps then, which have to hold all rows.
+// us a pass with 8 and 16 at once: 28 heads of 64 requests (1,792 rows) 32.5 and 30.3; 40 heads of 24 requests of five tokens 92.2 and 93.0, 28 heads of 180
+// requests 54.6 and 56.0. mass_merge_kernel's rows, 4 and 16 at once: 28 heads of 16 requests of up to five tokens 84.5 and 72.1, of 48 148 and 164.
+bool rows_in_flight(long long rows) { return rows <= 16LL * pae_attention::multiprocessors(); }
+
 template <int D>
 int launch(const Params& p, void* out, long long pages, int blocks, int seqs, int max_q_len, cudaStream_t s) {
   PageMaps maps;
@@ -913,8 +934,10 @@ int launch(const Params& p, void* out, long long pages, int blocks, int seqs, in
   if (int err = check_launch("paged_attention_prefix")) return err;
   // A warp a row where the rows fill the SMs with warps, a block a row below that. 12 heads of 4 requests 8.3 us a pass with warps and 7.7 with blocks,
   // 28 heads of 64 35.1 and 35.7, 14 heads of 123 18.8 and 19.8; the rows of mass_merge_kernel, 28 heads of 48 requests of five tokens, 154 and 199.
-  if ((long long)p.heads * max_q_len * seqs >= 8LL * pae_attention::multiprocessors()) {
-    launch_kernel(prefix_merge_rows_kernel<D>, dim3((p.heads + 3) / 4, max_q_len, seqs), dim3(128), 0, s, (__nv_bfloat16*)out, p);
+  const long long rows = (long long)p.heads * max_q_len * seqs;
+  if (rows >= 8LL * pae_attention::multiprocessors()) {
+    const auto merge = rows_in_flight(rows) ? prefix_merge_rows_kernel<D, 16> : prefix_merge_rows_kernel<D, 8>;
+    launch_kernel(merge, dim3((p.heads + 3) / 4, max_q_len, seqs), dim3(128), 0, s, (__nv_bfloat16*)out, p);
     return check_launch("paged_attention_prefix");
   }
   const auto merge = pae_attention::merge_in_few_registers(p.heads * max_q_len, seqs, p.slots) ? prefix_merge_kernel<D, 8> : prefix_merge_kernel<D, 24>;
@@ -923,7 +946,7 @@ int launch(const Params& p, void* out, long long pages, int blocks, int seqs, in
   return check_launch("paged_attention_prefix");
 }
 
-template <int D, bool WARPS>
+template <int D, bool WARPS, int DEPTH>
 int launch_mass(const Params& p, const MassParams& m, void* out, long long pages, int blocks, int seqs, cudaStream_t s) {
   PageMaps maps;
   if (int err = encode_page_maps(&maps, p.keys, p.values, pages, p.kv_heads, p.page_size, D, BKEYS)) return err;
@@ -931,7 +954,7 @@ int launch_mass(const Params& p, const MassParams& m, void* out, long long pages
   if (int err = raise_shared_memory(devices, prefix_kernel<D, true>, Layout<D>::SMEM_BYTES, "paged_attention_mass")) return err;
   launch_kernel(prefix_kernel<D, true>, dim3(blocks), dim3(THREADS), Layout<D>::SMEM_BYTES, s, maps, p);
   if (int err = check_launch("paged_attention_mass")) return err;
-  launch_kernel(mass_merge_kernel<D, WARPS>, dim3(m.row_blocks + p.kv_heads * m.chunks, seqs), dim3(128),
+  launch_kernel(mass_merge_kernel<D, WARPS, DEPTH>, dim3(m.row_blocks + p.kv_heads * m.chunks, seqs), dim3(128),
                 WARPS ? 0 : (p.slots + pae_attention::MERGE_WARPS * D) * sizeof(float), s, (__nv_bfloat16*)out, p, m);
   return check_launch("paged_attention_mass");
 }
@@ -1081,9 +1104,10 @@ PAE_EXPORT int pae_paged_attention_few_mass(void* out, const void* qkv, const vo
   p.part_max = p.part_out + (size_t)tokens * heads * p.slots * d;
   p.part_sum = p.part_max + (size_t)tokens * heads * p.slots;
   const int rows = heads * max_q_len;
-  const bool warps = (long long)rows * seqs >= 8LL * pae_attention::multiprocessors();
+  const bool warps = (long long)rows * seqs >= 8LL * pae_attention::multiprocessors(), deep = rows_in_flight((long long)rows * seqs);
   const MassParams m = {mass, slots, keep_first, warps ? (rows + 3) / 4 : rows, (p.span + MASS_CHUNK - 1) / MASS_CHUNK};
   const cudaStream_t s = (cudaStream_t)stream;
-  if (d == 64) return warps ? launch_mass<64, true>(p, m, out, pages, (int)blocks, seqs, s) : launch_mass<64, false>(p, m, out, pages, (int)blocks, seqs, s);
-  return warps ? launch_mass<128, true>(p, m, out, pages, (int)blocks, seqs, s) : launch_mass<128, false>(p, m, out, pages, (int)blocks, seqs, s);
+  const auto run = d == 64 ? (!warps ? launch_mass<64, false, 24> : deep ? launch_mass<64, true, 16> : launch_mass<64, true, 4>)
+                           : (!warps ? launch_mass<128, false, 24> : deep ? launch_mass<128, true, 16> : launch_mass<128, true, 4>);
+  return run(p, m, out, pages, (int)blocks, seqs, s);
 }

@@ -146,6 +146,14 @@ def test_few_tokens(ops, heads, kv_heads, dim, page, lengths, tokens):
     ops.check_device_errors()
 
 
+@pytest.mark.parametrize("dim,requests", [(64, 4), (64, 8), (128, 4)])
+def test_few_tokens_behind_more_than_32_slices(ops, dim, requests):
+    """A long context beside short ones; a warp merges a row, 32 slices a round."""
+    step = Step([26000, 40, 300, 17, 16, 90, 5000, 64][:requests], [16] * requests, 20, 1, dim, 16, BF16, requests)
+    _check(step, *_run(ops, step))
+    ops.check_device_errors()
+
+
 @pytest.mark.parametrize("dtype,dim,page", [(BF16, 128, 16), (BF16, 64, 64), (F32, 64, 16)])
 @pytest.mark.parametrize("tokens,max_q_len", [(1, 1), (3, 3), (90, 90)])
 def test_requests_without_keys(ops, dtype, dim, page, tokens, max_q_len):

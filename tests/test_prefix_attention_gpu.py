@@ -179,6 +179,12 @@ def test_a_step_without_tokens_and_operands_that_start_anywhere(ops):
         ops.paged_attention_mass(pools[0], pools[1], pools[2].transpose(0, 1).contiguous().transpose(0, 1), mass, *tables, *step.sizes, *step.longest, step.scale)
 
 
+@pytest.mark.parametrize("dim,requests", [(64, 4), (64, 8), (128, 4)])
+def test_own_keys_in_more_than_32_slices(ops, dim, requests):
+    step = _step(((requests, 100),), [26000, 40, 300, 17, 16, 90, 5000, 64][:requests], [16] * requests, 20, 1, dim, 16, BF16, requests)
+    _check(step, _run(ops, step))
+
+
 @pytest.mark.parametrize("tokens", [16, 63, 64, 65])
 def test_up_to_64_tokens_a_request_share(ops, tokens):
     step = _step(((3, 500), (2, 90)), [tokens + 9, 150, tokens, 130, 77], [tokens, 1, 5, tokens, 64], 12, 2, 128, 16, BF16, tokens)
