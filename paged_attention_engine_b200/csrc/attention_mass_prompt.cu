@@ -34,6 +34,7 @@ constexpr int SUM_WARPS = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Params {
+  __nv_bfloat16* out;           // [tokens, heads, d]
   float* mass;                  // [pages, kv_heads, page_size]
   float* part;                  // [chunks, requests, kv_heads, span]
   const float* lse;             // [tokens, heads], units of log2
@@ -42,7 +43,7 @@ struct Params {
   const int* q_pos0;
   const int* kv_len;
   const int* slots;             // [tokens] or null: a request whose first slot is negative pads the step
-  int table_width, heads, kv_heads, page_size, keep_first;
+  int table_width, heads, kv_heads, d, page_size, keep_first;
   int tile_tokens, chunk_tiles, span, seqs;
   float scale_log2;
   int* error;
@@ -287,6 +288,11 @@ __global__ void __launch_bounds__(KEYS) add_chunks_kernel(const Params p, int ch
   const int g = blockIdx.y, b = blockIdx.z, key0 = blockIdx.x * KEYS, j = key0 + threadIdx.x;
   Tiles tiles = tiles_of(p, b, key0, 0);
   const int n = min(p.kv_len[b], tiles.pos0 + tiles.tokens);
+  if (n <= 0 && key0 == 0 && tiles.tokens > 1) {      // a request without keys: the attention leaves its rows as they were
+    const int pieces = p.heads / p.kv_heads * p.d / 8;                                // of 16 bytes, of a token's heads of g
+    uint4* out = (uint4*)(p.out + (size_t)p.q_start[b] * p.heads * p.d) + g * pieces;
+    for (int i = threadIdx.x; i < tiles.tokens * pieces; i += KEYS) out[(size_t)(i / pieces) * p.kv_heads * pieces + i % pieces] = make_uint4(0, 0, 0, 0);
+  }
   if (j < p.keep_first || j >= min(n, p.span) || tiles.tokens < 2 || (p.slots != nullptr && p.slots[p.q_start[b]] < 0)) return;
   float w = 0.f;
   for (int c = 0; c < chunks; ++c) {
@@ -351,8 +357,9 @@ PAE_EXPORT long long pae_attention_mass_prompt_floats(int seqs, int heads, int k
   return (long long)chunk_count(seqs, kv_heads, max_q_len, max_kv_len, TILE / (heads / kv_heads)) * seqs * kv_heads * max_kv_len;
 }
 
-// Adds the weights of the requests that bring more than one token. `lse` [tokens, heads] is what the attention left of their rows.
-PAE_EXPORT int pae_attention_mass_prompt(float* mass, const void* qkv, const void* keys, long long pages, const float* lse, const int* block_table,
+// Adds the weights of the requests that bring more than one token. `lse` [tokens, heads] is what the attention left of their rows,
+// `out` its result, in which the rows of requests without keys become zeros.
+PAE_EXPORT int pae_attention_mass_prompt(void* out, float* mass, const void* qkv, const void* keys, long long pages, const float* lse, const int* block_table,
                                          int table_width, const int* q_start, const int* q_pos0, const int* kv_len, const int* slots, int tokens, int seqs,
                                          int max_q_len, int max_kv_len, int heads, int kv_heads, int d, int page_size, float scale, int keep_first,
                                          float* scratch, int* error, void* stream) {
@@ -361,6 +368,8 @@ PAE_EXPORT int pae_attention_mass_prompt(float* mass, const void* qkv, const voi
     return fail(2, "attention_mass: %d heads over %d of head_dim %d with pages of %d are not taken", heads, kv_heads, d, page_size);
   if (((uintptr_t)qkv | (uintptr_t)keys) & 15) return fail(2, "attention_mass: an operand does not start on a 16-byte boundary");
   Params p = {};
+  p.out = (__nv_bfloat16*)out;
+  p.d = d;
   p.mass = mass;
   p.part = scratch;
   p.lse = lse;

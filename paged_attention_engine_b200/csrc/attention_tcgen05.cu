@@ -937,10 +937,6 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_tcgen05_paired_kernel(cons
           }
         }
       }
-    } else if (active && n_tiles <= 0 && r < rows) {              // a request without keys: zeros
-      const size_t row = (size_t)(first_token + tile * BQ + r) * p.heads + h;
-      if (p.lse != nullptr) p.lse[row] = logarithm(reference, row_sum);
-      for (int c = 0; c < D; c += 8) *(uint4*)(p.out + row * D + c) = make_uint4(0, 0, 0, 0);
     }
   }
 

@@ -2558,7 +2558,7 @@ def _prompt_mass(lib, out, qkv, keys, values, mass, block_table, q_start, q_pos0
         q_pos0.data_ptr(), kv_len.data_ptr(), tokens, seqs, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, 0, 1, singles, 0, None,
         _ptr(listed), (listed.numel() if listed is not None else 0), logarithms.data_ptr(), error, _stream()))
     _check(lib, lib.pae_attention_mass_prompt(
-        mass.data_ptr(), qkv.data_ptr(), keys.data_ptr(), keys.shape[0], logarithms.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
+        out.data_ptr(), mass.data_ptr(), qkv.data_ptr(), keys.data_ptr(), keys.shape[0], logarithms.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
         q_pos0.data_ptr(), kv_len.data_ptr(), _ptr(slots), tokens, seqs, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first,
         scratch.data_ptr(), error, _stream()), 2)
 
@@ -2590,13 +2590,13 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
             raise KernelError(f"paged_attention_mass: slots {tuple(slots.shape)} for {tokens} tokens")
     _here(what, _MASS_TENSORS, qkv, keys, values, block_table, q_start, q_pos0, kv_len, mass, *(() if slots is None else (slots,)))
     operands = _aligned_operands(what, qkv, keys, values, head_dim)
-    if tokens == 0 or seqs == 0:
-        return qkv.new_empty((tokens, num_heads * head_dim))
+    if tokens == 0 or seqs == 0 or max_kv_len == 0:
+        return qkv.new_zeros((tokens, num_heads * head_dim))
     singles = num_single if num_single is not None else (seqs if max_q_len == 1 else -1)
     if singles < 0 and tokens > (seqs - 1) * max_q_len + 1:
         singles = 0                                       # a request of one token would leave more to the others than they can bring
     sizes = (num_heads, num_kv_heads, head_dim, page_size)
-    if max_kv_len > 0 and qkv.dtype is torch.bfloat16 and use_tensor_cores and max_q_len > 0:
+    if qkv.dtype is torch.bfloat16 and use_tensor_cores and max_q_len > 0:
         few = 1 < max_q_len <= MASS_FEW_TOKENS and _prefix_supports(*sizes)
         if few or (_mass_supports(*sizes) and (max_q_len == 1 or (use_tcgen05_attention and _prompt_mass_supports(*sizes)))):
             out = qkv.new_empty((tokens, num_heads * head_dim))
@@ -2611,7 +2611,7 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
                 _decode_mass(out, qkv, keys, operands, mass, block_table, table_width, q_start, kv_len, slots, seqs, sizes, max_kv_len, scale, keep_first,
                              seqs if singles < 0 else singles)
             return out
-    if max_q_len == 1 and max_kv_len > 0 and head_dim % 4 == 0 and head_dim <= 256 and num_heads // num_kv_heads <= 16 and not (
+    if max_q_len == 1 and head_dim % 4 == 0 and head_dim <= 256 and num_heads // num_kv_heads <= 16 and not (
             operands[0] | operands[1] | operands[2]) & (4 * qkv.element_size() - 1):
         slice_keys, max_slices, floats = _any_slicing(seqs, num_heads, num_kv_heads, head_dim, max_kv_len)
         out = qkv.new_empty((tokens, num_heads * head_dim))
