@@ -64,10 +64,11 @@ __device__ __forceinline__ uint32_t value_step(int k, int rows_a_box) {
 template <int D>
 __device__ __forceinline__ void clear_values(uint8_t* tile, int from, int rows, int rows_a_box, int lane) {
   constexpr int CHUNKS = D / 8;
-  for (int i = lane; i < (rows - from) * CHUNKS; i += 32) {
-    const int row = from + i / CHUNKS, chunk = i % CHUNKS;
-    *(uint4*)(tile + ((row / rows_a_box) * (D / 64) + chunk / 8) * rows_a_box * 128 + (row % rows_a_box) * 128 + (chunk % 8) * 16) = make_uint4(0, 0, 0, 0);
-  }
+  const int chunk = lane % CHUNKS, in_box = rows_a_box - 1;          // boxes have 16, 32, 64 or 128 rows
+  uint8_t* to = tile + chunk / 8 * rows_a_box * 128 + chunk % 8 * 16;
+#pragma unroll 4
+  for (int row = from + lane / CHUNKS; row < rows; row += 32 / CHUNKS)
+    *(uint4*)(to + ((row & ~in_box) * (D / 64) + (row & in_box)) * 128) = make_uint4(0, 0, 0, 0);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
 }
