@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(ANY_THREADS) row_stats_kernel(const RowParams<
   }
 }
 
-// Which row tiles a block of column_sums_kernel takes: those of its chunk that see its keys. Empty: first >= last.
+// Which row tiles a block of any_column_sums_kernel takes: those of its chunk that see its keys. Empty: first >= last.
 struct ChunkTiles {
   int first, last, pos0, tokens, n;
 };
@@ -572,7 +572,7 @@ __device__ __forceinline__ ChunkTiles chunk_tiles(const RowParams<T>& p, int b, 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(ANY_THREADS) column_sums_kernel(const RowParams<T> p, bool vector) {
+__global__ void __launch_bounds__(ANY_THREADS) any_column_sums_kernel(const RowParams<T> p, bool vector) {
   extern __shared__ __align__(16) float shared[];
   __shared__ float logarithm[ROWS], halves[ANY_KEYS];
   dependent_launch_prologue();
@@ -668,11 +668,11 @@ int launch_rows(RowParams<T> p, const RowCut& c, int max_kv_len, cudaStream_t s)
   const bool vector = p.d % 4 == 0 && (((uintptr_t)p.qkv | (uintptr_t)p.keys) & (4 * sizeof(T) - 1)) == 0;
   static DevicesSet stats_devices, column_devices;
   if (int err = raise_shared_memory(stats_devices, row_stats_kernel<T>, 200 * 1024, "attention_mass")) return err;
-  if (int err = raise_shared_memory(column_devices, column_sums_kernel<T>, 200 * 1024, "attention_mass")) return err;
+  if (int err = raise_shared_memory(column_devices, any_column_sums_kernel<T>, 200 * 1024, "attention_mass")) return err;
   const int key_tiles = (max_kv_len + ANY_KEYS - 1) / ANY_KEYS;
   launch_kernel(row_stats_kernel<T>, dim3(c.row_tiles * c.runs, p.m.kv_heads, p.seqs), dim3(ANY_THREADS), bytes, s, p, vector);
   if (int err = check_launch("attention_mass")) return err;
-  launch_kernel(column_sums_kernel<T>, dim3(key_tiles, p.m.kv_heads * c.chunks, p.seqs), dim3(ANY_THREADS), bytes, s, p, vector);
+  launch_kernel(any_column_sums_kernel<T>, dim3(key_tiles, p.m.kv_heads * c.chunks, p.seqs), dim3(ANY_THREADS), bytes, s, p, vector);
   if (int err = check_launch("attention_mass")) return err;
   launch_kernel(add_chunks_kernel<T>, dim3(key_tiles, p.m.kv_heads, p.seqs), dim3(ANY_KEYS), 0, s, p, c.chunks);
   return check_launch("attention_mass");

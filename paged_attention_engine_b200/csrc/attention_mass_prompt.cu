@@ -18,6 +18,7 @@
 // heads over 4 of 128, take 97 us beside 123 for the attention, the exponentials' pipe half busy. One thread a key, blocks of 256 keys alone on an SM, and three to
 // five stages of queries took the same time.
 #include <cfloat>
+#include <climits>
 
 #include "attention_pages.cuh"
 
@@ -97,17 +98,13 @@ __global__ void __launch_bounds__(THREADS, 2) column_sums_kernel(const __grid_co
   // The last chunks' rows see the most keys: their blocks go first, the shorter ones fill in behind them.
   const int g = blockIdx.y % p.kv_heads, b = blockIdx.y / p.kv_heads, chunk = gridDim.z - 1 - blockIdx.z, key0 = blockIdx.x * KEYS;
   const Tiles tiles = tiles_of(p, b, key0, chunk);
-  if (tiles.first >= tiles.last) {
-    dependent_launch_trigger();
-    dependent_launch_wait();
-    return;
-  }
+  const bool working = tiles.first < tiles.last;       // the same in every thread
   const int n_tiles = tiles.last - tiles.first;
   const int first_token = p.q_start[b];
   const int kv_end = min(p.kv_len[b], tiles.pos0 + tiles.tokens);
   const int groups = p.heads / p.kv_heads, tile_rows = p.tile_tokens * groups;
 
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && working) {
     mbar_init(bar(K_FULL), 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(Q_FULL, i), 1);
@@ -120,12 +117,12 @@ __global__ void __launch_bounds__(THREADS, 2) column_sums_kernel(const __grid_co
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
+  if (warp == 1 && working) {
     tmem_alloc(smem_u32((const void*)tmem_holder), L::TMEM_COLUMNS);
     tmem_relinquish();
   }
   // Rows of a stage that no box fills are zeros: their scores are masked, but they are computed.
-  for (int i = threadIdx.x; i < (TILE - tile_rows) * (D / 8) * STAGES; i += THREADS) {
+  for (int i = working ? threadIdx.x : INT_MAX; i < (TILE - tile_rows) * (D / 8) * STAGES; i += THREADS) {
     const int stage = i / ((TILE - tile_rows) * (D / 8)), rest = i % ((TILE - tile_rows) * (D / 8));
     const int row = tile_rows + rest / (D / 8), c = rest % (D / 8);
     *(uint4*)(generic_base + L::Q_OFFSET + stage * L::TILE_BYTES + (c >> 3) * L::HALF_BYTES + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -137,6 +134,7 @@ __global__ void __launch_bounds__(THREADS, 2) column_sums_kernel(const __grid_co
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_holder;
   dependent_launch_wait();
+  if (!working) return;
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer

@@ -191,19 +191,15 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
   auto bar = [&](int which, int i = 0) { return bars + 8u * (which + i); };
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const Work work = find_work<ROWS>(p, blockIdx.x);
-  if (work.rows <= 0 || work.begin >= work.end) {      // the same in every thread
-    dependent_launch_trigger();
-    dependent_launch_wait();
-    return;
-  }
+  const bool working = work.rows > 0 && work.begin < work.end;      // the same in every thread
   const int rows = work.rows, kv_begin = work.begin, kv_end = work.end, g = work.g, groups = p.heads / p.kv_heads;
   const int n_tiles = (kv_end - kv_begin + BKEYS - 1) / BKEYS;
   const int row_warps = (rows + 31) / 32;              // the softmax warps that have rows
 
   const int box_rows = min(p.page_size, BKEYS);
   PageRun pages;                                       // of the producer; the table was on the device before the step's first kernel began
-  if (warp == 0) pages.start(p.block_table + (size_t)work.b * p.table_width, kv_begin, kv_end, box_rows, p.page_size, p.table_width, lane);
-  if (threadIdx.x == 0) {
+  if (warp == 0 && working) pages.start(p.block_table + (size_t)work.b * p.table_width, kv_begin, kv_end, box_rows, p.page_size, p.table_width, lane);
+  if (threadIdx.x == 0 && working) {
     mbar_init(bar(Q_FULL), SOFTMAX_WARPS * 32);
     for (int i = 0; i < KV_STAGES; ++i) {
       mbar_init(bar(K_FULL, i), 1);
@@ -220,7 +216,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
+  if (warp == 1 && working) {
     tmem_alloc(smem_u32((const void*)tmem_holder), L::TMEM_COLUMNS);
     tmem_relinquish();
   }
@@ -230,6 +226,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_holder;
   dependent_launch_wait();
+  if (!working) return;
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer: lane i brings box i of a tile
