@@ -2571,7 +2571,8 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
     `mass` is float32 [pages, kv_heads, page_size], in the pages of the keys. A key of this step starts from nothing, whatever its place held
     before. Keys before `keep_first` are left alone (they are not to be evicted): requests may share
     the pages that hold such keys only; every other page belongs to one request of the step. `slots` (int32 [tokens], as
-    `qkv_projection` takes them): a request whose first slot is negative only pads the step and adds nothing."""
+    `qkv_projection` takes them): a request whose first slot is negative only pads the step and adds nothing. `num_single` and
+    `multi_index` as `paged_attention` takes them; rows of `qkv` behind the last request do not matter."""
     qkv = materialized(qkv)
     what = "paged_attention_mass"
     tokens, seqs, table_width, pages = _need_attention(what, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim,
@@ -2593,8 +2594,6 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
     if tokens == 0 or seqs == 0 or max_kv_len == 0:
         return qkv.new_zeros((tokens, num_heads * head_dim))
     singles = num_single if num_single is not None else (seqs if max_q_len == 1 else -1)
-    if singles < 0 and tokens > (seqs - 1) * max_q_len + 1:
-        singles = 0                                       # a request of one token would leave more to the others than they can bring
     sizes = (num_heads, num_kv_heads, head_dim, page_size)
     if qkv.dtype is torch.bfloat16 and use_tensor_cores and max_q_len > 0:
         few = 1 < max_q_len <= MASS_FEW_TOKENS and _prefix_supports(*sizes)
