@@ -157,7 +157,7 @@ __device__ __forceinline__ void add_chunk(const MassParams& m, const float* __re
     total = warp_sum(total);
     if (lane == 0) {
       top_of[r] = top;
-      inverse_of[r] = total > 0.f ? 1.f / total : 0.f;
+      inverse_of[r] = total == 0.f ? 0.f : 1.f / total;          // NaN for all keys of a row whose sum is NaN
     }
   }
   __syncthreads();

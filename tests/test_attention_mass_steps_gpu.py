@@ -50,3 +50,19 @@ def test_rows_behind_the_last_request(ops, lengths, tokens, dtype, dim, behind):
     step = Step(lengths, tokens, 12, 2, dim, 16, dtype, behind)
     qkv = torch.cat((step.qkv, torch.full((behind, step.qkv.shape[1]), math.nan, dtype=dtype))).cuda()
     _check(step, *_run(ops, step, qkv))
+
+
+@pytest.mark.parametrize("dtype,dim,tokens", [(BF16, 128, [1, 1]), (BF16, 32, [1, 1]), (F32, 64, [1, 1]), (BF16, 128, [3, 5]), (BF16, 64, [90, 30]), (F32, 64, [4, 30])])
+def test_a_key_that_is_no_number(ops, dtype, dim, tokens):
+    """A row whose denominator is no number has no weights: that is what all of its keys get, by whichever kernel, and no other row's."""
+    step = Step([400, 290], tokens, 12, 2, dim, 16, dtype, dim)
+    step.keys[int(step.table[0, 7]), 1, 3] = math.nan           # key 115 of request 0 for kv head 1, which all of its tokens see
+    out, mass = (t.cpu().double() for t in _run(ops, step))
+    broken = torch.zeros_like(mass, dtype=torch.bool)
+    j = torch.arange(400)
+    broken[step.table[0].long()[j // 16], 1, j % 16] = True
+    expected = step.masses()
+    assert torch.equal(expected.isnan(), broken)
+    assert torch.equal(mass.isnan(), broken)
+    assert ((mass - expected)[~broken].abs() <= MASS_RTOL * expected[~broken] + MASS_ATOL).all()
+    assert torch.equal(out.isnan(), step.attention().isnan())
