@@ -44,6 +44,15 @@ __device__ __forceinline__ void add_mass(const MassParams& m, int b, int g, int 
   *to = (fresh ? 0.f : *to) + w;
 }
 
+// The weights of the step's keys start from nothing: for a step whose attention adds none. A block a request.
+__global__ void __launch_bounds__(128) start_keys_kernel(const MassParams m, const int* __restrict__ q_pos0) {
+  dependent_launch_prologue();
+  const int b = blockIdx.x, token0 = m.q_start[b], tokens = m.q_start[b + 1] - token0;
+  if (tokens < 1 || pads(m, token0)) return;
+  const int first = q_pos0[b], count = min(tokens, m.kv_len[b] - first);
+  for (int i = threadIdx.x; i < count * m.kv_heads; i += 128) add_mass(m, b, i / count, first + i % count, true, 0.f);
+}
+
 // ---------------------------------------------------------------------------------------
 // single tokens, bfloat16
 // ---------------------------------------------------------------------------------------
@@ -695,6 +704,15 @@ int launch_any(AnyParams<T> p, int seqs, cudaStream_t s) {
 }  // namespace
 
 PAE_DEFINE_LAST_ERROR()
+
+// mass of this step's keys = 0, of requests whose first slot is not negative (slots null: of all).
+PAE_EXPORT int pae_start_mass(float* mass, const int* block_table, int table_width, const int* q_start, const int* q_pos0, const int* kv_len, const int* slots, int seqs,
+                              int kv_heads, int page_size, void* stream) {
+  if (seqs < 1) return 0;
+  const MassParams m = {mass, block_table, q_start, kv_len, slots, table_width, kv_heads, kv_heads, page_size, 0};
+  launch_kernel(start_keys_kernel, dim3(seqs), dim3(128), 0, (cudaStream_t)stream, m, q_pos0);
+  return check_launch("start_mass");
+}
 
 // Floats of scratch for a step of single tokens in bfloat16, cut into slices (as pae_paged_attention_decode).
 PAE_EXPORT long long pae_decode_mass_floats(int seqs, int heads, int d, int slice_keys, int max_slices) {

@@ -2372,6 +2372,16 @@ def _need_attention(what: str, qkv, keys, values, block_table, q_start, q_pos0, 
     raise KernelError(f"{what}: tensors of {qkv.dim()}, {keys.dim()} and {block_table.dim()} dimensions for qkv, keys and the block table")
 
 
+def _need_mass(what: str, mass, slots, tokens: int, pages: int, kv_heads: int, page_size: int) -> None:
+    """Weights per key beside a pool of `pages`, and a step's slots where there are any."""
+    if mass.dtype is not torch.float32 or mass.shape != (pages, kv_heads, page_size):
+        raise KernelError(f"{what}: mass {mass.dtype} {tuple(mass.shape)}, torch.float32 {(pages, kv_heads, page_size)} is needed beside the keys")
+    if slots is not None:
+        _int32(what, slots=slots)
+        if slots.shape != (tokens,):
+            raise KernelError(f"{what}: slots {tuple(slots.shape)} for {tokens} tokens")
+
+
 # Up to how many tokens a request the shared keys are taken once for all; from there on a query tile of one request fills the tensor cores and its keys are
 # read once for all of its tokens anyway. us a pass, captured, shared and each request by itself: 24 requests behind 30,011 keys, 40 heads over 8 of 128, 48
 # tokens each 949 and 4,916, 64 1,060 and 2,006, 96 1,570 and 2,052, 128 2,063 and 2,032; 16 behind 8,000, 28 heads over 4, 48 145 and 854, 64 159 and 253,
@@ -2407,7 +2417,7 @@ def _prefix_floats(*sizes) -> int:
 
 def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_len, prefix_len, group_start, num_heads: int, num_kv_heads: int,
                            head_dim: int, page_size: int, max_q_len: int, max_prefix_len: int, max_own_len: int, max_group_tokens: int, scale: float,
-                           num_single=None, info: dict | None = None) -> torch.Tensor:
+                           num_single=None, info: dict | None = None, mass=None, slots=None) -> torch.Tensor:
     """`paged_attention` without a window for requests that share the first keys of their contexts, which are read once for all.
     Requests group_start[i] .. group_start[i + 1] - 1 (int32 [groups + 1], from 0 to the number of requests) are a group: their first
     prefix_len[b] keys (int32 [requests], the same for all of a group; 0: nothing is shared) are the same, and every token of the step stands behind
@@ -2416,7 +2426,9 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     keys behind them. `info`, when given, receives which kernel ran ("kernel"): "shared", on tensor cores (bfloat16, head sizes 64 and 128, pages
     of 16, 32, 64 or 128 keys), "shared simt" (long prefixes in float32 and of what no tensor-core attention takes; head sizes that are multiples of 4 up
     to 256), or what
-    `paged_attention` says where each request reads its keys by itself (other sizes, long portions, groups of one request)."""
+    `paged_attention` says where each request reads its keys by itself (other sizes, long portions, groups of one request).
+    This attention adds no weights. With `mass` (as `paged_attention_mass` keeps it; `slots` as there) the step's keys start from nothing in it, so that a later
+    step's weights are added to 0 and not to what the page's earlier owner left."""
     qkv = materialized(qkv)
     what = "paged_attention_prefix"
     tokens, seqs, table_width, pages = _need_attention(what, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim,
@@ -2434,10 +2446,19 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
         raise KernelError(f"{what}: scores scaled by {scale}")
     if max_group_tokens > tokens:
         max_q_len, max_group_tokens = min(max_q_len, tokens), tokens
+    if mass is not None:
+        _need_mass(what, mass, slots, tokens, pages, num_kv_heads, page_size)
     _here(what, _PREFIX_TENSORS, qkv, keys, values, block_table, q_start, q_pos0, kv_len, prefix_len, group_start)
+    if mass is not None:
+        _here(what, ("mass", "slots"), mass, *(() if slots is None else (slots,)))
     operands = _aligned_operands(what, qkv, keys, values, head_dim)
     if tokens == 0:
         return qkv.new_empty((0, num_heads * head_dim))
+    if mass is not None:
+        lib = _lib("attention_mass")
+        _set_bounds("attention_mass", keys)
+        _check(lib, lib.pae_start_mass(mass.data_ptr(), block_table.data_ptr(), table_width, q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(), _ptr(slots), seqs,
+                                       num_kv_heads, page_size, _stream()))
     sizes = (tokens, seqs, groups, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_prefix_len, max_own_len, max_group_tokens)
     form = None
     if 0 < max_q_len <= PREFIX_ATTENTION_MAX_TOKENS and max_prefix_len > 0 and max_group_tokens > max_q_len:
@@ -2572,23 +2593,21 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
     before. Keys before `keep_first` are left alone (they are not to be evicted): requests may share
     the pages that hold such keys only; every other page belongs to one request of the step. `slots` (int32 [tokens], as
     `qkv_projection` takes them): a request whose first slot is negative only pads the step and adds nothing. `num_single` and
-    `multi_index` as `paged_attention` takes them; rows of `qkv` behind the last request do not matter."""
+    `multi_index` as `paged_attention` takes them; rows of `qkv` behind the last request do not matter.
+    A key that came with a step of another attention has no start here: its place still holds what the page's earlier owner left, unless
+    `paged_attention_prefix` was given `mass` in that step, or the caller wrote 0 there. What a drafted token gave to the keys before it stays in their sums when
+    the token is rejected later; the place of its own key starts anew with the key that takes it."""
     qkv = materialized(qkv)
     what = "paged_attention_mass"
     tokens, seqs, table_width, pages = _need_attention(what, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim,
                                                        page_size)
-    if mass.dtype is not torch.float32 or mass.shape != (pages, num_kv_heads, page_size):
-        raise KernelError(f"paged_attention_mass: mass {mass.dtype} {tuple(mass.shape)} beside keys {tuple(keys.shape)}")
+    _need_mass(what, mass, slots, tokens, pages, num_kv_heads, page_size)
     if keep_first < 0:
         raise KernelError(f"paged_attention_mass: {keep_first} first keys")
     if not scale >= 0:
         raise KernelError(f"paged_attention_mass: scores scaled by {scale}")
     if not 0 <= max_kv_len <= table_width * page_size:
         raise KernelError(f"paged_attention_mass: {max_kv_len} keys for tables of {table_width} pages of {page_size}")
-    if slots is not None:
-        _int32("paged_attention_mass", slots=slots)
-        if slots.shape != (tokens,):
-            raise KernelError(f"paged_attention_mass: slots {tuple(slots.shape)} for {tokens} tokens")
     _here(what, _MASS_TENSORS, qkv, keys, values, block_table, q_start, q_pos0, kv_len, mass, *(() if slots is None else (slots,)))
     operands = _aligned_operands(what, qkv, keys, values, head_dim)
     if tokens == 0 or seqs == 0 or max_kv_len == 0:
