@@ -2421,7 +2421,8 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     """`paged_attention` without a window for requests that share the first keys of their contexts, which are read once for all.
     Requests group_start[i] .. group_start[i + 1] - 1 (int32 [groups + 1], from 0 to the number of requests) are a group: their first
     prefix_len[b] keys (int32 [requests], the same for all of a group; 0: nothing is shared) are the same, and every token of the step stands behind
-    them. They are read through the block table of the group's first request. The result is that of `paged_attention` but for the order of the sums.
+    them. Every request's block table names pages that hold them, the group's or copies: the shared kernels read them through the table of the group's first
+    request, and in the page that the prefix ends in, and wherever requests read by themselves, through their own. The result is that of `paged_attention` but for the order of the sums.
     The longest request brings at most `max_q_len` tokens, the largest group `max_group_tokens`; `max_prefix_len` and `max_own_len` bound the shared keys and the
     keys behind them. `info`, when given, receives which kernel ran ("kernel"): "shared", on tensor cores (bfloat16, head sizes 64 and 128, pages
     of 16, 32, 64 or 128 keys), "shared simt" (long prefixes in float32 and of what no tensor-core attention takes; head sizes that are multiples of 4 up
