@@ -787,7 +787,8 @@ PAE_EXPORT int pae_paged_attention_any_mass(void* out, const void* qkv, const vo
 // Floats of scratch for pae_attention_mass_rows.
 PAE_EXPORT long long pae_attention_mass_floats(int tokens, int seqs, int heads, int kv_heads, int max_q_len, int max_kv_len) {
   if (seqs < 1 || max_q_len < 1 || max_kv_len < 1) return 1;
-  return 2ll * MOST_RUNS * tokens * heads + (long long)cut_rows(seqs, heads, kv_heads, max_q_len, max_kv_len).chunks * seqs * kv_heads * max_kv_len;
+  const RowCut c = cut_rows(seqs, heads, kv_heads, max_q_len, max_kv_len);
+  return 2ll * c.runs * tokens * heads + (long long)c.chunks * seqs * kv_heads * max_kv_len;
 }
 
 // The weights of any step's keys, whatever its rows, type (0 float32, 1 bfloat16) and head size; the attention's output is not computed.
@@ -801,8 +802,8 @@ PAE_EXPORT int pae_attention_mass_rows(float* mass, const void* qkv, const void*
     return fail(1, "paged_attention_mass: %d requests of %d kv heads x %d chunks exceed one launch", seqs, kv_heads, c.chunks);
   const MassParams m = {mass, block_table, q_start, kv_len, slots, table_width, heads, kv_heads, page_size, keep_first};
   const long long rows = (long long)tokens * heads;
-  float* part_sum = scratch + (long long)MOST_RUNS * rows;
-  float* part = part_sum + (long long)MOST_RUNS * rows;
+  float* part_sum = scratch + c.runs * rows;
+  float* part = part_sum + c.runs * rows;
   const float scale_log2 = scale * LOG2E;
   const cudaStream_t s = (cudaStream_t)stream;
   if (dtype == kF32)

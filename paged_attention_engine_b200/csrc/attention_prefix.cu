@@ -15,8 +15,9 @@
 //            own keys, which few rows read, a tile costs little more than its bytes.
 //   merge    a row's slices, shared and own, in their order.
 //
-// The same kernel without shared keys is the attention of paged_attention_mass for steps of few tokens: it leaves its scores besides (4 bytes for each query
-// head and key, where keys and values are 4 * head size bytes for each kv head and key), and further blocks of the merge turn them into
+// The same kernel without shared keys is the attention of paged_attention_mass for steps of few tokens: it leaves its scores besides (4 bytes for each token, query
+// head and key, where keys and values are 4 * head size bytes for each kv head and key; in rows as long as the longest context, whatever the request's own, so a
+// launch takes as many of the step's requests as a bound on its scratch allows), and further blocks of the merge turn them into
 // weights once a row's maximum and sum are known, and add them up per key (attention_mass.cu says what is computed).
 //
 // Other types and sizes than those of the tensor-core kernel take the same slices of 16 rows on CUDA cores (any_slices_kernel).
@@ -60,7 +61,9 @@ struct Params {
   int own_row_tiles, own_slices, own_keys;                       // likewise of the own ones
   int slots;                    // slices of a row at most: shared ones, then own ones
   int box;                      // own slices start on multiples of it
-  float* scores;                // [tokens, heads, span], not scaled, of own keys
+  int max_tokens;               // of a request
+  int part_tokens;              // that the scratch holds where it holds scores
+  float* scores;                // [tokens, heads, span], not scaled, of own keys; token 0 is the first request's first
   int span;
   float scale_log2, slack;
   int* error;
@@ -129,6 +132,10 @@ __device__ __forceinline__ OwnSpan own_span(const Params& p, int shared, int kv_
   return s;
 }
 
+__device__ __forceinline__ int tokens_of(const Params& p, int b) { return min(p.q_start[b + 1] - p.q_start[b], p.max_tokens); }
+// Whether a request's tokens have room in the scratch: they do unless a request before brought more than `max_tokens`.
+__device__ __forceinline__ bool in_part(const Params& p, int token0, int tokens) { return p.scores == nullptr || token0 - p.q_start[0] + tokens <= p.part_tokens; }
+
 // What a block works on: rows row0 .. row0 + rows - 1 (token, head of kv head g) behind `first_token`, keys begin .. end - 1 by the table of
 // request b. Row r sees those from `first` on that stand at or before pos0 + its token's index.
 struct Work {
@@ -165,7 +172,8 @@ __device__ __forceinline__ Work find_work(const Params& p, int index) {
   w.g = index % p.kv_heads;
   w.b = index / p.kv_heads;
   w.first_token = p.q_start[w.b];
-  const int tokens = p.q_start[w.b + 1] - w.first_token, shared = p.max_prefix > 0 ? min(p.prefix_len[w.b], p.max_prefix) : 0;
+  const int tokens = tokens_of(p, w.b), shared = p.max_prefix > 0 ? min(p.prefix_len[w.b], p.max_prefix) : 0;
+  if (!in_part(p, w.first_token, tokens)) return w;
   w.pos0 = p.q_pos0[w.b];
   const OwnSpan span = own_span<TILE_ROWS>(p, shared, p.kv_len[w.b], w.pos0, tokens, groups, row_tile);
   if (span.end <= span.first) return w;
@@ -326,6 +334,8 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
     const int row = work.row0 + r;
     const size_t token = (size_t)(work.first_token + row / groups);
     const int head = g * groups + row % groups;
+    // Beside scores the parts of one launch's requests are kept, which may be some of the step's (the weights' scratch has a bound).
+    const size_t part_row = (token - (SCORES ? p.q_start[0] : 0)) * p.heads + head;
     const int row_end = min(kv_end, work.pos0 + row / groups + 1);               // the keys before it are visible to the row
     const int all_see = min(kv_end, work.pos0 + work.row0 / groups + 1);         // those before it to every row
     {
@@ -395,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
       auto leave = [&](const float* s, int first, int count) {
         if constexpr (SCORES) {
           if (r < rows) {
-            float* to = p.scores + (token * p.heads + head) * p.span + key0 + first;
+            float* to = p.scores + part_row * p.span + key0 + first;
 #pragma unroll
             for (int i = 0; i < count; i += 4) *(float4*)(to + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
           }
@@ -475,7 +485,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
       if (ok) {
         tcgen05_fence_after();
         // Through shared memory, where keys and values lay (every product has read them): a row leaves as one run of bytes.
-        const uint32_t at = (uint32_t)((token * p.heads + head) * p.slots + work.slot);
+        const uint32_t at = (uint32_t)(part_row * p.slots + work.slot);
         float* mine = (float*)(generic_base + L::K_OFFSET) + quadrant * 32 * D;      // [32][D], 16-byte chunk c of row r at c ^ (r & 7)
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
@@ -523,7 +533,7 @@ __global__ void __launch_bounds__(pae_attention::MERGE_WARPS * 32) prefix_merge_
   dependent_launch_trigger();
   extern __shared__ float weights[];          // [slots], then [MERGE_WARPS][D]
   const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
-  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0;
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = tokens_of(p, b);
   const int shared = min(p.prefix_len[b], p.max_prefix), kv_len = p.kv_len[b], pos0 = p.q_pos0[b];
   dependent_launch_wait();
   if (i >= tokens) return;
@@ -593,7 +603,7 @@ template <int D, int DEPTH>
 __global__ void __launch_bounds__(128) prefix_merge_rows_kernel(__nv_bfloat16* __restrict__ out, const Params p) {
   dependent_launch_trigger();
   const int h = blockIdx.x * 4 + (threadIdx.x >> 5), i = blockIdx.y, b = blockIdx.z;
-  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0;
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = tokens_of(p, b);
   const int shared = min(p.prefix_len[b], p.max_prefix), kv_len = p.kv_len[b], pos0 = p.q_pos0[b];
   dependent_launch_wait();
   if (i >= tokens || h >= p.heads) return;
@@ -619,21 +629,21 @@ __global__ void __launch_bounds__(128) mass_merge_kernel(__nv_bfloat16* __restri
   extern __shared__ float weights[];     // [slots], then [MERGE_WARPS][D]
   __shared__ float logarithm[MASS_ROWS];
   const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0, n = p.kv_len[b], pos0 = p.q_pos0[b];
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], part0 = token0 - p.q_start[0], tokens = tokens_of(p, b), n = p.kv_len[b], pos0 = p.q_pos0[b];
   dependent_launch_wait();
   if ((int)blockIdx.x < m.row_blocks) {
     const int index = WARPS ? (int)blockIdx.x * 4 + warp : (int)blockIdx.x, i = index / p.heads, h = index % p.heads;
-    if (i >= tokens) return;
+    if (i >= tokens || part0 + tokens > p.part_tokens) return;
     const int slices = slices_of<ROWS>(p, 0, n, pos0, tokens, i, h % groups);
-    const size_t row = (size_t)(token0 + i) * p.heads + h;
-    if constexpr (WARPS) merge_row<D, DEPTH>(out + row * D, p, row * p.slots, slices, lane);
-    else
-      pae_attention::merge_parts<D, DEPTH>(out + row * D, p.part_out + row * p.slots * D, p.part_max + row * p.slots, p.part_sum + row * p.slots, slices, p.slots, weights);
+    const size_t at = ((size_t)(part0 + i) * p.heads + h) * p.slots;
+    __nv_bfloat16* to = out + ((size_t)(token0 + i) * p.heads + h) * D;
+    if constexpr (WARPS) merge_row<D, DEPTH>(to, p, at, slices, lane);
+    else pae_attention::merge_parts<D, DEPTH>(to, p.part_out + at * D, p.part_max + at, p.part_sum + at, slices, p.slots, weights);
     return;
   }
   const int g = ((int)blockIdx.x - m.row_blocks) / m.chunks, key0 = (((int)blockIdx.x - m.row_blocks) % m.chunks) * MASS_CHUNK;
   const int last = min(min(n, pos0 + tokens), p.span), rows = tokens * groups;
-  if (rows <= 0 || key0 >= last || key0 + MASS_CHUNK <= m.keep_first || (m.slots != nullptr && m.slots[token0] < 0)) return;
+  if (rows <= 0 || part0 + tokens > p.part_tokens || key0 >= last || key0 + MASS_CHUNK <= m.keep_first || (m.slots != nullptr && m.slots[token0] < 0)) return;
   const int j0 = key0 + threadIdx.x * 4;
   float w[4] = {0.f, 0.f, 0.f, 0.f};
   for (int first = 0; first < rows; first += MASS_ROWS) {
@@ -641,7 +651,7 @@ __global__ void __launch_bounds__(128) mass_merge_kernel(__nv_bfloat16* __restri
     for (int u = warp; u < min(MASS_ROWS, rows - first); u += 4) {
       const int i = (first + u) / groups, r = (first + u) % groups;
       const int slices = slices_of<ROWS>(p, 0, n, pos0, tokens, i, r);
-      const size_t at = ((size_t)(token0 + i) * p.heads + g * groups + r) * p.slots;
+      const size_t at = ((size_t)(part0 + i) * p.heads + g * groups + r) * p.slots;
       float top = -FLT_MAX, total = 0.f;
       for (int s = lane; s < slices; s += 32) top = fmaxf(top, p.part_max[at + s]);
 #pragma unroll
@@ -656,7 +666,7 @@ __global__ void __launch_bounds__(128) mass_merge_kernel(__nv_bfloat16* __restri
 #pragma unroll 4
       for (int u = 0; u < count; ++u) {
         const int i = (first + u) / groups, seen = pos0 + i;
-        const float4 s = *(const float4*)(p.scores + ((size_t)(token0 + i) * p.heads + g * groups + (first + u) % groups) * p.span + j0);
+        const float4 s = *(const float4*)(p.scores + ((size_t)(part0 + i) * p.heads + g * groups + (first + u) % groups) * p.span + j0);
         const float l = logarithm[u];
         if (j0 <= seen) w[0] += exp2f(fmaf(s.x, p.scale_log2, -l));
         if (j0 + 1 <= seen) w[1] += exp2f(fmaf(s.y, p.scale_log2, -l));
@@ -851,7 +861,7 @@ template <typename T>
 __global__ void __launch_bounds__(ANY_THREADS) any_merge_kernel(const AnyOperands<T> x, const Params p) {
   dependent_launch_prologue();
   const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
-  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0;
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = tokens_of(p, b);
   if (i >= tokens) return;
   const int slices = slices_of<ANY_ROWS>(p, min(p.prefix_len[b], p.max_prefix), p.kv_len[b], p.q_pos0[b], tokens, i, h % groups);
   const size_t row = (size_t)(token0 + i) * p.heads + h, at = row * p.slots;
@@ -1005,6 +1015,7 @@ int set_up(Params* to, long long* blocks, const int* block_table, int table_widt
   p.own_keys = c.own_keys;
   p.slots = c.slots;
   p.box = box_of(page_size, any);
+  p.max_tokens = max_q_len;
   p.scale_log2 = scale * LOG2E;
   p.slack = REFERENCE_SLACK;
   *to = p;
@@ -1070,13 +1081,14 @@ PAE_EXPORT int pae_paged_attention_prefix_any(void* out, const void* qkv, const 
                                    max_q_len, (cudaStream_t)stream);
 }
 
-// Floats of scratch that pae_paged_attention_few_mass needs.
+// Floats of scratch that pae_paged_attention_few_mass needs; `tokens`: what the requests bring at most.
 PAE_EXPORT long long pae_attention_few_mass_floats(int tokens, int seqs, int heads, int kv_heads, int d, int page_size, int max_q_len, int max_kv_len) {
   const Cut c = cut_keys(seqs, 1, heads, kv_heads, box_of(page_size, false), max_q_len, 0, max_kv_len, max_q_len, false);
   return (long long)tokens * heads * (c.slots * (d + 2) + (long long)c.own_slices * c.own_keys);
 }
 
-// Attention of a step whose requests bring few tokens, and the weights of their keys; `slots` and `keep_first` as pae_paged_attention_any_mass (attention_mass.cu) takes them.
+// Attention of consecutive requests that bring few tokens, and the weights of their keys: those that block_table, q_start, q_pos0 and kv_len begin with (q_start
+// counts tokens of the whole step, as qkv, out and `slots` do); `slots` and `keep_first` as pae_paged_attention_any_mass (attention_mass.cu) takes them.
 PAE_EXPORT int pae_paged_attention_few_mass(void* out, const void* qkv, const void* keys, const void* values, float* mass, long long pages, const int* block_table,
                                             int table_width, const int* q_start, const int* q_pos0, const int* kv_len, const int* slots, int tokens, int seqs,
                                             int heads, int kv_heads, int d, int page_size, int max_q_len, int max_kv_len, float scale, int keep_first,
@@ -1097,6 +1109,7 @@ PAE_EXPORT int pae_paged_attention_few_mass(void* out, const void* qkv, const vo
   p.error = error;
   p.span = p.own_slices * p.own_keys;
   p.scores = scratch;                                    // rows of a multiple of 64 floats
+  p.part_tokens = tokens;
   p.part_out = scratch + (size_t)tokens * heads * p.span;
   p.part_max = p.part_out + (size_t)tokens * heads * p.slots * d;
   p.part_sum = p.part_max + (size_t)tokens * heads * p.slots;

@@ -2496,6 +2496,27 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
 MASS_FEW_TOKENS = 16
 
 
+# Of the weights' scratch, which follows from the longest context: beyond it a step's requests go by parts, one after the other. us a pass whole, and by parts of
+# 1 GB, 512 and 256 MB at most: 64 requests of five tokens, 40 heads over 8 of 128, over 32,768 keys (1.9 GB) 2,332, 2,563, 2,611 and 2,938, over 20 to
+# 2,000 and one of 40,000 (2.3 GB) 436, 525, 623 and 877; 256 single tokens, 28 heads over 4, over 20 to 2,000 and one of 100,000 (2.7 GB) 2,372, 1,618, 1,458 and 1,841.
+MASS_SCRATCH_BYTES = 1 << 30
+
+
+def _mass_parts(limit: int, seqs: int, floats_of, most: int = 65535) -> tuple[list[tuple[int, int]], int]:
+    """The requests of a step in parts of as many as a launch takes (`most`) and `limit` bytes hold, floats_of(count) floats for so many; one at least:
+    ([(first request, count), ...], floats of scratch)."""
+    count = min(seqs, most)
+    while count > 1 and 4 * floats_of(count) > limit:
+        count = (count + 1) // 2
+    parts = [(b, min(count, seqs - b)) for b in range(0, seqs, count)]
+    return parts, max(floats_of(count), floats_of(parts[-1][1]))
+
+
+def _tokens_of_part(tokens: int, seqs: int, count: int, max_q_len: int) -> int:
+    """What `count` of a step's requests bring at most."""
+    return tokens if count == seqs else min(tokens, count * max_q_len)
+
+
 @functools.lru_cache(maxsize=64)
 def _prompt_mass_supports(*sizes) -> bool:
     return bool(_lib("attention_mass_prompt").pae_attention_mass_prompt_supports(*sizes))
@@ -2506,16 +2527,29 @@ def _few_mass_floats(*sizes) -> int:
     return _lib("attention_prefix").pae_attention_few_mass_floats(*sizes)
 
 
-def _few_mass(out, qkv, keys, operands, mass, pages: int, block_table, table_width: int, q_start, q_pos0, kv_len, slots, tokens: int, seqs: int, sizes,
+@functools.lru_cache(maxsize=1024)
+def _few_mass_parts(limit: int, tokens: int, seqs: int, sizes, max_q_len: int, max_kv_len: int):
+    """`_mass_parts` of a step of few tokens; none where `limit` does not hold one request's scores."""
+    def floats_of(count):
+        return _few_mass_floats(_tokens_of_part(tokens, seqs, count, max_q_len), count, *sizes, max_q_len, max_kv_len)
+
+    parts, most = _mass_parts(limit, seqs, floats_of)
+    return (parts, most) if 4 * most <= limit else None
+
+
+def _few_mass(out, qkv, keys, operands, mass, taken, pages: int, block_table, table_width: int, q_start, q_pos0, kv_len, slots, tokens: int, seqs: int, sizes,
               max_q_len: int, max_kv_len: int, scale: float, keep_first: int) -> None:
-    """A step whose requests bring few tokens: `out`, and the keys' weights."""
+    """A step whose requests bring few tokens, in the parts `taken`: `out`, and the keys' weights."""
     lib = _lib("attention_prefix")
-    scratch = qkv.new_empty(2 * _few_mass_floats(tokens, seqs, *sizes, max_q_len, max_kv_len))            # bfloat16
+    parts, most = taken
+    scratch = qkv.new_empty(2 * most)                     # bfloat16
     if bounds_checked:
         _set_bounds("attention_prefix", keys)
-    _check(lib, lib.pae_paged_attention_few_mass(
-        out.data_ptr(), *operands, mass.data_ptr(), pages, block_table.data_ptr(), table_width, q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(),
-        _ptr(slots), tokens, seqs, *sizes, max_q_len, max_kv_len, scale, keep_first, scratch.data_ptr(), _error_flag(qkv.device).data_ptr(), _stream()), 2)
+    for b, count in parts:
+        _check(lib, lib.pae_paged_attention_few_mass(
+            out.data_ptr(), *operands, mass.data_ptr(), pages, block_table.data_ptr() + 4 * b * table_width, table_width, q_start.data_ptr() + 4 * b,
+            q_pos0.data_ptr() + 4 * b, kv_len.data_ptr() + 4 * b, _ptr(slots), _tokens_of_part(tokens, seqs, count, max_q_len), count, *sizes, max_q_len, max_kv_len, scale,
+            keep_first, scratch.data_ptr(), _error_flag(qkv.device).data_ptr(), _stream()), 2)
 
 
 @functools.lru_cache(maxsize=64)
@@ -2542,6 +2576,23 @@ def _any_slicing(seqs: int, num_heads: int, num_kv_heads: int, head_dim: int, ma
     return slice_keys, max_slices, _lib("attention_mass").pae_decode_mass_floats(seqs, num_heads, head_dim, slice_keys, max_slices)
 
 
+@functools.lru_cache(maxsize=1024)
+def _decode_mass_parts(limit: int, singles: int, seqs: int, num_heads: int, num_kv_heads: int, head_dim: int, max_kv_len: int):
+    """`_mass_parts` of single tokens, each with its (keys per slice, slices)."""
+    def slicing(count):
+        return _mass_slicing(min(singles, count), count, num_heads, num_kv_heads, head_dim, max_kv_len)
+
+    parts, most = _mass_parts(limit, seqs, lambda count: slicing(count)[2])
+    return [(b, count, *slicing(count)[:2]) for b, count in parts], most
+
+
+@functools.lru_cache(maxsize=1024)
+def _any_mass_parts(limit: int, seqs: int, *sizes):
+    """The same on CUDA cores."""
+    parts, most = _mass_parts(limit, seqs, lambda count: _any_slicing(count, *sizes)[2])
+    return [(b, count, *_any_slicing(count, *sizes)[:2]) for b, count in parts], most
+
+
 _MASS_TENSORS = (*_STEP_TENSORS, "mass", "slots")
 
 
@@ -2550,13 +2601,14 @@ def _decode_mass(out, qkv, keys, operands, mass, block_table, table_width: int, 
     """The requests of a step that bring one token: their rows of `out`, and their keys' weights."""
     num_heads, num_kv_heads, head_dim, page_size = sizes
     lib = _lib("attention_mass")
-    slice_keys, max_slices, floats = _mass_slicing(singles, seqs, num_heads, num_kv_heads, head_dim, max_kv_len)
-    scratch = qkv.new_empty(2 * floats)                   # bfloat16
+    parts, most = _decode_mass_parts(MASS_SCRATCH_BYTES, singles, seqs, num_heads, num_kv_heads, head_dim, max_kv_len)
+    scratch = qkv.new_empty(2 * most)                     # bfloat16
     if bounds_checked:
         _set_bounds("attention_mass", keys)
-    _check(lib, lib.pae_paged_attention_decode_mass(
-        out.data_ptr(), *operands, mass.data_ptr(), block_table.data_ptr(), table_width, q_start.data_ptr(), kv_len.data_ptr(), _ptr(slots), seqs, num_heads,
-        num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices, scratch.data_ptr(), _stream()), 2)
+    for b, count, slice_keys, max_slices in parts:
+        _check(lib, lib.pae_paged_attention_decode_mass(
+            out.data_ptr(), *operands, mass.data_ptr(), block_table.data_ptr() + 4 * b * table_width, table_width, q_start.data_ptr() + 4 * b, kv_len.data_ptr() + 4 * b,
+            _ptr(slots), count, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices, scratch.data_ptr(), _stream()), 2)
 
 
 def _prompt_mass(lib, out, qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, slots, sizes, max_q_len: int, max_kv_len: int, scale: float,
@@ -2571,7 +2623,8 @@ def _prompt_mass(lib, out, qkv, keys, values, mass, block_table, q_start, q_pos0
             raise KernelError(f"paged_attention_mass: {listed.numel()} requests listed, {seqs - singles} bring more than one token")
     attention = _lib("attention_tcgen05")
     logarithms = torch.empty((tokens, num_heads), dtype=torch.float32, device=qkv.device)
-    scratch = torch.empty(lib.pae_attention_mass_prompt_floats(seqs, num_heads, num_kv_heads, max_q_len, max_kv_len), dtype=torch.float32, device=qkv.device)
+    parts, most = _mass_parts(MASS_SCRATCH_BYTES, seqs, lambda count: lib.pae_attention_mass_prompt_floats(count, num_heads, num_kv_heads, max_q_len, max_kv_len), 65535 // num_kv_heads)
+    scratch = torch.empty(most, dtype=torch.float32, device=qkv.device)
     error = _error_flag(qkv.device).data_ptr()
     _set_bounds("attention_tcgen05", keys)
     _set_bounds("attention_mass_prompt", keys)
@@ -2579,10 +2632,11 @@ def _prompt_mass(lib, out, qkv, keys, values, mass, block_table, q_start, q_pos0
         out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), keys.shape[0], block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
         q_pos0.data_ptr(), kv_len.data_ptr(), tokens, seqs, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, 0, 1, singles, 0, None,
         _ptr(listed), (listed.numel() if listed is not None else 0), logarithms.data_ptr(), error, _stream()))
-    _check(lib, lib.pae_attention_mass_prompt(
-        out.data_ptr(), mass.data_ptr(), qkv.data_ptr(), keys.data_ptr(), keys.shape[0], logarithms.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
-        q_pos0.data_ptr(), kv_len.data_ptr(), _ptr(slots), tokens, seqs, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first,
-        scratch.data_ptr(), error, _stream()), 2)
+    for b, count in parts:
+        _check(lib, lib.pae_attention_mass_prompt(
+            out.data_ptr(), mass.data_ptr(), qkv.data_ptr(), keys.data_ptr(), keys.shape[0], logarithms.data_ptr(), block_table.data_ptr() + 4 * b * block_table.shape[1],
+            block_table.shape[1], q_start.data_ptr() + 4 * b, q_pos0.data_ptr() + 4 * b, kv_len.data_ptr() + 4 * b, _ptr(slots), tokens, count, max_q_len, max_kv_len, num_heads,
+            num_kv_heads, head_dim, page_size, scale, keep_first, scratch.data_ptr(), error, _stream()), 2)
 
 
 def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -2616,11 +2670,13 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
     singles = num_single if num_single is not None else (seqs if max_q_len == 1 else -1)
     sizes = (num_heads, num_kv_heads, head_dim, page_size)
     if qkv.dtype is torch.bfloat16 and use_tensor_cores and max_q_len > 0:
-        few = 1 < max_q_len <= MASS_FEW_TOKENS and _prefix_supports(*sizes)
+        few = None
+        if 1 < max_q_len <= MASS_FEW_TOKENS and _prefix_supports(*sizes):
+            few = _few_mass_parts(MASS_SCRATCH_BYTES, tokens, seqs, sizes, max_q_len, max_kv_len)
         if few or (_mass_supports(*sizes) and (max_q_len == 1 or (use_tcgen05_attention and _prompt_mass_supports(*sizes)))):
             out = qkv.new_empty((tokens, num_heads * head_dim))
             if few:
-                _few_mass(out, qkv, keys, operands, mass, pages, block_table, table_width, q_start, q_pos0, kv_len, slots, tokens, seqs, sizes, max_q_len,
+                _few_mass(out, qkv, keys, operands, mass, few, pages, block_table, table_width, q_start, q_pos0, kv_len, slots, tokens, seqs, sizes, max_q_len,
                           max_kv_len, scale, keep_first)
                 return out
             if max_q_len > 1:
@@ -2632,26 +2688,28 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
             return out
     if max_q_len == 1 and head_dim % 4 == 0 and head_dim <= 256 and num_heads // num_kv_heads <= 16 and not (
             operands[0] | operands[1] | operands[2]) & (4 * qkv.element_size() - 1):
-        slice_keys, max_slices, floats = _any_slicing(seqs, num_heads, num_kv_heads, head_dim, max_kv_len)
-        out = qkv.new_empty((tokens, num_heads * head_dim))
-        scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device)
         lib = _lib("attention_mass")
+        out = qkv.new_empty((tokens, num_heads * head_dim))
+        parts, most = _any_mass_parts(MASS_SCRATCH_BYTES, seqs, num_heads, num_kv_heads, head_dim, max_kv_len)
+        scratch = torch.empty(most, dtype=torch.float32, device=qkv.device)
         if bounds_checked:
             _set_bounds("attention_mass", keys)
-        _check(lib, lib.pae_paged_attention_any_mass(
-            out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), mass.data_ptr(), block_table.data_ptr(), block_table.shape[1],
-            q_start.data_ptr(), kv_len.data_ptr(), _ptr(slots), seqs, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices,
-            _code(qkv), scratch.data_ptr(), _stream()), 2)
+        for b, count, slice_keys, max_slices in parts:
+            _check(lib, lib.pae_paged_attention_any_mass(
+                out.data_ptr(), *operands, mass.data_ptr(), block_table.data_ptr() + 4 * b * table_width, table_width, q_start.data_ptr() + 4 * b, kv_len.data_ptr() + 4 * b,
+                _ptr(slots), count, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices, _code(qkv), scratch.data_ptr(), _stream()), 2)
         return out
     out = paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_kv_len, scale,
                           0, num_single=num_single, multi_index=multi_index)
     lib = _lib("attention_mass")
-    scratch = torch.empty(lib.pae_attention_mass_floats(tokens, seqs, num_heads, num_kv_heads, max_q_len, max_kv_len), dtype=torch.float32, device=qkv.device)
+    parts, most = _mass_parts(MASS_SCRATCH_BYTES, seqs, lambda count: lib.pae_attention_mass_floats(tokens, count, num_heads, num_kv_heads, max_q_len, max_kv_len))
+    scratch = torch.empty(most, dtype=torch.float32, device=qkv.device)
     _set_bounds("attention_mass", keys)
-    _check(lib, lib.pae_attention_mass_rows(
-        mass.data_ptr(), qkv.data_ptr(), keys.data_ptr(), block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(),
-        _ptr(slots), tokens, seqs, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, _code(qkv), scratch.data_ptr(),
-        _stream()), 2)
+    for b, count in parts:
+        _check(lib, lib.pae_attention_mass_rows(
+            mass.data_ptr(), operands[0], operands[1], block_table.data_ptr() + 4 * b * table_width, table_width, q_start.data_ptr() + 4 * b, q_pos0.data_ptr() + 4 * b,
+            kv_len.data_ptr() + 4 * b, _ptr(slots), tokens, count, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, _code(qkv),
+            scratch.data_ptr(), _stream()), 3)
     return out
 
 

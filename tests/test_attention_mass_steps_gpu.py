@@ -66,3 +66,44 @@ def test_a_key_that_is_no_number(ops, dtype, dim, tokens):
     assert torch.equal(mass.isnan(), broken)
     assert ((mass - expected)[~broken].abs() <= MASS_RTOL * expected[~broken] + MASS_ATOL).all()
     assert torch.equal(out.isnan(), step.attention().isnan())
+
+
+@pytest.mark.parametrize("tokens,heads,kv_heads,longest", [
+    ([1] * 64, 40, 8, 9000),                                    # slices of single tokens
+    ([5] * 64, 40, 8, 9000),                                    # few tokens
+    ([16] + [1 + 5 * b % 16 for b in range(63)], 40, 8, 9000),
+    ([16] * 6, 128, 1, 9000),                                   # one request's scores alone are beyond the limit
+    ([20] + [17] * 300, 8, 8, 9000),                            # portions
+    ([1] * 64, 17, 1, 40000),                                    # more query heads than the slices of single tokens take
+])
+def test_scratch_has_a_bound(ops, monkeypatch, tokens, heads, kv_heads, longest):
+    """One long context among many short ones: what a call takes beside its operands and results stays below the limit, in requests by parts."""
+    monkeypatch.setattr(ops, "MASS_SCRATCH_BYTES", 64 << 20, raising=False)
+    lengths = [longest] + [max(t, 20 + 37 * b % 300) for b, t in enumerate(tokens[1:])]
+    step = Step(lengths, tokens, heads, kv_heads, 128, 64, BF16, 3)
+    pools, tables = step.on()
+    mass = step.mass.cuda()
+    run = lambda: ops.paged_attention_mass(*pools, mass, *tables, *step.sizes, *step.longest, step.scale)
+    out = run()
+    got = mass.clone()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    again = run()
+    torch.cuda.synchronize()
+    beside = torch.cuda.max_memory_allocated() - before - 2 * again.numel()
+    ops.check_device_errors()
+    assert beside <= ops.MASS_SCRATCH_BYTES + (4 << 20)
+    del again
+    # The requests of the first and the last part against the definition.
+    start = step.q_start.tolist()
+    for b in (0, 1, len(tokens) - 1):
+        w = step.weights(b)
+        v = step.rows(step.values, b).double().repeat_interleave(heads // kv_heads, 0)
+        want = (w @ v).transpose(0, 1).flatten(1)
+        assert (out[start[b] : start[b + 1]].cpu().double() - want).abs().max() <= output_tolerance(BF16, want)
+        n, t = lengths[b], tokens[b]
+        j = torch.arange(n)
+        p, o = step.table[b].long()[j // 64], j % 64
+        expected = torch.where(j[:, None] >= n - t, 0.0, step.mass[p, :, o].double()) + w.sum(1).view(kv_heads, -1, n).sum(1).T
+        assert ((got.cpu()[p, :, o].double() - expected).abs() <= MASS_RTOL * expected + MASS_ATOL).all()
