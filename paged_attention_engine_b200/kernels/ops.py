@@ -2391,6 +2391,10 @@ PREFIX_ATTENTION_MAX_TOKENS = 64
 # 2 requests behind 200 keys 15 and 8, 16 behind 1,000 20.3 and 19.5, 64 behind 2,000 56 and 92, 4 behind 8,000 35 and 106; 32 of 28 heads over 4 of 128
 # behind 4,000 293 and 416.
 PREFIX_SIMT_MIN_KEYS = 1024
+# Of the scratch, a row's output for each of its slices; a step that would take more has each request read its keys by itself, which takes none. us a pass
+# shared and by itself, and MB that the former takes: 64 requests of 64 tokens, 40 heads over 8 of 128, behind 8,000 keys, own 1,000 to 32,000: 3,526 and 3,673, 3,534 MB; 1,000 to
+# 8,000: 1,782 and 1,777, 1,015 MB; 512 requests of 16 tokens, own 16 to 2,000: 2,125 and 19,520, 730 MB.
+PREFIX_SCRATCH_BYTES = 1 << 32
 
 
 _PREFIX_TENSORS = (*_STEP_TENSORS, "prefix_len", "group_start")
@@ -2427,7 +2431,7 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     keys behind them. `info`, when given, receives which kernel ran ("kernel"): "shared", on tensor cores (bfloat16, head sizes 64 and 128, pages
     of 16, 32, 64 or 128 keys), "shared simt" (long prefixes in float32 and of what no tensor-core attention takes; head sizes that are multiples of 4 up
     to 256), or what
-    `paged_attention` says where each request reads its keys by itself (other sizes, long portions, groups of one request).
+    `paged_attention` says where each request reads its keys by itself (other sizes, long portions, groups of one request, steps whose scratch would be too large).
     This attention adds no weights. With `mass` (as `paged_attention_mass` keeps it; `slots` as there) the step's keys start from nothing in it, so that a later
     step's weights are added to 0 and not to what the page's earlier owner left."""
     qkv = materialized(qkv)
@@ -2468,6 +2472,10 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
         elif max_prefix_len >= PREFIX_SIMT_MIN_KEYS and head_dim % 4 == 0 and head_dim <= 256 and not plain_attention_takes(num_heads, num_kv_heads, head_dim, page_size, qkv.dtype) and not (
                 operands[0] | operands[1] | operands[2]) & (4 * qkv.element_size() - 1):
             form = "shared simt"
+    if form is not None:
+        floats = _prefix_floats(*sizes, 0 if form == "shared" else 1)
+        if 4 * floats > PREFIX_SCRATCH_BYTES:
+            form = None
     if form is None:
         return paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len,
                                min(max_prefix_len + max_own_len, table_width * page_size), scale, 0, num_single=num_single, info=info)
@@ -2478,12 +2486,12 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     if bounds_checked:
         _set_bounds("attention_prefix", keys)
     if form == "shared":
-        scratch = qkv.new_empty(2 * _prefix_floats(*sizes, 0))            # bfloat16
+        scratch = qkv.new_empty(2 * floats)               # bfloat16
         _check(lib, lib.pae_paged_attention_prefix(
             out.data_ptr(), *operands, pages, block_table.data_ptr(), table_width, q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(),
             prefix_len.data_ptr(), group_start.data_ptr(), *sizes, scale, scratch.data_ptr(), _error_flag(qkv.device).data_ptr(), _stream()), 2)
         return out
-    scratch = torch.empty(_prefix_floats(*sizes, 1), dtype=torch.float32, device=qkv.device)
+    scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device)
     _check(lib, lib.pae_paged_attention_prefix_any(
         out.data_ptr(), *operands, block_table.data_ptr(), table_width, q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(), prefix_len.data_ptr(),
         group_start.data_ptr(), *sizes, scale, _code(qkv), scratch.data_ptr(), _stream()), 2)
