@@ -16,7 +16,7 @@
 //                   heads a kv head): a block takes 64 keys a tile, one thread per key and half of the rows for the scores, one per four channels and a share
 //                   of the keys for the output.
 //   stats, columns  every other step: the rows' maxima and sums over runs of keys, then per tile of keys and chunk of rows the
-//                   weights, from scores that are computed again, and the chunks' sums in their order. CUDA cores, any type and head size. (Steps of several tokens in
+//                   weights, from scores that are computed again, and the chunks' sums in their order. CUDA cores, any type and head size that is a multiple of 4 up to 256. (Steps of several tokens in
 //                   bfloat16 go to attention_prefix.cu and attention_mass_prompt.cu where those take their sizes.)
 #include "attention_mma.cuh"
 
@@ -440,27 +440,17 @@ struct RowParams {
   float scale_log2;
 };
 
-// Elements c .. c + 3 of a row of d: zeros behind the last. (Rows of a multiple of four start on a boundary of four: `vector`.)
-template <typename T>
-__device__ __forceinline__ float4 load4_of(const T* row, int c, int d, bool vector) {
-  if (vector) return load4(row + c);
-  float v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = c + i < d ? to_float<T>(row[c + i]) : 0.f;
-  return make_float4(v[0], v[1], v[2], v[3]);
-}
-
 // Rows 0 .. rows - 1 of a tile, row r from row_ptr(r) (null: zeros), `stride` floats each.
 template <typename T, typename RowPtr>
-__device__ __forceinline__ void load_tile(float* tile, int rows, int d, int stride, bool vector, RowPtr row_ptr) {
-  const int units = (d + 3) / 4;
+__device__ __forceinline__ void load_tile(float* tile, int rows, int d, int stride, RowPtr row_ptr) {
+  const int units = d / 4;
   for (int i0 = threadIdx.x; i0 < rows * units; i0 += ANY_THREADS * AT_ONCE) {
     float4 v[AT_ONCE];
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
       const int i = i0 + u * ANY_THREADS;
       const T* from = i < rows * units ? row_ptr(i / units) : nullptr;
-      v[u] = from != nullptr ? load4_of<T>(from, (i % units) * 4, d, vector) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[u] = from != nullptr ? load4(from + (i % units) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
@@ -501,7 +491,7 @@ __device__ __forceinline__ const T* query_row(const RowParams<T>& p, int token0,
 __device__ __forceinline__ int seen_by(int row0, int count, int groups, int pos0, int n) { return min(n, pos0 + (min(row0 + ROWS, count) - 1) / groups + 1); }
 
 template <typename T>
-__global__ void __launch_bounds__(ANY_THREADS) row_stats_kernel(const RowParams<T> p, bool vector) {
+__global__ void __launch_bounds__(ANY_THREADS) row_stats_kernel(const RowParams<T> p) {
   extern __shared__ __align__(16) float shared[];
   __shared__ float tops[2][2][ROWS / 2], sums[2][2][ROWS / 2];       // [half of the keys][parity of the row][row / 2]
   dependent_launch_prologue();
@@ -512,10 +502,10 @@ __global__ void __launch_bounds__(ANY_THREADS) row_stats_kernel(const RowParams<
   if (row0 >= count || pads(p.m, token0)) return;
   const int pos0 = p.q_pos0[b], visible = seen_by(row0, count, groups, pos0, p.m.kv_len[b]);
   const int begin = run * p.run_keys, end = min(visible, begin + p.run_keys);
-  const int stride = (p.d + 3) / 4 * 4 + 4, key = threadIdx.x % ANY_KEYS, half = threadIdx.x / ANY_KEYS, lane = threadIdx.x & 31;
+  const int stride = p.d + 4, key = threadIdx.x % ANY_KEYS, half = threadIdx.x / ANY_KEYS, lane = threadIdx.x & 31;
   float* q_tile = shared;
   float* k_tile = shared + ROWS * stride;
-  load_tile<T>(q_tile, ROWS, p.d, stride, vector, [&](int r) -> const T* { return row0 + r < count ? query_row(p, token0, g, groups, row0 + r) : nullptr; });
+  load_tile<T>(q_tile, ROWS, p.d, stride, [&](int r) -> const T* { return row0 + r < count ? query_row(p, token0, g, groups, row0 + r) : nullptr; });
   float top[ROWS / 2], sum[ROWS / 2];
 #pragma unroll
   for (int i = 0; i < ROWS / 2; ++i) {
@@ -524,7 +514,7 @@ __global__ void __launch_bounds__(ANY_THREADS) row_stats_kernel(const RowParams<
   }
   for (int key0 = begin; key0 < end; key0 += ANY_KEYS) {
     __syncthreads();
-    load_tile<T>(k_tile, ANY_KEYS, p.d, stride, vector, [&](int r) -> const T* { return key0 + r < end ? key_row(p, b, g, key0 + r) : nullptr; });
+    load_tile<T>(k_tile, ANY_KEYS, p.d, stride, [&](int r) -> const T* { return key0 + r < end ? key_row(p, b, g, key0 + r) : nullptr; });
     __syncthreads();
     float s[ROWS / 2];
     eight_scores(s, q_tile, k_tile, p.d, stride, p.scale_log2);
@@ -581,7 +571,7 @@ __device__ __forceinline__ ChunkTiles chunk_tiles(const RowParams<T>& p, int b, 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(ANY_THREADS) any_column_sums_kernel(const RowParams<T> p, bool vector) {
+__global__ void __launch_bounds__(ANY_THREADS) any_column_sums_kernel(const RowParams<T> p) {
   extern __shared__ __align__(16) float shared[];
   __shared__ float logarithm[ROWS], halves[ANY_KEYS];
   dependent_launch_prologue();
@@ -589,15 +579,15 @@ __global__ void __launch_bounds__(ANY_THREADS) any_column_sums_kernel(const RowP
   const ChunkTiles tiles = chunk_tiles(p, b, key0, chunk);
   if (tiles.first >= tiles.last) return;
   const int groups = p.m.heads / p.m.kv_heads, token0 = p.m.q_start[b], count = tiles.tokens * groups;
-  const int stride = (p.d + 3) / 4 * 4 + 4, key = threadIdx.x % ANY_KEYS, half = threadIdx.x / ANY_KEYS, j = key0 + key;
+  const int stride = p.d + 4, key = threadIdx.x % ANY_KEYS, half = threadIdx.x / ANY_KEYS, j = key0 + key;
   float* q_tile = shared;
   float* k_tile = shared + ROWS * stride;
-  load_tile<T>(k_tile, ANY_KEYS, p.d, stride, vector, [&](int r) -> const T* { return key0 + r < tiles.n ? key_row(p, b, g, key0 + r) : nullptr; });
+  load_tile<T>(k_tile, ANY_KEYS, p.d, stride, [&](int r) -> const T* { return key0 + r < tiles.n ? key_row(p, b, g, key0 + r) : nullptr; });
   float sum = 0.f;
   for (int tile = tiles.first; tile < tiles.last; ++tile) {
     const int row0 = tile * ROWS;
     __syncthreads();
-    load_tile<T>(q_tile, ROWS, p.d, stride, vector, [&](int r) -> const T* { return row0 + r < count ? query_row(p, token0, g, groups, row0 + r) : nullptr; });
+    load_tile<T>(q_tile, ROWS, p.d, stride, [&](int r) -> const T* { return row0 + r < count ? query_row(p, token0, g, groups, row0 + r) : nullptr; });
     if (threadIdx.x < ROWS && row0 + (int)threadIdx.x < count) {
       const int i = row0 + threadIdx.x;
       const size_t at = (size_t)(token0 + i / groups) * p.m.heads + g * groups + i % groups;
@@ -673,15 +663,14 @@ RowCut cut_rows(int seqs, int heads, int kv_heads, int max_q_len, int max_kv_len
 
 template <typename T>
 int launch_rows(RowParams<T> p, const RowCut& c, int max_kv_len, cudaStream_t s) {
-  const size_t bytes = (size_t)(ROWS + ANY_KEYS) * ((p.d + 3) / 4 * 4 + 4) * sizeof(float);
-  const bool vector = p.d % 4 == 0 && (((uintptr_t)p.qkv | (uintptr_t)p.keys) & (4 * sizeof(T) - 1)) == 0;
+  const size_t bytes = (size_t)(ROWS + ANY_KEYS) * (p.d + 4) * sizeof(float);
   static DevicesSet stats_devices, column_devices;
-  if (int err = raise_shared_memory(stats_devices, row_stats_kernel<T>, 200 * 1024, "attention_mass")) return err;
-  if (int err = raise_shared_memory(column_devices, any_column_sums_kernel<T>, 200 * 1024, "attention_mass")) return err;
+  if (int err = raise_shared_memory(stats_devices, row_stats_kernel<T>, (ROWS + ANY_KEYS) * 260 * sizeof(float), "attention_mass")) return err;
+  if (int err = raise_shared_memory(column_devices, any_column_sums_kernel<T>, (ROWS + ANY_KEYS) * 260 * sizeof(float), "attention_mass")) return err;
   const int key_tiles = (max_kv_len + ANY_KEYS - 1) / ANY_KEYS;
-  launch_kernel(row_stats_kernel<T>, dim3(c.row_tiles * c.runs, p.m.kv_heads, p.seqs), dim3(ANY_THREADS), bytes, s, p, vector);
+  launch_kernel(row_stats_kernel<T>, dim3(c.row_tiles * c.runs, p.m.kv_heads, p.seqs), dim3(ANY_THREADS), bytes, s, p);
   if (int err = check_launch("attention_mass")) return err;
-  launch_kernel(any_column_sums_kernel<T>, dim3(key_tiles, p.m.kv_heads * c.chunks, p.seqs), dim3(ANY_THREADS), bytes, s, p, vector);
+  launch_kernel(any_column_sums_kernel<T>, dim3(key_tiles, p.m.kv_heads * c.chunks, p.seqs), dim3(ANY_THREADS), bytes, s, p);
   if (int err = check_launch("attention_mass")) return err;
   launch_kernel(add_chunks_kernel<T>, dim3(key_tiles, p.m.kv_heads, p.seqs), dim3(ANY_KEYS), 0, s, p, c.chunks);
   return check_launch("attention_mass");
@@ -791,12 +780,13 @@ PAE_EXPORT long long pae_attention_mass_floats(int tokens, int seqs, int heads, 
   return 2ll * c.runs * tokens * heads + (long long)c.chunks * seqs * kv_heads * max_kv_len;
 }
 
-// The weights of any step's keys, whatever its rows, type (0 float32, 1 bfloat16) and head size; the attention's output is not computed.
+// The weights of any step's keys, whatever its rows, type (0 float32, 1 bfloat16) and head size (a multiple of 4 up to 256); the attention's output is not computed.
 PAE_EXPORT int pae_attention_mass_rows(float* mass, const void* qkv, const void* keys, const int* block_table, int table_width, const int* q_start,
                                        const int* q_pos0, const int* kv_len, const int* slots, int tokens, int seqs, int max_q_len, int max_kv_len, int heads,
                                        int kv_heads, int d, int page_size, float scale, int keep_first, int dtype, float* scratch, void* stream) {
   if (seqs < 1 || tokens < 1 || max_q_len < 1 || max_kv_len < 1) return 0;
-  if (d < 1 || d > 512) return fail(2, "paged_attention_mass: head_dim %d is not 1 to 512", d);
+  if (d < 4 || d > 256 || d % 4) return fail(2, "paged_attention_mass: head_dim %d is not a multiple of 4 up to 256", d);
+  if (((uintptr_t)qkv | (uintptr_t)keys) & (dtype == kF32 ? 15 : 7)) return fail(2, "paged_attention_mass: an operand does not start on a boundary of four elements");
   const RowCut c = cut_rows(seqs, heads, kv_heads, max_q_len, max_kv_len);
   if ((long long)kv_heads * c.chunks > 65535 || seqs > 65535 || (long long)c.row_tiles * c.runs > 0x7fffffffll)
     return fail(1, "paged_attention_mass: %d requests of %d kv heads x %d chunks exceed one launch", seqs, kv_heads, c.chunks);

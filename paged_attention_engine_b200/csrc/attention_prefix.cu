@@ -863,7 +863,7 @@ __global__ void __launch_bounds__(ANY_THREADS) any_merge_kernel(const AnyOperand
   const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
   const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = tokens_of(p, b);
   if (i >= tokens) return;
-  const int slices = slices_of<ANY_ROWS>(p, min(p.prefix_len[b], p.max_prefix), p.kv_len[b], p.q_pos0[b], tokens, i, h % groups);
+  const int slices = slices_of<ANY_ROWS>(p, p.max_prefix > 0 ? min(p.prefix_len[b], p.max_prefix) : 0, p.kv_len[b], p.q_pos0[b], tokens, i, h % groups);
   const size_t row = (size_t)(token0 + i) * p.heads + h, at = row * p.slots;
   float top = -FLT_MAX, total = 0.f;
   for (int s = lane; s < slices; s += 32) top = fmaxf(top, p.part_max[at + s]);           // every warp works them out for itself
@@ -1061,7 +1061,8 @@ PAE_EXPORT int pae_paged_attention_prefix(void* out, const void* qkv, const void
   return launch<128>(p, out, pages, (int)blocks, seqs, max_q_len, (cudaStream_t)stream);
 }
 
-// The same on CUDA cores: dtype 0 float32, 1 bfloat16; head sizes that are multiples of 4 up to 256, pages of any size.
+// The same on CUDA cores: dtype 0 float32, 1 bfloat16; head sizes that are multiples of 4 up to 256, pages of any size. max_prefix 0: nothing is shared, and
+// prefix_len and group_start are not read.
 PAE_EXPORT int pae_paged_attention_prefix_any(void* out, const void* qkv, const void* keys, const void* values, const int* block_table, int table_width,
                                               const int* q_start, const int* q_pos0, const int* kv_len, const int* prefix_len, const int* group_start, int tokens,
                                               int seqs, int groups, int heads, int kv_heads, int d, int page_size, int max_q_len, int max_prefix, int max_own,

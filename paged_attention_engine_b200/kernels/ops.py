@@ -2391,6 +2391,8 @@ PREFIX_ATTENTION_MAX_TOKENS = 64
 # 2 requests behind 200 keys 15 and 8, 16 behind 1,000 20.3 and 19.5, 64 behind 2,000 56 and 92, 4 behind 8,000 35 and 106; 32 of 28 heads over 4 of 128
 # behind 4,000 293 and 416.
 PREFIX_SIMT_MIN_KEYS = 1024
+# (Heads that `paged_attention` does not take go this way in every step. A threshold of PREFIX_SIMT_NEVER keeps the kernel out of use, of these too: tests.)
+PREFIX_SIMT_NEVER = 1 << 30
 # Of the scratch, a row's output for each of its slices; a step that would take more has each request read its keys by itself, which takes none. us a pass
 # shared and by itself, and MB that the former takes: 64 requests of 64 tokens, 40 heads over 8 of 128, behind 8,000 keys, own 1,000 to 32,000: 3,526 and 3,673, 3,534 MB; 1,000 to
 # 8,000: 1,782 and 1,777, 1,015 MB; 512 requests of 16 tokens, own 16 to 2,000: 2,125 and 19,520, 730 MB.
@@ -2400,12 +2402,24 @@ PREFIX_SCRATCH_BYTES = 1 << 32
 _PREFIX_TENSORS = (*_STEP_TENSORS, "prefix_len", "group_start")
 
 
+def _need_head_dim(what: str, head_dim: int) -> None:
+    """The head sizes that the attentions of this part take, whatever a step's lengths are."""
+    if head_dim % 4 or not 4 <= head_dim <= 256:
+        raise KernelError(f"{what}: head_dim {head_dim} is not a multiple of 4 in [4, 256]")
+
+
 def _aligned_operands(what: str, qkv, keys, values, head_dim: int) -> tuple[int, int, int]:
-    """Where the operands lie: on 16-byte boundaries wherever their rows are whole 16-byte pieces, which the kernels copy."""
+    """Where the operands lie: on 16-byte boundaries wherever their rows are whole 16-byte pieces, which the kernels copy, else of four elements."""
     operands = qkv.data_ptr(), keys.data_ptr(), values.data_ptr()
-    if (operands[0] | operands[1] | operands[2]) & 15 and head_dim * qkv.element_size() % 16 == 0:
-        raise KernelError(f"{what}: an operand does not start on a 16-byte boundary")
+    boundary = 16 if head_dim * qkv.element_size() % 16 == 0 else 8
+    if (operands[0] | operands[1] | operands[2]) & (boundary - 1):
+        raise KernelError(f"{what}: an operand does not start on {'a 16' if boundary == 16 else 'an 8'}-byte boundary")
     return operands
+
+
+def _plain_attention_takes_head(head_dim: int) -> bool:
+    """Whether `paged_attention` has a kernel for these heads, among those that are taken here."""
+    return head_dim % 8 == 0
 
 
 @functools.lru_cache(maxsize=64)
@@ -2429,8 +2443,8 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     request, and in the page that the prefix ends in, and wherever requests read by themselves, through their own. The result is that of `paged_attention` but for the order of the sums.
     The longest request brings at most `max_q_len` tokens, the largest group `max_group_tokens`; `max_prefix_len` and `max_own_len` bound the shared keys and the
     keys behind them. `info`, when given, receives which kernel ran ("kernel"): "shared", on tensor cores (bfloat16, head sizes 64 and 128, pages
-    of 16, 32, 64 or 128 keys), "shared simt" (long prefixes in float32 and of what no tensor-core attention takes; head sizes that are multiples of 4 up
-    to 256), or what
+    of 16, 32, 64 or 128 keys), "shared simt" (long prefixes in float32 and of what no tensor-core attention takes, and every step of heads that `paged_attention` does
+    not take: head sizes are multiples of 4 up to 256), or what
     `paged_attention` says where each request reads its keys by itself (other sizes, long portions, groups of one request, steps whose scratch would be too large).
     This attention adds no weights. With `mass` (as `paged_attention_mass` keeps it; `slots` as there) the step's keys start from nothing in it, so that a later
     step's weights are added to 0 and not to what the page's earlier owner left."""
@@ -2438,6 +2452,7 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     what = "paged_attention_prefix"
     tokens, seqs, table_width, pages = _need_attention(what, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim,
                                                        page_size)
+    _need_head_dim(what, head_dim)
     if prefix_len.dtype is not torch.int32 or group_start.dtype is not torch.int32:
         _int32(what, prefix_len=prefix_len, group_start=group_start)
     groups = group_start.numel() - 1
@@ -2457,8 +2472,8 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
     if mass is not None:
         _here(what, ("mass", "slots"), mass, *(() if slots is None else (slots,)))
     operands = _aligned_operands(what, qkv, keys, values, head_dim)
-    if tokens == 0:
-        return qkv.new_empty((0, num_heads * head_dim))
+    if tokens == 0 or max_q_len == 0:
+        return qkv.new_zeros((tokens, num_heads * head_dim))
     if mass is not None:
         lib = _lib("attention_mass")
         _set_bounds("attention_mass", keys)
@@ -2466,15 +2481,17 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
                                        num_kv_heads, page_size, _stream()))
     sizes = (tokens, seqs, groups, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_prefix_len, max_own_len, max_group_tokens)
     form = None
-    if 0 < max_q_len <= PREFIX_ATTENTION_MAX_TOKENS and max_prefix_len > 0 and max_group_tokens > max_q_len:
+    if not _plain_attention_takes_head(head_dim):
+        if PREFIX_SIMT_MIN_KEYS < PREFIX_SIMT_NEVER:
+            form = "shared simt"
+    elif max_q_len <= PREFIX_ATTENTION_MAX_TOKENS and max_prefix_len > 0 and max_group_tokens > max_q_len:
         if qkv.dtype is torch.bfloat16 and use_tensor_cores and _prefix_supports(num_heads, num_kv_heads, head_dim, page_size):
             form = "shared"
-        elif max_prefix_len >= PREFIX_SIMT_MIN_KEYS and head_dim % 4 == 0 and head_dim <= 256 and not plain_attention_takes(num_heads, num_kv_heads, head_dim, page_size, qkv.dtype) and not (
-                operands[0] | operands[1] | operands[2]) & (4 * qkv.element_size() - 1):
+        elif max_prefix_len >= PREFIX_SIMT_MIN_KEYS and not plain_attention_takes(num_heads, num_kv_heads, head_dim, page_size, qkv.dtype):
             form = "shared simt"
     if form is not None:
         floats = _prefix_floats(*sizes, 0 if form == "shared" else 1)
-        if 4 * floats > PREFIX_SCRATCH_BYTES:
+        if 4 * floats > PREFIX_SCRATCH_BYTES and _plain_attention_takes_head(head_dim):
             form = None
     if form is None:
         return paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len,
@@ -2664,6 +2681,7 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
     what = "paged_attention_mass"
     tokens, seqs, table_width, pages = _need_attention(what, qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim,
                                                        page_size)
+    _need_head_dim(what, head_dim)
     _need_mass(what, mass, slots, tokens, pages, num_kv_heads, page_size)
     if keep_first < 0:
         raise KernelError(f"paged_attention_mass: {keep_first} first keys")
@@ -2673,11 +2691,13 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
         raise KernelError(f"paged_attention_mass: {max_kv_len} keys for tables of {table_width} pages of {page_size}")
     _here(what, _MASS_TENSORS, qkv, keys, values, block_table, q_start, q_pos0, kv_len, mass, *(() if slots is None else (slots,)))
     operands = _aligned_operands(what, qkv, keys, values, head_dim)
-    if tokens == 0 or seqs == 0 or max_kv_len == 0:
+    if max_q_len < 0:
+        raise KernelError(f"{what}: requests of up to {max_q_len} tokens")
+    if tokens == 0 or seqs == 0 or max_kv_len == 0 or max_q_len == 0:
         return qkv.new_zeros((tokens, num_heads * head_dim))
     singles = num_single if num_single is not None else (seqs if max_q_len == 1 else -1)
     sizes = (num_heads, num_kv_heads, head_dim, page_size)
-    if qkv.dtype is torch.bfloat16 and use_tensor_cores and max_q_len > 0:
+    if qkv.dtype is torch.bfloat16 and use_tensor_cores:
         few = None
         if 1 < max_q_len <= MASS_FEW_TOKENS and _prefix_supports(*sizes):
             few = _few_mass_parts(MASS_SCRATCH_BYTES, tokens, seqs, sizes, max_q_len, max_kv_len)
@@ -2694,8 +2714,7 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
                 _decode_mass(out, qkv, keys, operands, mass, block_table, table_width, q_start, kv_len, slots, seqs, sizes, max_kv_len, scale, keep_first,
                              seqs if singles < 0 else singles)
             return out
-    if max_q_len == 1 and head_dim % 4 == 0 and head_dim <= 256 and num_heads // num_kv_heads <= 16 and not (
-            operands[0] | operands[1] | operands[2]) & (4 * qkv.element_size() - 1):
+    if max_q_len == 1 and num_heads // num_kv_heads <= 16:
         lib = _lib("attention_mass")
         out = qkv.new_empty((tokens, num_heads * head_dim))
         parts, most = _any_mass_parts(MASS_SCRATCH_BYTES, seqs, num_heads, num_kv_heads, head_dim, max_kv_len)
@@ -2707,8 +2726,11 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
                 out.data_ptr(), *operands, mass.data_ptr(), block_table.data_ptr() + 4 * b * table_width, table_width, q_start.data_ptr() + 4 * b, kv_len.data_ptr() + 4 * b,
                 _ptr(slots), count, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, slice_keys, max_slices, _code(qkv), scratch.data_ptr(), _stream()), 2)
         return out
-    out = paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_kv_len, scale,
-                          0, num_single=num_single, multi_index=multi_index)
+    if _plain_attention_takes_head(head_dim):
+        out = paged_attention(qkv, keys, values, block_table, q_start, q_pos0, kv_len, num_heads, num_kv_heads, head_dim, page_size, max_q_len, max_kv_len, scale,
+                              0, num_single=num_single, multi_index=multi_index)
+    else:
+        out = _attention_of_any_head(qkv, keys, operands, block_table, table_width, q_start, q_pos0, kv_len, tokens, seqs, sizes, max_q_len, max_kv_len, scale)
     lib = _lib("attention_mass")
     parts, most = _mass_parts(MASS_SCRATCH_BYTES, seqs, lambda count: lib.pae_attention_mass_floats(tokens, count, num_heads, num_kv_heads, max_q_len, max_kv_len))
     scratch = torch.empty(most, dtype=torch.float32, device=qkv.device)
@@ -2718,6 +2740,21 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
             mass.data_ptr(), operands[0], operands[1], block_table.data_ptr() + 4 * b * table_width, table_width, q_start.data_ptr() + 4 * b, q_pos0.data_ptr() + 4 * b,
             kv_len.data_ptr() + 4 * b, _ptr(slots), tokens, count, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, keep_first, _code(qkv),
             scratch.data_ptr(), _stream()), 3)
+    return out
+
+
+def _attention_of_any_head(qkv, keys, operands, block_table, table_width: int, q_start, q_pos0, kv_len, tokens: int, seqs: int, sizes, max_q_len: int, max_kv_len: int,
+                           scale: float) -> torch.Tensor:
+    """The attention of heads that `paged_attention` does not take: the one of shared prefixes on CUDA cores, with nothing shared."""
+    lib = _lib("attention_prefix")
+    sizes = (tokens, seqs, 1, *sizes, max_q_len, 0, max_kv_len, max_q_len)
+    out = qkv.new_empty((tokens, qkv.shape[1] * sizes[3] // (sizes[3] + 2 * sizes[4])))
+    scratch = torch.empty(_prefix_floats(*sizes, 1), dtype=torch.float32, device=qkv.device)
+    if bounds_checked:
+        _set_bounds("attention_prefix", keys)
+    _check(lib, lib.pae_paged_attention_prefix_any(
+        out.data_ptr(), *operands, block_table.data_ptr(), table_width, q_start.data_ptr(), q_pos0.data_ptr(), kv_len.data_ptr(), None, None, *sizes, scale, _code(qkv),
+        scratch.data_ptr(), _stream()), 2)
     return out
 
 
