@@ -46,6 +46,7 @@ struct Params {
   const int* slots;             // [tokens] or null: a request whose first slot is negative pads the step
   int table_width, heads, kv_heads, d, page_size, keep_first;
   int tile_tokens, chunk_tiles, span, seqs;
+  int least;                    // tokens of the requests that are taken: 2 where the kernel of single tokens takes the others, else 1
   float scale_log2;
   int* error;
 };
@@ -77,8 +78,7 @@ __device__ __forceinline__ Tiles tiles_of(const Params& p, int b, int key0, int 
   const int all = (t.tokens + p.tile_tokens - 1) / p.tile_tokens;
   t.first = max(chunk * p.chunk_tiles, max(0, key0 - t.pos0) / p.tile_tokens);
   t.last = min((chunk + 1) * p.chunk_tiles, all);
-  // Requests of one token are the decode kernel's.
-  if (t.tokens < 2 || key0 >= min(p.kv_len[b], t.pos0 + t.tokens) || key0 + KEYS <= p.keep_first || (p.slots != nullptr && p.slots[start] < 0)) t.last = t.first;
+  if (t.tokens < p.least || key0 >= min(p.kv_len[b], t.pos0 + t.tokens) || key0 + KEYS <= p.keep_first || (p.slots != nullptr && p.slots[start] < 0)) t.last = t.first;
   return t;
 }
 
@@ -286,12 +286,12 @@ __global__ void __launch_bounds__(KEYS) add_chunks_kernel(const Params p, int ch
   const int g = blockIdx.y, b = blockIdx.z, key0 = blockIdx.x * KEYS, j = key0 + threadIdx.x;
   Tiles tiles = tiles_of(p, b, key0, 0);
   const int n = min(p.kv_len[b], tiles.pos0 + tiles.tokens);
-  if (n <= 0 && key0 == 0 && tiles.tokens > 1) {      // a request without keys: the attention leaves its rows as they were
+  if (n <= 0 && key0 == 0 && tiles.tokens >= p.least) {      // a request without keys: the attention leaves its rows as they were
     const int pieces = p.heads / p.kv_heads * p.d / 8;                                // of 16 bytes, of a token's heads of g
     uint4* out = (uint4*)(p.out + (size_t)p.q_start[b] * p.heads * p.d) + g * pieces;
     for (int i = threadIdx.x; i < tiles.tokens * pieces; i += KEYS) out[(size_t)(i / pieces) * p.kv_heads * pieces + i % pieces] = make_uint4(0, 0, 0, 0);
   }
-  if (j < p.keep_first || j >= min(n, p.span) || tiles.tokens < 2 || (p.slots != nullptr && p.slots[p.q_start[b]] < 0)) return;
+  if (j < p.keep_first || j >= min(n, p.span) || tiles.tokens < p.least || (p.slots != nullptr && p.slots[p.q_start[b]] < 0)) return;
   float w = 0.f;
   for (int c = 0; c < chunks; ++c) {
     tiles = tiles_of(p, b, key0, c);
@@ -355,12 +355,12 @@ PAE_EXPORT long long pae_attention_mass_prompt_floats(int seqs, int heads, int k
   return (long long)chunk_count(seqs, kv_heads, max_q_len, max_kv_len, TILE / (heads / kv_heads)) * seqs * kv_heads * max_kv_len;
 }
 
-// Adds the weights of the requests that bring more than one token. `lse` [tokens, heads] is what the attention left of their rows,
+// Adds the weights of the requests that bring `least` (1 or 2) tokens and more. `lse` [tokens, heads] is what the attention left of their rows,
 // `out` its result, in which the rows of requests without keys become zeros.
 PAE_EXPORT int pae_attention_mass_prompt(void* out, float* mass, const void* qkv, const void* keys, long long pages, const float* lse, const int* block_table,
                                          int table_width, const int* q_start, const int* q_pos0, const int* kv_len, const int* slots, int tokens, int seqs,
                                          int max_q_len, int max_kv_len, int heads, int kv_heads, int d, int page_size, float scale, int keep_first,
-                                         float* scratch, int* error, void* stream) {
+                                         int least, float* scratch, int* error, void* stream) {
   if (tokens == 0 || seqs == 0 || max_kv_len < 1) return 0;
   if (!pae_attention_mass_prompt_supports(heads, kv_heads, d, page_size))
     return fail(2, "attention_mass: %d heads over %d of head_dim %d with pages of %d are not taken", heads, kv_heads, d, page_size);
@@ -385,6 +385,7 @@ PAE_EXPORT int pae_attention_mass_prompt(void* out, float* mass, const void* qkv
   p.chunk_tiles = tiles_a_chunk(seqs, kv_heads, max_q_len, max_kv_len, p.tile_tokens);
   p.span = max_kv_len;
   p.seqs = seqs;
+  p.least = least;
   p.scale_log2 = scale * LOG2E;
   p.error = error;
   const int chunks = chunk_count(seqs, kv_heads, max_q_len, max_kv_len, p.tile_tokens);

@@ -2637,11 +2637,11 @@ def _decode_mass(out, qkv, keys, operands, mass, block_table, table_width: int, 
 
 
 def _prompt_mass(lib, out, qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, slots, sizes, max_q_len: int, max_kv_len: int, scale: float,
-                 keep_first: int, singles: int, multi_index) -> None:
-    """The requests of a step that bring several tokens: the attention, which leaves the logarithms of the rows' denominators, and the weights."""
+                 keep_first: int, singles: int, multi_index, least: int) -> None:
+    """The requests of a step that bring `least` tokens (1 or 2) and more: the attention, which leaves the logarithms of the rows' denominators, and the weights."""
     num_heads, num_kv_heads, head_dim, page_size = sizes
     tokens, seqs = qkv.shape[0], kv_len.shape[0]
-    listed = multi_index if multi_index is not None and singles > 0 else None
+    listed = multi_index if multi_index is not None and singles > 0 and least > 1 else None
     if listed is not None:
         _need(listed, "paged_attention_mass: multi_index", torch.int32)
         if listed.numel() != seqs - singles:
@@ -2655,25 +2655,28 @@ def _prompt_mass(lib, out, qkv, keys, values, mass, block_table, q_start, q_pos0
     _set_bounds("attention_mass_prompt", keys)
     _check(attention, attention.pae_paged_attention_prefill_tcgen05(
         out.data_ptr(), qkv.data_ptr(), keys.data_ptr(), values.data_ptr(), keys.shape[0], block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(),
-        q_pos0.data_ptr(), kv_len.data_ptr(), tokens, seqs, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, 0, 1, singles, 0, None,
-        _ptr(listed), (listed.numel() if listed is not None else 0), logarithms.data_ptr(), error, _stream()))
+        q_pos0.data_ptr(), kv_len.data_ptr(), tokens, seqs, max_q_len, max_kv_len, num_heads, num_kv_heads, head_dim, page_size, scale, 0, least - 1, singles, 0,
+        None, _ptr(listed), (listed.numel() if listed is not None else 0), logarithms.data_ptr(), error, _stream()))
     for b, count in parts:
         _check(lib, lib.pae_attention_mass_prompt(
             out.data_ptr(), mass.data_ptr(), qkv.data_ptr(), keys.data_ptr(), keys.shape[0], logarithms.data_ptr(), block_table.data_ptr() + 4 * b * block_table.shape[1],
             block_table.shape[1], q_start.data_ptr() + 4 * b, q_pos0.data_ptr() + 4 * b, kv_len.data_ptr() + 4 * b, _ptr(slots), tokens, count, max_q_len, max_kv_len, num_heads,
-            num_kv_heads, head_dim, page_size, scale, keep_first, scratch.data_ptr(), error, _stream()), 2)
+            num_kv_heads, head_dim, page_size, scale, keep_first, least, scratch.data_ptr(), error, _stream()), 2)
 
 
 def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, num_heads: int, num_kv_heads: int, head_dim: int,
                          page_size: int, max_q_len: int, max_kv_len: int, scale: float, keep_first: int = 0, slots=None, num_single=None,
-                         multi_index=None) -> torch.Tensor:
+                         multi_index=None, info: dict | None = None) -> torch.Tensor:
     """`paged_attention` without a window, which also adds up what weight the step's queries gave each key: mass[page, g, place]
     += the sum over the step's tokens that see the key, and over the query heads of kv head g, of the key's softmax weight.
     `mass` is float32 [pages, kv_heads, page_size], in the pages of the keys. A key of this step starts from nothing, whatever its place held
     before. Keys before `keep_first` are left alone (they are not to be evicted): requests may share
     the pages that hold such keys only; every other page belongs to one request of the step. `slots` (int32 [tokens], as
     `qkv_projection` takes them): a request whose first slot is negative only pads the step and adds nothing. `num_single` and
-    `multi_index` as `paged_attention` takes them; rows of `qkv` behind the last request do not matter.
+    `multi_index` as `paged_attention` takes them; rows of `qkv` behind the last request do not matter. `info`, when given, receives what added the weights ("kernel"):
+    "single" (bfloat16 steps of single tokens; head sizes 32, 64 and 128, pages of a multiple of 16 keys, up to 16 query heads a kv head), "few" (up to MASS_FEW_TOKENS
+    tokens a request) or "portions" (beside the former for single tokens among them) with head sizes 64 and 128 and pages of 16, 32, 64 or 128 keys, on
+    tensor cores; "single simt" (up to 16 query heads a kv head) or "rows" for the rest, on CUDA cores.
     A key that came with a step of another attention has no start here: its place still holds what the page's earlier owner left, unless
     `paged_attention_prefix` was given `mass` in that step, or the caller wrote 0 there. What a drafted token gave to the keys before it stays in their sums when
     the token is rejected later; the place of its own key starts anew with the key that takes it."""
@@ -2698,22 +2701,28 @@ def paged_attention_mass(qkv, keys, values, mass, block_table, q_start, q_pos0, 
     singles = num_single if num_single is not None else (seqs if max_q_len == 1 else -1)
     sizes = (num_heads, num_kv_heads, head_dim, page_size)
     if qkv.dtype is torch.bfloat16 and use_tensor_cores:
-        few = None
-        if 1 < max_q_len <= MASS_FEW_TOKENS and _prefix_supports(*sizes):
+        # The slices of single tokens take up to 16 query heads a kv head; where there are more, single tokens are taken as few tokens or short portions are.
+        decode_takes, few = _mass_supports(*sizes), None
+        if (2 if decode_takes else 1) <= max_q_len <= MASS_FEW_TOKENS and _prefix_supports(*sizes):
             few = _few_mass_parts(MASS_SCRATCH_BYTES, tokens, seqs, sizes, max_q_len, max_kv_len)
-        if few or (_mass_supports(*sizes) and (max_q_len == 1 or (use_tcgen05_attention and _prompt_mass_supports(*sizes)))):
+        portions = few is None and (max_q_len > 1 or not decode_takes)
+        if not portions or (use_tcgen05_attention and _prompt_mass_supports(*sizes)):
+            if info is not None:
+                info.update(kernel="few" if few is not None else "portions" if portions else "single")
             out = qkv.new_empty((tokens, num_heads * head_dim))
-            if few:
+            if few is not None:
                 _few_mass(out, qkv, keys, operands, mass, few, pages, block_table, table_width, q_start, q_pos0, kv_len, slots, tokens, seqs, sizes, max_q_len,
                           max_kv_len, scale, keep_first)
                 return out
-            if max_q_len > 1:
+            if portions:
                 _prompt_mass(_lib("attention_mass_prompt"), out, qkv, keys, values, mass, block_table, q_start, q_pos0, kv_len, slots, sizes, max_q_len, max_kv_len,
-                             scale, keep_first, singles, multi_index)
-            if singles != 0:
+                             scale, keep_first, singles, multi_index, 2 if decode_takes else 1)
+            if decode_takes and singles != 0:
                 _decode_mass(out, qkv, keys, operands, mass, block_table, table_width, q_start, kv_len, slots, seqs, sizes, max_kv_len, scale, keep_first,
                              seqs if singles < 0 else singles)
             return out
+    if info is not None:
+        info.update(kernel="single simt" if max_q_len == 1 and num_heads // num_kv_heads <= 16 else "rows")
     if max_q_len == 1 and num_heads // num_kv_heads <= 16:
         lib = _lib("attention_mass")
         out = qkv.new_empty((tokens, num_heads * head_dim))
