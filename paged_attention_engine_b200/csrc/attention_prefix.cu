@@ -69,6 +69,11 @@ struct Params {
   int* error;
 };
 
+enum Bar : int {
+  Q_FULL = 0, O_FULL = 1, S_FULL = 2, P_READY = 4, O_REST = 6,
+  K_FULL = 7, K_EMPTY = K_FULL + KV_STAGES, V_FULL = K_EMPTY + KV_STAGES, V_EMPTY = V_FULL + KV_STAGES, NUM_BARS = V_EMPTY + KV_STAGES
+};
+
 template <int D>
 struct Layout {
   static constexpr int HALVES = D / 64;
@@ -80,15 +85,11 @@ struct Layout {
   static constexpr int K_OFFSET = Q_BYTES;
   static constexpr int V_OFFSET = K_OFFSET + KV_STAGES * KV_BYTES;
   static constexpr int BAR_OFFSET = V_OFFSET + KV_STAGES * KV_BYTES;
-  static constexpr size_t SMEM_BYTES = (size_t)BAR_OFFSET + 256 + 768;     // 768 for the 1024-byte alignment of the tiles: two blocks fit an SM
+  static constexpr size_t SMEM_BYTES = (size_t)BAR_OFFSET + 256 + 1024;    // wherever the block's memory begins, the tiles begin on 1024 bytes
+  static_assert(8 * NUM_BARS + 8 <= 256 && 2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two blocks fit an SM");
   static constexpr int S_COLUMNS = BKEYS;
   static constexpr int O_COLUMN = 2 * S_COLUMNS;
   static constexpr int TMEM_COLUMNS = 256;
-};
-
-enum Bar : int {
-  Q_FULL = 0, O_FULL = 1, S_FULL = 2, P_READY = 4, O_REST = 6,
-  K_FULL = 7, K_EMPTY = K_FULL + KV_STAGES, V_FULL = K_EMPTY + KV_STAGES, V_EMPTY = V_FULL + KV_STAGES, NUM_BARS = V_EMPTY + KV_STAGES
 };
 
 // The pages of a run of keys from `begin` (where a box of rows starts) to `end`, for a converged warp: the table is read 32 boxes at a time, one
