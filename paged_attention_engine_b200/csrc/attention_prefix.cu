@@ -133,9 +133,10 @@ __device__ __forceinline__ OwnSpan own_span(const Params& p, int shared, int kv_
   return s;
 }
 
+// Of a launch that keeps scores: the tokens of a request, and whether they have room in the scratch (they do unless a request before brought more
+// than `max_tokens`).
 __device__ __forceinline__ int tokens_of(const Params& p, int b) { return min(p.q_start[b + 1] - p.q_start[b], p.max_tokens); }
-// Whether a request's tokens have room in the scratch: they do unless a request before brought more than `max_tokens`.
-__device__ __forceinline__ bool in_part(const Params& p, int token0, int tokens) { return p.scores == nullptr || token0 - p.q_start[0] + tokens <= p.part_tokens; }
+__device__ __forceinline__ bool in_part(const Params& p, int token0, int tokens) { return token0 - p.q_start[0] + tokens <= p.part_tokens; }
 
 // What a block works on: rows row0 .. row0 + rows - 1 (token, head of kv head g) behind `first_token`, keys begin .. end - 1 by the table of
 // request b. Row r sees those from `first` on that stand at or before pos0 + its token's index.
@@ -143,7 +144,7 @@ struct Work {
   int b, g, first_token, row0, rows, begin, end, first, pos0, slot;
 };
 constexpr int EVERY_KEY = 1 << 30;       // pos0 of rows behind all keys
-template <int TILE_ROWS>
+template <int TILE_ROWS, bool SCORES>
 __device__ __forceinline__ Work find_work(const Params& p, int index) {
   const int groups = p.heads / p.kv_heads;
   Work w = {0, 0, 0, 0, 0, 0, 0, 0, EVERY_KEY, 0};
@@ -173,8 +174,8 @@ __device__ __forceinline__ Work find_work(const Params& p, int index) {
   w.g = index % p.kv_heads;
   w.b = index / p.kv_heads;
   w.first_token = p.q_start[w.b];
-  const int tokens = tokens_of(p, w.b), shared = p.max_prefix > 0 ? min(p.prefix_len[w.b], p.max_prefix) : 0;
-  if (!in_part(p, w.first_token, tokens)) return w;
+  const int tokens = SCORES ? tokens_of(p, w.b) : p.q_start[w.b + 1] - w.first_token, shared = p.max_prefix > 0 ? min(p.prefix_len[w.b], p.max_prefix) : 0;
+  if (SCORES && !in_part(p, w.first_token, tokens)) return w;
   w.pos0 = p.q_pos0[w.b];
   const OwnSpan span = own_span<TILE_ROWS>(p, shared, p.kv_len[w.b], w.pos0, tokens, groups, row_tile);
   if (span.end <= span.first) return w;
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefix_kernel(const __grid_constan
   volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
   auto bar = [&](int which, int i = 0) { return bars + 8u * (which + i); };
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  const Work work = find_work<ROWS>(p, blockIdx.x);
+  const Work work = find_work<ROWS, SCORES>(p, blockIdx.x);
   const bool working = work.rows > 0 && work.begin < work.end;      // the same in every thread
   const int rows = work.rows, kv_begin = work.begin, kv_end = work.end, g = work.g, groups = p.heads / p.kv_heads;
   const int n_tiles = (kv_end - kv_begin + BKEYS - 1) / BKEYS;
@@ -534,7 +535,7 @@ __global__ void __launch_bounds__(pae_attention::MERGE_WARPS * 32) prefix_merge_
   dependent_launch_trigger();
   extern __shared__ float weights[];          // [slots], then [MERGE_WARPS][D]
   const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
-  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = tokens_of(p, b);
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0;
   const int shared = min(p.prefix_len[b], p.max_prefix), kv_len = p.kv_len[b], pos0 = p.q_pos0[b];
   dependent_launch_wait();
   if (i >= tokens) return;
@@ -604,7 +605,7 @@ template <int D, int DEPTH>
 __global__ void __launch_bounds__(128) prefix_merge_rows_kernel(__nv_bfloat16* __restrict__ out, const Params p) {
   dependent_launch_trigger();
   const int h = blockIdx.x * 4 + (threadIdx.x >> 5), i = blockIdx.y, b = blockIdx.z;
-  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = tokens_of(p, b);
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0;
   const int shared = min(p.prefix_len[b], p.max_prefix), kv_len = p.kv_len[b], pos0 = p.q_pos0[b];
   dependent_launch_wait();
   if (i >= tokens || h >= p.heads) return;
@@ -634,7 +635,7 @@ __global__ void __launch_bounds__(128) mass_merge_kernel(__nv_bfloat16* __restri
   dependent_launch_wait();
   if ((int)blockIdx.x < m.row_blocks) {
     const int index = WARPS ? (int)blockIdx.x * 4 + warp : (int)blockIdx.x, i = index / p.heads, h = index % p.heads;
-    if (i >= tokens || part0 + tokens > p.part_tokens) return;
+    if (i >= tokens || !in_part(p, token0, tokens)) return;
     const int slices = slices_of<ROWS>(p, 0, n, pos0, tokens, i, h % groups);
     const size_t at = ((size_t)(part0 + i) * p.heads + h) * p.slots;
     __nv_bfloat16* to = out + ((size_t)(token0 + i) * p.heads + h) * D;
@@ -644,7 +645,7 @@ __global__ void __launch_bounds__(128) mass_merge_kernel(__nv_bfloat16* __restri
   }
   const int g = ((int)blockIdx.x - m.row_blocks) / m.chunks, key0 = (((int)blockIdx.x - m.row_blocks) % m.chunks) * MASS_CHUNK;
   const int last = min(min(n, pos0 + tokens), p.span), rows = tokens * groups;
-  if (rows <= 0 || part0 + tokens > p.part_tokens || key0 >= last || key0 + MASS_CHUNK <= m.keep_first || (m.slots != nullptr && m.slots[token0] < 0)) return;
+  if (rows <= 0 || !in_part(p, token0, tokens) || key0 >= last || key0 + MASS_CHUNK <= m.keep_first || (m.slots != nullptr && m.slots[token0] < 0)) return;
   const int j0 = key0 + threadIdx.x * 4;
   float w[4] = {0.f, 0.f, 0.f, 0.f};
   for (int first = 0; first < rows; first += MASS_ROWS) {
@@ -723,7 +724,7 @@ __global__ void __launch_bounds__(ANY_THREADS) any_slices_kernel(const AnyOperan
   extern __shared__ __align__(16) float any_smem[];
   __shared__ float weight[BKEYS][ANY_ROWS], top_of[ANY_ROWS], sum_of[ANY_ROWS], shrink_of[ANY_ROWS];
   dependent_launch_prologue();
-  const Work work = find_work<ANY_ROWS>(p, blockIdx.x);
+  const Work work = find_work<ANY_ROWS, false>(p, blockIdx.x);
   if (work.rows <= 0 || work.begin >= work.end) return;
   const int rows = work.rows, groups = p.heads / p.kv_heads, units = x.d / 4, stride = x.d + 4, tid = threadIdx.x;
   float* q = any_smem;                                   // [ANY_ROWS][d]
@@ -862,7 +863,7 @@ template <typename T>
 __global__ void __launch_bounds__(ANY_THREADS) any_merge_kernel(const AnyOperands<T> x, const Params p) {
   dependent_launch_prologue();
   const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
-  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = tokens_of(p, b);
+  const int groups = p.heads / p.kv_heads, token0 = p.q_start[b], tokens = p.q_start[b + 1] - token0;
   if (i >= tokens) return;
   const int slices = slices_of<ANY_ROWS>(p, p.max_prefix > 0 ? min(p.prefix_len[b], p.max_prefix) : 0, p.kv_len[b], p.q_pos0[b], tokens, i, h % groups);
   const size_t row = (size_t)(token0 + i) * p.heads + h, at = row * p.slots;
