@@ -107,3 +107,17 @@ def test_scratch_has_a_bound(ops, monkeypatch, tokens, heads, kv_heads, longest)
         p, o = step.table[b].long()[j // 64], j % 64
         expected = torch.where(j[:, None] >= n - t, 0.0, step.mass[p, :, o].double()) + w.sum(1).view(kv_heads, -1, n).sum(1).T
         assert ((got.cpu()[p, :, o].double() - expected).abs() <= MASS_RTOL * expected + MASS_ATOL).all()
+
+
+@pytest.mark.parametrize("dtype,dim,tokens,padding", [
+    (BF16, 128, [70, 20, 130], 1), (BF16, 64, [300, 17, 1, 40], 1), (BF16, 128, [1, 90, 1], 0), (BF16, 64, [3, 2, 5], 1), (BF16, 128, [16, 16], 1), (F32, 64, [3, 2, 5], 1),
+    (F32, 64, [70, 90, 1], 1), (BF16, 32, [20, 33, 5], 1), (F32, 64, [1, 1, 1], 2), (BF16, 32, [1, 1, 1], 0)])
+def test_requests_that_pad_a_step(ops, dtype, dim, tokens, padding):
+    """Slots of -1, whether such a request brings one token or many, in every kernel: the pages it names keep their weights bit for bit."""
+    step = Step([340, 150, 420, 95][: len(tokens)], tokens, 12, 2, dim, 16, dtype, dim + sum(tokens))
+    named = step.table[padding].clone()
+    slots = torch.cat([torch.full((t,), -1 if b == padding else 5, dtype=torch.int32) for b, t in enumerate(tokens)]).cuda()
+    out, mass = _run(ops, step, slots=slots)
+    _check(step, out, mass, pads=(padding,))
+    named = named[named >= 0].long()
+    assert torch.equal(mass.cpu()[named], step.mass[named])
