@@ -5,7 +5,8 @@
 //                exp(s_thj - max_k s_thk) / sum_k exp(s_thk - max_k s_thk),   s = scale q . k
 //   mass[page(b, j), g, place(b, j)] = (j is a key of this step ? 0 : mass) + w,    j >= keep_first
 //
-// in float32 throughout: scores, maxima, sums, weights. Requests that only pad a step (slot -1) add nothing.
+// in float32 throughout: scores, maxima, sums, weights. (The output of the bfloat16 kernels is paged_attention's: there the probabilities, but not the weights, are
+// rounded to bfloat16 for the second product on tensor cores.) Requests that only pad a step (slot -1) add nothing.
 // No atomics: a key's sum is one thread's, in the order of the rows.
 //
 //   slices, merge   steps of single tokens in bfloat16 (head sizes 32, 64, 128): the sliced decode attention of attention_mma.cuh,
@@ -17,7 +18,7 @@
 //                   of the keys for the output.
 //   stats, columns  every other step: the rows' maxima and sums over runs of keys, then per tile of keys and chunk of rows the
 //                   weights, from scores that are computed again, and the chunks' sums in their order. CUDA cores, any type and head size that is a multiple of 4 up to 256. (Steps of several tokens in
-//                   bfloat16 go to attention_prefix.cu and attention_mass_prompt.cu where those take their sizes.)
+//                   bfloat16, and of more than 16 query heads a kv head, go to attention_prefix.cu and attention_mass_prompt.cu where those take their sizes.)
 #include "attention_mma.cuh"
 
 using namespace pae;

@@ -15,7 +15,7 @@
 // The rows are cut into chunks so that many blocks of nearly one length are there (a causal mask makes late key tiles short); their sums
 // are added in the chunks' order by a second kernel, which writes the mass. Two blocks share an SM. The exponentials, 16 a clock and SM, bound it at 1,024 clocks a
 // tile of 128 x 128, the operands of the MMA in shared memory at 565; three portions of 700 to 1,500 tokens over 1,500 to 2,900 keys, 28
-// heads over 4 of 128, take 97 us beside 123 for the attention, the exponentials' pipe half busy. One thread a key, blocks of 256 keys alone on an SM, and three to
+// heads over 4 of 128, take some 100 us of a pass's 230 (108 alone, with cold caches), the attention the rest, the exponentials' pipe half busy. One thread a key, blocks of 256 keys alone on an SM, and three to
 // five stages of queries took the same time.
 #include <cfloat>
 #include <climits>

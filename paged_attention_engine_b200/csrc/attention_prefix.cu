@@ -892,10 +892,11 @@ struct Cut {
 // Two blocks share an SM (three of the CUDA-core kernel). Own keys are cut into as many slices as fill a wave, of one tile at least and OWN_TILES at most. The shared keys' blocks fill
 // that share of one wave that their tiles are of all tiles (a request's own keys taken as half of the longest's), half of it at least: what is left
 // goes to the own blocks, which wait for memory while the others compute. 64 requests, 8,000 shared and 20 to 700 own keys, 28 heads over 4 of
-// 128, us with the merge: 37.6 with the wave full of shared blocks, 36.2 with three quarters, 33.5 with half; 24 requests of five
-// tokens, 30,011 shared and 100 to 900 own keys, 40 heads over 8: 94.8, 112 and 154. With 4 and 32 tiles at most in place of 12: the former 39.2 and
-// 35.1 (35.1), with 3,000 to 5,000 own keys 153 and 104 (110); the latter 100.4 and 95.8 (97.1); the weights of 48 requests of five tokens over 300 to
-// 6,000 keys, 28 heads over 4, whose slices follow the same rule, 192 and 164 (154).
+// 128, us a pass, captured, with the merge, in turn: 36.8 with the wave full of shared blocks, 36.0 with three quarters, 31.9 with half (32.5 by the rule), with 3,000 to
+// 5,000 own keys 122.6, 120.1 and 113.0 (112.1), 180 requests 71.2, 72.5 and 75.7 (73.2); 24 requests of five tokens, 30,011 shared and 100 to 900 own keys, 40 heads over 8:
+// 100.9, 111.7 and 142.2 (98.8). With 4 and 32 tiles at most in place of 12, in another call: 64 requests 35.4 and 30.3 (30.4), with the longer own keys 146 and 101 (107), 180
+// requests 88.6 and 69.8 (69.8), the 24 of five tokens 99.0 and 94.1 (95.1); the weights of 48 requests of five tokens over 300 to
+// 6,000 keys, 28 heads over 4, whose slices follow the same rule, 193 and 158 (149).
 constexpr int OWN_TILES = 12;
 Cut cut_keys(int seqs, int groups, int heads, int kv_heads, int box, int max_q_len, int max_prefix, int max_own, int max_group_tokens, bool any) {
   const int share = heads / kv_heads, wave = (any ? 3 : 2) * pae_attention::multiprocessors(), rows = any ? ANY_ROWS : ROWS;
@@ -929,8 +930,8 @@ Cut cut_keys(int seqs, int groups, int heads, int kv_heads, int box, int max_q_l
 }
 
 // Whether the merge of so many rows, a warp each, asks for 16 slices of a row at once: the registers leave an SM some 20 warps then, which have to hold all rows.
-// us a pass with 8 and 16 at once: 28 heads of 64 requests (1,792 rows) 32.5 and 30.3; 40 heads of 24 requests of five tokens 92.2 and 93.0, 28 heads of 180
-// requests 54.6 and 56.0. mass_merge_kernel's rows, 4 and 16 at once: 28 heads of 16 requests of up to five tokens 84.5 and 72.1, of 48 148 and 164.
+// us a pass, captured, with 8 and 16 at once: 28 heads of 64 requests (1,792 rows) 32.0 and 30.3; 40 heads of 24 requests of five tokens 95.1 and 95.7, 28 heads of 180
+// requests 69.8 and 70.5. mass_merge_kernel's rows, 4 and 16 at once: 28 heads of 16 requests of up to five tokens 76.5 and 68.1, of 48 of five 149 and 163.
 bool rows_in_flight(long long rows) { return rows <= 16LL * pae_attention::multiprocessors(); }
 
 template <int D>
@@ -941,8 +942,8 @@ int launch(const Params& p, void* out, long long pages, int blocks, int seqs, in
   if (int err = raise_shared_memory(devices, prefix_kernel<D, false>, Layout<D>::SMEM_BYTES, "paged_attention_prefix")) return err;
   launch_kernel(prefix_kernel<D, false>, dim3(blocks), dim3(THREADS), Layout<D>::SMEM_BYTES, s, maps, p);
   if (int err = check_launch("paged_attention_prefix")) return err;
-  // A warp a row where the rows fill the SMs with warps, a block a row below that. 12 heads of 4 requests 8.3 us a pass with warps and 7.7 with blocks,
-  // 28 heads of 64 35.1 and 35.7, 14 heads of 123 18.8 and 19.8; the rows of mass_merge_kernel, 28 heads of 48 requests of five tokens, 154 and 199.
+  // A warp a row where the rows fill the SMs with warps, a block a row below that. us a pass, captured, with warps and with blocks: 12 heads of 4 requests
+  // 7.4 and 7.6, 28 heads of 64 30.4 and 35.1, 14 heads of 123 18.2 and 19.8; the rows of mass_merge_kernel, 28 heads of 48 requests of five tokens, 149 and 201, of 4 38.1 and 39.9.
   const long long rows = (long long)p.heads * max_q_len * seqs;
   if (rows >= 8LL * pae_attention::multiprocessors()) {
     const auto merge = rows_in_flight(rows) ? prefix_merge_rows_kernel<D, 16> : prefix_merge_rows_kernel<D, 8>;

@@ -2517,7 +2517,7 @@ def paged_attention_prefix(qkv, keys, values, block_table, q_start, q_pos0, kv_l
 
 # Up to how many tokens a request of a step of several go by slices of the keys, whose scores are kept until the weights are known; longer portions by the
 # attention of prompts and a second pass over the scores. us a pass, captured, the one and the other: 48 requests of five tokens over 300 to 6,000 keys, 28 heads
-# over 4 of 128, 154 and 431, four requests 39 and 92, 16 of 16 tokens 196 and 195. (Single tokens go by slices of their own, csrc/attention_mass.cu: 77 and 90.)
+# over 4 of 128, 140 and 418, four requests 40 and 96, 16 of 8 tokens 122 and 195, of 16 212 and 190. (Single tokens go by slices of their own, csrc/attention_mass.cu: 79, and 95 as few tokens.)
 MASS_FEW_TOKENS = 16
 
 
